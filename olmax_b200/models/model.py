@@ -20,6 +20,7 @@ from ..nn.lm_head import LMHead, LMHeadConfig
 from ..nn.module import BuildContext, Module
 from ..nn.normalization import NormalizerConfig, RMSNormConfig
 from ..nn.rope import BufferCache
+from ..ops.functional import TokenLogProbs
 from ..parallel import dist_utils
 from ..parallel.mesh import DeviceMesh, MeshResource, get_mesh
 from ..parallel.param_store import FSDPUnit, ParamStore
@@ -204,6 +205,54 @@ class Transformer(Module):
         if self.store.reshard_after_forward and self.store.mesh.shard.size > 1 and not torch.is_grad_enabled():
             head_unit.release()
         return loss, zl
+
+    def _head_input(self, ids: torch.Tensor, cache: Optional[BufferCache], *per_token: Optional[torch.Tensor]):
+        """Hidden states of ids [B, S] in front of the head, and what belongs to every token ([B, S, ...]) as this rank's rows."""
+        x, _ = self._trunk(ids, cache)
+        if self.config.tie_embeddings:
+            self._unit("embedding").gathered()
+        tp = self.mesh.tp
+        rows = []
+        for t in per_token:
+            if t is not None:
+                if t.shape[:2] != ids.shape:
+                    raise ValueError(f"tensor of shape {tuple(t.shape)} does not fit token ids of shape {tuple(ids.shape)}")
+                t = t.flatten(0, 1)
+                t = t.chunk(tp.size)[tp.rank] if tp.size > 1 else t
+            rows.append(t)
+        return (x, *rows)
+
+    def _release_head(self) -> None:
+        if self.store.reshard_after_forward and self.store.mesh.shard.size > 1 and not torch.is_grad_enabled():
+            self._unit("head").release()
+
+    def token_log_probs(self, ids: torch.Tensor, labels: Optional[torch.Tensor] = None, cache: Optional[BufferCache] = None, *,
+                        top_k: int = 0, temperature: float = 1.0, ignore_index: int = -100) -> TokenLogProbs:
+        """
+        Log probability of every label [B, S] (None: none), entropy and ``top_k`` most likely tokens at every position of ids
+        [B, S], without materialising the logits; shaped ``[B, S(, top_k)]``, under tensor parallelism as this rank's
+        rows.  ``log_probs`` and ``entropy`` are differentiable.  With ``top_k`` it is a teacher for :meth:`distillation_loss`.
+        """
+        x, lab = self._head_input(ids, cache, labels)
+        out = self.lm_head.token_log_probs(x, lab, top_k=top_k, temperature=temperature, ignore_index=ignore_index,
+                                           chunk_rows=self.ce_chunk_rows)
+        self._release_head()
+        if self.mesh.tp.size > 1:
+            return out
+        return TokenLogProbs(*(t.view(*ids.shape, *t.shape[1:]) if t is not None else None for t in out))
+
+    def distillation_loss(self, ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor,
+                          cache: Optional[BufferCache] = None, *, weight: float = 1.0, temperature: float = 1.0,
+                          tail: str = "rest") -> torch.Tensor:
+        """
+        ``weight`` times the mean distillation loss of this rank's tokens from a teacher's top classes ``[B, S, k]``
+        (:func:`~olmax_b200.ops.functional.distillation_loss`), fused with the head like the cross entropy of :meth:`forward`.
+        """
+        x, t_ids, t_log_probs = self._head_input(ids, cache, teacher_ids, teacher_log_probs)
+        loss = self.lm_head.distillation_loss(x, t_ids, t_log_probs, weight=weight, temperature=temperature, tail=tail,
+                                              chunk_rows=self.ce_chunk_rows)
+        self._release_head()
+        return loss
 
 
 @dataclass

@@ -1,7 +1,8 @@
 """
 Functional API (``olmax/nn/functional.py``): weight-as-tensor versions of the ops for analysis and tests, evaluated
 with the PyTorch restatement, plus the loss helpers.  Models call the handle-based ops in
-:mod:`olmax_b200.ops.functional`, which dispatch to the CUDA kernels.
+:mod:`olmax_b200.ops.functional`, which dispatch to the CUDA kernels; so do ``token_log_probs`` and ``distillation_loss``, which
+take logits and run the kernels on a GPU.
 """
 
 from __future__ import annotations
@@ -10,11 +11,13 @@ from typing import Callable, Optional, Sequence
 
 import torch
 
+from ..ops.functional import TokenLogProbs, distillation_loss, token_log_probs
 from ..ops.reference import cross_entropy as cross_entropy_loss
 from ..ops.reference import fused_cross_entropy as fused_cross_entropy_loss
 from ..ops.reference import layer_norm, rms_norm
 
-__all__ = ["linear", "layer_norm", "rms_norm", "cross_entropy_loss", "fused_cross_entropy_loss", "scan_module"]
+__all__ = ["linear", "layer_norm", "rms_norm", "cross_entropy_loss", "fused_cross_entropy_loss", "scan_module",
+           "TokenLogProbs", "token_log_probs", "distillation_loss"]
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

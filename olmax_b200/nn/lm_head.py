@@ -68,6 +68,27 @@ class LMHead(Module):
         return F.linear_cross_entropy(x, self._weight, labels, ignore_index, self.logit_softcap or 0.0,
                                       z_loss_multiplier, chunk_rows)
 
+    def _refuse_vocab_parallel(self, what: str) -> None:
+        if self.vocab_parallel:
+            raise OLMaxConfigurationError(f"{what} needs the whole vocabulary on every member of the tensor-parallel group; build the "
+                                          f"head without vocab_parallel")
+
+    def token_log_probs(self, x: torch.Tensor, ids: Optional[torch.Tensor] = None, *, top_k: int = 0, temperature: float = 1.0,
+                        ignore_index: int = -100, chunk_rows: int = 2048) -> F.TokenLogProbs:
+        """Log probabilities of tokens, entropies and top classes of hidden states x ``[..., d]``
+        (:func:`~olmax_b200.ops.functional.linear_token_log_probs`), differentiable with respect to x and the head's weight."""
+        self._refuse_vocab_parallel("token_log_probs")
+        return F.linear_token_log_probs(x, self._weight, ids, top_k=top_k, temperature=temperature, logit_softcap=self.logit_softcap,
+                                        ignore_index=ignore_index, chunk_rows=chunk_rows)
+
+    def distillation_loss(self, x: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, *, weight: float = 1.0,
+                          temperature: float = 1.0, tail: str = "rest", chunk_rows: int = 2048) -> torch.Tensor:
+        """Distillation of a teacher's top classes into hidden states x ``[..., d]``
+        (:func:`~olmax_b200.ops.functional.linear_distillation_loss`)."""
+        self._refuse_vocab_parallel("distillation")
+        return F.linear_distillation_loss(x, self._weight, teacher_ids, teacher_log_probs, weight=weight, temperature=temperature,
+                                          tail=tail, logit_softcap=self.logit_softcap, chunk_rows=chunk_rows)
+
 
 @dataclass
 class LMHeadConfig:

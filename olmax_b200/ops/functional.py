@@ -13,7 +13,7 @@ restatement), which is the path the gloo multi-process tests use.
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.distributed as dist
@@ -25,6 +25,7 @@ from . import reference as ref
 __all__ = [
     "linear", "linears", "gated_mlp", "rms_norm", "layer_norm", "rope", "rope_pair", "attention", "attention_block_fwd", "attention_block_bwd",
     "embedding", "linear_cross_entropy", "glu", "tp_column_linears", "tp_row_linear",
+    "TokenLogProbs", "token_log_probs", "linear_token_log_probs", "distillation_loss", "linear_distillation_loss",
 ]
 
 
@@ -1126,3 +1127,425 @@ def linear_cross_entropy(x: torch.Tensor, handle, labels: torch.Tensor, ignore_i
     """(loss, z_loss) of the LM head fused with the cross entropy; ``handle`` is the ``(vocab, d)`` head weight."""
     return _LinearCrossEntropyFn.apply(x, handle, labels, ignore_index, float(logit_softcap or 0.0),
                                        float(z_loss_multiplier or 0.0), int(chunk_rows))
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# The LM head's distribution: log probabilities of given tokens with entropy and top classes, distillation
+# ----------------------------------------------------------------------------------------------------------------------
+class TokenLogProbs(NamedTuple):
+    """What :func:`token_log_probs` returns, fp32 and shaped like the tokens (``top_*`` with a last dimension of ``top_k``)."""
+
+    log_probs: Optional[torch.Tensor]
+    """log p of the given tokens (0 for a token that is not scored); None without tokens."""
+    entropy: torch.Tensor
+    """-sum p log p of every row."""
+    top_log_probs: Optional[torch.Tensor]
+    """log p of the ``top_k`` largest logits, largest first; None without ``top_k``."""
+    top_ids: Optional[torch.Tensor]
+    """Their classes (int64); equal logits in the order of their classes."""
+
+
+def _distribution_options(V: int, temperature: float, logit_softcap: Optional[float], top_k: int = 0) -> float:
+    if not (0.0 < temperature < math.inf):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    cap = float(logit_softcap or 0.0)
+    if not (0.0 <= cap < math.inf):
+        raise ValueError(f"logit_softcap must be positive and finite (or None), got {logit_softcap}")
+    if V < 1:
+        raise ValueError("logits need at least one class")
+    if not 0 <= top_k <= min(V, K.TOP_K_MAX):
+        raise ValueError(f"top_k must lie between 0 and min(classes, {K.TOP_K_MAX}) = {min(V, K.TOP_K_MAX)}, got {top_k}")
+    return cap
+
+
+def _logit_rows(logits: torch.Tensor) -> torch.Tensor:
+    """logits [..., V] as [rows, V] with contiguous classes (a view wherever the strides allow one)."""
+    if logits.dim() < 1:
+        raise ValueError("logits need a class dimension")
+    allowed = (torch.float32, torch.bfloat16) if logits.is_cuda else (torch.float32, torch.bfloat16, torch.float64)
+    if logits.dtype not in allowed:
+        raise K.KernelError(f"logits must be fp32 or bf16, got {logits.dtype}")
+    z = logits.reshape(math.prod(logits.shape[:-1]), logits.shape[-1])
+    return z if z.stride(-1) == 1 else z.contiguous()
+
+
+def _token_rows(ids: torch.Tensor, shape, device) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"token ids must be int64 or int32, got {ids.dtype}")
+    if tuple(ids.shape) != tuple(shape) or ids.device != device:
+        raise ValueError(f"token ids of shape {tuple(ids.shape)} on {ids.device} do not fit rows of shape {tuple(shape)} on {device}")
+    return ids.reshape(-1).long().contiguous()
+
+
+def _upstream(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """An upstream gradient as fp32 [rows]; one that is a broadcast scalar (the gradient of a sum) stays one."""
+    if g is None:
+        return None
+    g = g.float()
+    if g.dim() and not any(g.stride()):
+        return g.as_strided((g.numel(),), (0,))
+    return g.reshape(-1)
+
+
+class _TokenLogProbsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, ids, top_k, ignore_index, cap, temperature):
+        ctx.set_materialize_grads(False)
+        ctx.options = dict(ignore_index=ignore_index, temperature=temperature)
+        ctx.cap = cap
+        rows = z.shape[0]
+        if z.is_cuda:
+            log_probs = torch.empty(rows, dtype=torch.float32, device=z.device) if ids is not None else None
+            entropy = torch.empty(rows, dtype=torch.float32, device=z.device)
+            lse = torch.empty_like(entropy) if ctx.needs_input_grad[0] else None
+            top = torch.empty((rows, top_k), dtype=torch.float32, device=z.device) if top_k else None
+            top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=z.device) if top_k else None
+            if rows:
+                K.token_log_probs_fwd(z, ids, log_probs, entropy, lse, top, top_ids, softcap=cap, **ctx.options)
+        else:
+            log_probs, entropy, lse, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(z, ids, lse, entropy)
+        ctx.mark_non_differentiable(*(t for t in (top, top_ids) if t is not None))
+        return log_probs, entropy, top, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_log_probs, g_entropy, _top, _ids):
+        if g_log_probs is None and g_entropy is None:
+            return None, None, None, None, None, None
+        z, ids, lse, entropy = ctx.saved_tensors
+        if z.is_cuda:
+            d = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+            if z.shape[0]:
+                K.token_log_probs_bwd(z, ids, lse, entropy, _upstream(g_log_probs), _upstream(g_entropy), d, softcap=ctx.cap,
+                                      **ctx.options)
+        else:
+            d = ref.token_log_probs_bwd(z, ids, g_log_probs, g_entropy, cap=ctx.cap, **ctx.options)
+        return d, None, None, None, None, None
+
+
+def token_log_probs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, *, top_k: int = 0, temperature: float = 1.0,
+                    logit_softcap: Optional[float] = None, ignore_index: int = -100) -> TokenLogProbs:
+    """
+    Scores of tokens under ``p = softmax(y)``, ``y = cap * tanh(logits / cap) / temperature`` (``y = logits / temperature``
+    without ``logit_softcap``), for fp32 or bf16 ``logits [..., V]``:
+
+    * ``log_probs``: log p of ``ids [...]``.  A token equal to ``ignore_index`` or outside ``[0, V)`` is not scored: 0 and
+      no gradient.
+    * ``entropy`` of every row.
+    * ``top_k`` > 0 (at most 128): log p and class of the largest logits, largest first, equal ones in the order of their
+      classes.
+
+    ``log_probs`` and ``entropy`` are differentiable with respect to the logits, the top classes are not.  Masked classes
+    (-inf) have no part; a row without any class has log p = -inf, entropy 0 and gradient 0; NaN in a row gives NaN.
+    """
+    cap = _distribution_options(logits.shape[-1] if logits.dim() else 0, temperature, logit_softcap, top_k)
+    z = _logit_rows(logits)
+    shape = logits.shape[:-1]
+    lab = _token_rows(ids, shape, logits.device) if ids is not None else None
+    log_probs, entropy, top, top_ids = _TokenLogProbsFn.apply(z, lab, int(top_k), int(ignore_index), cap, float(temperature))
+    return TokenLogProbs(log_probs.view(shape) if log_probs is not None else None, entropy.view(shape),
+                         top.view(*shape, top_k) if top_k else None, top_ids.view(*shape, top_k) if top_k else None)
+
+
+def _check_tail(tail: str) -> bool:
+    """True: the teacher's masses are normalised over its classes."""
+    if tail not in ("rest", "renormalize"):
+        raise ValueError(f"tail must be 'rest' or 'renormalize', got {tail!r}")
+    return tail == "renormalize"
+
+
+def _teacher_rows(teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, shape, device):
+    """The teacher's pairs as contiguous [rows, k]: int32 / int64 ids and fp32 values."""
+    if teacher_ids.dtype not in (torch.int64, torch.int32) or not teacher_log_probs.dtype.is_floating_point:
+        raise ValueError(f"a teacher is int64 or int32 ids with floating-point log probabilities, got {teacher_ids.dtype}, "
+                         f"{teacher_log_probs.dtype}")
+    if (teacher_ids.dim() < 1 or teacher_ids.shape != teacher_log_probs.shape or tuple(teacher_ids.shape[:-1]) != tuple(shape)
+            or teacher_ids.device != device or teacher_log_probs.device != device):
+        raise ValueError(f"teacher of shapes {tuple(teacher_ids.shape)} and {tuple(teacher_log_probs.shape)} on {teacher_ids.device} "
+                         f"does not fit rows of shape {tuple(shape)} on {device}")
+    k = teacher_ids.shape[-1]
+    if not 1 <= k <= K.TOP_K_MAX:
+        raise ValueError(f"a teacher names between 1 and {K.TOP_K_MAX} classes, got {k}")
+    rows = math.prod(shape)
+    values = teacher_log_probs.detach()
+    values = values if values.dtype == torch.float64 and not values.is_cuda else values.float()
+    return teacher_ids.reshape(rows, k).contiguous(), values.reshape(rows, k).contiguous()
+
+
+class _DistillationFn(torch.autograd.Function):
+    """Row losses, or their sum / mean over the rows with a teacher."""
+
+    @staticmethod
+    def forward(ctx, z, ids, values, renormalize, cap, temperature, reduction):
+        ctx.options = (renormalize, cap, temperature, reduction)
+        rows, k = ids.shape
+        keep = ctx.needs_input_grad[0]
+        if z.is_cuda:
+            dev = z.device
+            loss = torch.empty(rows, dtype=torch.float32, device=dev)
+            stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+            q = torch.empty((rows, k), dtype=torch.float32, device=dev)
+            total = torch.empty((), dtype=torch.float32, device=dev)
+            inv = torch.empty((), dtype=torch.float32, device=dev)
+            if rows:
+                K.distill_fwd(z, ids, values, loss, stats, q, renormalize=renormalize, softcap=cap, temperature=temperature)
+            if reduction != "none":
+                K.distill_reduce(loss, stats, total, inv, mean=reduction == "mean")
+            if keep:
+                ctx.save_for_backward(z, ids, stats, q, inv)
+            return loss if reduction == "none" else total
+        loss, some = ref.distillation(z, ids, values, renormalize, cap, temperature)
+        inv = 1.0 / some.sum().clamp(min=1).to(loss.dtype) if reduction == "mean" else torch.ones((), dtype=loss.dtype)
+        if keep:
+            ctx.save_for_backward(z, ids, values, inv)
+        return loss if reduction == "none" else loss.sum() * inv
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        renormalize, cap, temperature, reduction = ctx.options
+        if not ctx.needs_input_grad[0]:
+            return (None,) * 7
+        z, ids = ctx.saved_tensors[:2]
+        rows = z.shape[0]
+        if z.is_cuda:
+            stats, q, inv = ctx.saved_tensors[2:]
+            d = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+            g = g.expand(rows) if reduction != "none" else g
+            if rows:
+                K.distill_bwd(z, ids, stats, q, _upstream(g), inv if reduction == "mean" else None, d, softcap=cap,
+                              temperature=temperature)
+        else:
+            values, inv = ctx.saved_tensors[2:]
+            d = ref.distillation_bwd(z, ids, values, g if reduction == "none" else (g * inv).expand(rows), renormalize, cap,
+                                     temperature)
+        return d, None, None, None, None, None, None
+
+
+def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, *,
+                      temperature: float = 1.0, tail: str = "rest", logit_softcap: Optional[float] = None,
+                      reduction: str = "mean") -> torch.Tensor:
+    """
+    Kullback-Leibler divergence of the student's ``p = softmax(y)`` (``y`` as in :func:`token_log_probs`; logits ``[..., V]``, fp32
+    or bf16) from a teacher of which only some classes are kept: ``teacher_ids [..., k]`` and ``teacher_log_probs [..., k]``, what
+    ``token_log_probs(teacher_logits, top_k=k, temperature=temperature)`` gives.
+
+    * ``tail="rest"``: the classes that the teacher does not name are one further class, with what its probabilities leave of one
+      against what the student gives to all of them (no such class where the student has none outside the named ones).
+    * ``tail="renormalize"``: the teacher's masses are ``softmax(teacher_log_probs)`` (any logits will do).
+
+    A pair whose id lies outside ``[0, V)`` is padding, of several pairs with one id the first counts.  A row without a pair
+    (renormalised: without one above -inf) has loss 0 and gradient 0.  ``reduction``: ``mean`` over the rows with a teacher, ``sum``, or
+    ``none`` (a loss per row, fp32).  The gradient goes to the logits alone; a loss at a temperature is usually weighted by its square.
+    """
+    cap = _distribution_options(logits.shape[-1] if logits.dim() else 0, temperature, logit_softcap)
+    renormalize = _check_tail(tail)
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    z = _logit_rows(logits)
+    shape = logits.shape[:-1]
+    ids, values = _teacher_rows(teacher_ids, teacher_log_probs, shape, logits.device)
+    loss = _DistillationFn.apply(z, ids, values, renormalize, cap, float(temperature), reduction)
+    return loss.view(shape) if reduction == "none" else loss
+
+
+class _HeadChunks:
+    """The rows of x [M, d] in chunks, with the logits of each in one fp32 buffer.  The GEMMs take row counts that are multiples of
+    8: the last chunk is filled up with zero rows, which no output and no gradient sees."""
+
+    def __init__(self, x2: torch.Tensor, handle, chunk_rows: int):
+        if chunk_rows < 1:
+            raise ValueError(f"chunk_rows must be positive, got {chunk_rows}")
+        self.x2, self.handle = x2, handle
+        self.M, self.V = x2.shape[0], handle.tp_shape[0]
+        if handle.tp_shape[1] != x2.shape[1]:
+            raise ValueError(f"hidden states of width {x2.shape[1]} do not fit a head of width {handle.tp_shape[1]}")
+        self.step = max(8, min((chunk_rows + 7) // 8 * 8, (self.M + 7) // 8 * 8))
+        self.padded = (self.M + 7) // 8 * 8
+        self.logits = torch.empty((self.step, self.V), dtype=torch.float32, device=x2.device)
+
+    def __iter__(self):
+        """(first row, last row + 1, padded rows of x, logits of the real rows)."""
+        for r0 in range(0, self.M, self.step):
+            r1 = min(self.M, r0 + self.step)
+            xc = self.x2[r0:r1]
+            if (r1 - r0) % 8:
+                xc = torch.cat([xc, xc.new_zeros((-(r1 - r0) % 8, xc.shape[1]))])
+            _gemm_fwd(xc, self.handle, out=self.logits[: xc.shape[0]], epi=K.EPI_F32)
+            yield r0, r1, xc, self.logits[: r1 - r0]
+
+    def gradients(self):
+        """(dlogits buffer, whether its rows are kept for one weight gradient at the end)."""
+        # as in the cross entropy: the store-based reduce-scatter takes one weight gradient per weight
+        single = getattr(self.handle.store, "symm_rs", None) is not None and self.handle.shard_count > 1
+        rows = self.padded if single else self.step
+        return torch.empty((rows, self.V), dtype=torch.bfloat16, device=self.x2.device), single
+
+    def finish(self, dlogits, single):
+        if single:
+            x2 = self.x2
+            if self.padded > self.M:
+                x2 = torch.cat([x2, x2.new_zeros((self.padded - self.M, x2.shape[1]))])
+            _gemm_wgrad(dlogits, x2, self.handle)
+            self.handle.store.reduce_unit_now(self.handle.unit)
+
+    def chunk_gradient(self, dlogits, single, r0, r1, xc, dx):
+        """dx of one chunk from its dlogits rows, and (unless one weight gradient follows) its part of the weight's."""
+        n = xc.shape[0]
+        dl = dlogits[r0 : r0 + n] if single else dlogits[:n]
+        if n == r1 - r0:
+            _gemm_dgrad(dl, self.handle, out=dx[r0:r1])
+        else:
+            dx[r0:r1] = _gemm_dgrad(dl, self.handle)[: r1 - r0]
+        if not single:
+            _gemm_wgrad(dl, xc, self.handle)
+
+    @staticmethod
+    def rows_of(dlogits, single, r0, r1):
+        """Where the gradient of rows r0..r1 goes; the zero rows behind the last one are cleared."""
+        at = r0 if single else 0
+        pad = -(r1 - r0) % 8
+        if pad:
+            dlogits[at + r1 - r0 : at + r1 - r0 + pad].zero_()
+        return dlogits[at : at + r1 - r0]
+
+
+class _LinearTokenLogProbsFn(torch.autograd.Function):
+    """:class:`_TokenLogProbsFn` of ``x @ W^T`` without the logits of more than ``chunk_rows`` rows: they are computed again in the
+    backward pass, which then forms the gradients of x and of the weight chunk by chunk."""
+
+    @staticmethod
+    def forward(ctx, x2, handle, ids, top_k, ignore_index, cap, temperature, chunk_rows):
+        ctx.set_materialize_grads(False)
+        ctx.handle, ctx.chunk_rows = handle, chunk_rows
+        ctx.options = dict(ignore_index=ignore_index, temperature=temperature)
+        ctx.cap = cap
+        keep = bool(ctx.needs_input_grad[0])
+        M = x2.shape[0]
+        if _on_gpu(x2):
+            dev = x2.device
+            log_probs = torch.empty(M, dtype=torch.float32, device=dev) if ids is not None else None
+            entropy = torch.empty(M, dtype=torch.float32, device=dev)
+            lse = torch.empty_like(entropy) if keep else None
+            top = torch.empty((M, top_k), dtype=torch.float32, device=dev) if top_k else None
+            top_ids = torch.empty((M, top_k), dtype=torch.int64, device=dev) if top_k else None
+            for r0, r1, _, z in _HeadChunks(x2, handle, chunk_rows):
+                cut = [t[r0:r1] if t is not None else None for t in (ids, log_probs, entropy, lse, top, top_ids)]
+                K.token_log_probs_fwd(z, *cut, softcap=cap, **ctx.options)
+        else:
+            z = (x2 @ handle.full().t()).float()
+            log_probs, entropy, lse, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
+        if keep:
+            ctx.save_for_backward(x2, ids, lse, entropy)
+        ctx.mark_non_differentiable(*(t for t in (top, top_ids) if t is not None))
+        return log_probs, entropy, top, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_log_probs, g_entropy, _top, _ids):
+        if g_log_probs is None and g_entropy is None:
+            return (None,) * 8
+        x2, ids, lse, entropy = ctx.saved_tensors
+        handle = ctx.handle
+        if _on_gpu(x2):
+            gl, ge = _upstream(g_log_probs), _upstream(g_entropy)
+            chunks = _HeadChunks(x2, handle, ctx.chunk_rows)
+            dlogits, single = chunks.gradients()
+            dx = torch.empty_like(x2)
+            for r0, r1, xc, z in chunks:
+                cut = [t[r0:r1] if t is not None else None for t in (ids, lse, entropy, gl, ge)]
+                K.token_log_probs_bwd(z, *cut, chunks.rows_of(dlogits, single, r0, r1), softcap=ctx.cap, **ctx.options)
+                chunks.chunk_gradient(dlogits, single, r0, r1, xc, dx)
+            chunks.finish(dlogits, single)
+            return dx, None, None, None, None, None, None, None
+        w = handle.full()
+        d = ref.token_log_probs_bwd((x2 @ w.t()).float(), ids, g_log_probs, g_entropy, cap=ctx.cap, **ctx.options)
+        handle.add_grad(d.t() @ x2.float())
+        return (d @ w.float()).to(x2.dtype), None, None, None, None, None, None, None
+
+
+def linear_token_log_probs(x: torch.Tensor, handle, ids: Optional[torch.Tensor] = None, *, top_k: int = 0,
+                           temperature: float = 1.0, logit_softcap: Optional[float] = None, ignore_index: int = -100,
+                           chunk_rows: int = 2048) -> TokenLogProbs:
+    """:func:`token_log_probs` of the LM head ``x @ W^T`` (``handle``: the ``(vocab, d)`` weight, x ``[..., d]``), whose logits exist
+    ``chunk_rows`` rows at a time.  Differentiable with respect to x and the weight (the logits are computed again)."""
+    cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap, top_k)
+    shape = x.shape[:-1]
+    lab = _token_rows(ids, shape, x.device) if ids is not None else None
+    x2 = x.reshape(math.prod(shape), x.shape[-1]).contiguous()
+    log_probs, entropy, top, top_ids = _LinearTokenLogProbsFn.apply(x2, handle, lab, int(top_k), int(ignore_index), cap,
+                                                                    float(temperature), int(chunk_rows))
+    return TokenLogProbs(log_probs.view(shape) if log_probs is not None else None, entropy.view(shape),
+                         top.view(*shape, top_k) if top_k else None, top_ids.view(*shape, top_k) if top_k else None)
+
+
+class _LinearDistillationFn(torch.autograd.Function):
+    """:class:`_DistillationFn` (mean) of ``x @ W^T``.  Like :class:`_LinearCrossEntropyFn` it forms the gradients of x and of the
+    weight in the forward pass, a chunk of rows at a time, so the loss must be back-propagated with a unit gradient;
+    ``weight`` is the factor of this loss in the objective."""
+
+    @staticmethod
+    def forward(ctx, x2, handle, ids, values, weight, renormalize, cap, temperature, chunk_rows):
+        need_grad = bool(ctx.needs_input_grad[0])
+        M, V = x2.shape[0], handle.tp_shape[0]
+        if _on_gpu(x2):
+            dev = x2.device
+            total = torch.empty((), dtype=torch.float32, device=dev)
+            inv = torch.empty((), dtype=torch.float32, device=dev)
+            K.distill_count(ids, values, inv, renormalize=renormalize, V=V)
+            loss = torch.empty(M, dtype=torch.float32, device=dev)
+            stats = torch.empty((M, 4), dtype=torch.float32, device=dev)
+            chunks = _HeadChunks(x2, handle, chunk_rows)
+            q = torch.empty((chunks.step, ids.shape[1]), dtype=torch.float32, device=dev)
+            dx = torch.empty_like(x2) if need_grad else None
+            dlogits, single = chunks.gradients() if need_grad else (None, False)
+            for r0, r1, xc, z in chunks:
+                K.distill_fwd(z, ids[r0:r1], values[r0:r1], loss[r0:r1], stats[r0:r1], q[: r1 - r0], renormalize=renormalize,
+                              softcap=cap, temperature=temperature)
+                if need_grad:
+                    K.distill_bwd(z, ids[r0:r1], stats[r0:r1], q[: r1 - r0], None, inv,
+                                  chunks.rows_of(dlogits, single, r0, r1), scale=weight, softcap=cap, temperature=temperature)
+                    chunks.chunk_gradient(dlogits, single, r0, r1, xc, dx)
+            if need_grad:
+                chunks.finish(dlogits, single)
+            K.distill_reduce(loss, stats, total, None, mean=True)
+            total = total * weight if weight != 1.0 else total
+        else:
+            w = handle.full()
+            z = (x2 @ w.t()).float()
+            row_loss, some = ref.distillation(z, ids, values, renormalize, cap, temperature)
+            inv = 1.0 / some.sum().clamp(min=1).to(row_loss.dtype)
+            total = row_loss.sum() * inv * weight
+            dx = None
+            if need_grad:
+                d = ref.distillation_bwd(z, ids, values, (inv * weight).expand(M), renormalize, cap, temperature)
+                handle.add_grad(d.t() @ x2.float())
+                dx = (d @ w.float()).to(x2.dtype)
+        if need_grad:
+            ctx.save_for_backward(dx)
+        return total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (dx,) = ctx.saved_tensors
+        # g is 1 for loss.backward(); the weight gradient was already accumulated under that assumption
+        return (dx * g.to(dx.dtype),) + (None,) * 8
+
+
+def linear_distillation_loss(x: torch.Tensor, handle, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, *,
+                             weight: float = 1.0, temperature: float = 1.0, tail: str = "rest",
+                             logit_softcap: Optional[float] = None, chunk_rows: int = 2048) -> torch.Tensor:
+    """``weight`` times the mean :func:`distillation_loss` of the LM head ``x @ W^T``, whose logits exist ``chunk_rows`` rows at a
+    time.  As with :func:`linear_cross_entropy` the weight's gradient is accumulated in the forward pass: add the loss to others as
+    it is and scale it with ``weight``."""
+    cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap)
+    renormalize = _check_tail(tail)
+    if not math.isfinite(weight):
+        raise ValueError(f"weight must be finite, got {weight}")
+    shape = x.shape[:-1]
+    ids, values = _teacher_rows(teacher_ids, teacher_log_probs, shape, x.device)
+    x2 = x.reshape(math.prod(shape), x.shape[-1]).contiguous()
+    return _LinearDistillationFn.apply(x2, handle, ids, values, float(weight), renormalize, cap, float(temperature), int(chunk_rows))

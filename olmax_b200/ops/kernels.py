@@ -28,12 +28,14 @@ __all__ = [
     "embed_gather", "embed_scatter", "ce_fwd_bwd", "ce_vp_stats", "ce_vp_grad", "count_valid", "adamw", "sumsq", "clip_coef", "cast_f32_bf16",
     "layernorm_fwd", "layernorm_bwd", "gather_shards", "scatter_add_shards", "allreduce_p2p", "allreduce_multimem",
     "peer_barrier", "peer_signal", "peer_wait", "copy_bytes", "push_copy", "fold_slots_bf16", "reduce_slots",
+    "token_log_probs_fwd", "token_log_probs_bwd", "distill_fwd", "distill_bwd", "distill_reduce", "distill_count", "TOP_K_MAX",
     "launch_count", "reset_launch_count", "pointer_table",
     "timing_enabled", "set_timing", "timed_region", "timing_report", "format_timing",
 ]
 
 EPI_BF16, EPI_F32, EPI_F32_ACC, EPI_F32_RED, EPI_SWIGLU, EPI_GEGLU, EPI_BF16_ACC = range(7)
 SEG_NONE, SEG_A_K, SEG_A_M, SEG_C_N = range(4)
+TOP_K_MAX = 128   # classes per row of the top-class and distillation kernels
 
 _LAUNCHES = 0
 
@@ -77,6 +79,12 @@ register_signature("ob_adamw", [_vp, _vp, _vp, _vp, _vp, _ll, _f, _f, _f, _f, _f
 register_signature("ob_sumsq", [_vp, _ll, _vp, _vp])
 register_signature("ob_clip_coef", [_vp, _f, _f, _vp, _vp])
 register_signature("ob_cast_f32_bf16", [_vp, _vp, _ll, _vp])
+register_signature("ob_token_log_probs_fwd", [_vp, _i, _ll, _vp, _vp, _vp, _vp, _i, _vp, _vp, _ll, _i, _i, _f, _f, _vp])
+register_signature("ob_token_log_probs_bwd", [_vp, _i, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _i, _ll, _ll, _i, _i, _f, _f, _vp])
+register_signature("ob_distill_fwd", [_vp, _i, _ll, _vp, _i, _vp, _ll, _i, _i, _vp, _vp, _vp, _ll, _i, _f, _f, _vp])
+register_signature("ob_distill_bwd", [_vp, _i, _ll, _vp, _i, _ll, _i, _vp, _vp, _vp, _ll, _vp, _f, _vp, _i, _ll, _ll, _i, _f, _f, _vp])
+register_signature("ob_distill_reduce", [_vp, _vp, _ll, _i, _vp, _vp, _vp])
+register_signature("ob_distill_count", [_vp, _i, _vp, _ll, _i, _i, _ll, _i, _vp, _vp])
 register_signature("ob_peer_barrier", [_vp, _i, _i, ctypes.c_uint, _ll, _vp, _vp])
 register_signature("ob_peer_signal", [_vp, _i, _i, ctypes.c_uint, _vp])
 register_signature("ob_peer_wait", [_vp, _i, _i, ctypes.c_uint, _ll, _vp, _vp])
@@ -400,6 +408,100 @@ def ce_vp_grad(logits, labels, dlogits, peer_stats, n_peers, inv_counts, loss_su
     _count()
 
 
+# The kernels over the LM head's distribution (csrc/token_probs.h) take fp32 or bf16 logits [rows, V] with contiguous classes, on
+# any device of the process: the launch runs with the tensors' device current, on its current stream.
+_LOGITS_DTYPE = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _logits_dtype(t: torch.Tensor) -> int:
+    if t.dtype not in _LOGITS_DTYPE or not t.is_cuda or t.stride(-1) != 1:
+        raise KernelError(f"expected CUDA fp32 or bf16 logits with contiguous classes, got {t.dtype} on {t.device} "
+                          f"with strides {tuple(t.stride())}")
+    return _LOGITS_DTYPE[t.dtype]
+
+
+def _on(device: torch.device):
+    """Make ``device`` current for a launch (nothing to do where it is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def token_log_probs_fwd(logits, ids, log_probs, entropy, lse, top_log_probs, top_ids, *, ignore_index=-100, softcap=0.0,
+                        temperature=1.0) -> None:
+    """Any of the outputs but ``entropy`` may be None; the number of top classes is ``top_ids.shape[1]``."""
+    rows, V = logits.shape
+    with _on(logits.device):
+        check(lib().ob_token_log_probs_fwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), _ptr(ids), _ptr(log_probs),
+                                           entropy.data_ptr(), _ptr(lse), 0 if top_ids is None else top_ids.shape[1],
+                                           _ptr(top_log_probs), _ptr(top_ids), rows, V, ignore_index, softcap,
+                                           1.0 / temperature, stream_ptr(logits.device)), "token_log_probs_fwd")
+    _count()
+
+
+def token_log_probs_bwd(logits, ids, lse, entropy, g_log_probs, g_entropy, dlogits, *, ignore_index=-100, softcap=0.0,
+                        temperature=1.0) -> None:
+    """``g_log_probs`` / ``g_entropy``: fp32 [rows] of any stride, or None."""
+    rows, V = logits.shape
+    with _on(logits.device):
+        check(lib().ob_token_log_probs_bwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), _ptr(ids), lse.data_ptr(),
+                                           entropy.data_ptr(), _ptr(g_log_probs), 0 if g_log_probs is None else g_log_probs.stride(0),
+                                           _ptr(g_entropy), 0 if g_entropy is None else g_entropy.stride(0), dlogits.data_ptr(),
+                                           _logits_dtype(dlogits), dlogits.stride(0), rows, V, ignore_index, softcap,
+                                           1.0 / temperature, stream_ptr(logits.device)), "token_log_probs_bwd")
+    _count()
+
+
+def _teacher_ids(t: torch.Tensor) -> int:
+    if t.dtype not in (torch.int32, torch.int64) or t.stride(1) != 1:
+        raise KernelError(f"teacher ids must be int32 or int64 [rows, k] with contiguous rows, got {t.dtype}")
+    return int(t.dtype == torch.int64)
+
+
+def distill_fwd(logits, teacher_ids, teacher_log_probs, row_loss, row_stats, q, *, renormalize, softcap=0.0,
+                temperature=1.0) -> None:
+    """``teacher_ids`` (int32 / int64) and ``teacher_log_probs`` (fp32) [rows, k] with one row stride; row_loss [rows], row_stats
+    [rows, 4] and q [rows, k] are fp32 outputs that :func:`distill_bwd` reads."""
+    rows, V = logits.shape
+    if teacher_log_probs.stride() != teacher_ids.stride() or teacher_log_probs.dtype != torch.float32:
+        raise KernelError("distillation: fp32 teacher values laid out like the teacher's ids are needed")
+    with _on(logits.device):
+        check(lib().ob_distill_fwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), teacher_ids.data_ptr(),
+                                   _teacher_ids(teacher_ids), teacher_log_probs.data_ptr(), teacher_ids.stride(0),
+                                   teacher_ids.shape[1], int(renormalize), row_loss.data_ptr(), row_stats.data_ptr(), q.data_ptr(),
+                                   rows, V, softcap, 1.0 / temperature, stream_ptr(logits.device)), "distill_fwd")
+    _count()
+
+
+def distill_bwd(logits, teacher_ids, row_stats, q, g, inv_count, dlogits, *, scale=1.0, softcap=0.0, temperature=1.0) -> None:
+    """``g``: fp32 [rows] of any stride (0: one value for all rows) or None; ``inv_count``: device scalar or None."""
+    rows, V = logits.shape
+    with _on(logits.device):
+        check(lib().ob_distill_bwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), teacher_ids.data_ptr(),
+                                   _teacher_ids(teacher_ids), teacher_ids.stride(0), teacher_ids.shape[1], row_stats.data_ptr(),
+                                   q.data_ptr(), _ptr(g), 0 if g is None else g.stride(0), _ptr(inv_count), scale,
+                                   dlogits.data_ptr(), _logits_dtype(dlogits), dlogits.stride(0), rows, V, softcap,
+                                   1.0 / temperature, stream_ptr(logits.device)), "distill_bwd")
+    _count()
+
+
+def distill_reduce(row_loss, row_stats, loss, inv_count, *, mean: bool) -> None:
+    """loss = sum (or mean over the rows with a teacher) of ``row_loss``; inv_count (or None) = 1 / max(1, these rows)."""
+    with _on(row_loss.device):
+        check(lib().ob_distill_reduce(row_loss.data_ptr(), row_stats.data_ptr(), row_loss.shape[0], int(mean), loss.data_ptr(),
+                                      _ptr(inv_count), stream_ptr(row_loss.device)), "distill_reduce")
+    _count()
+
+
+def distill_count(teacher_ids, teacher_log_probs, inv_count, *, renormalize, V) -> None:
+    """inv_count = 1 / max(1, rows with a teacher), before the student's logits are there."""
+    with _on(teacher_ids.device):
+        check(lib().ob_distill_count(teacher_ids.data_ptr(), _teacher_ids(teacher_ids), teacher_log_probs.data_ptr(),
+                                     teacher_ids.stride(0), teacher_ids.shape[1], int(renormalize), teacher_ids.shape[0], V,
+                                     inv_count.data_ptr(), stream_ptr(teacher_ids.device)), "distill_count")
+    _count()
+
+
 def count_valid(labels, ignore_index, V, out, counter) -> None:
     check(lib().ob_count_valid(labels.data_ptr(), labels.numel(), ignore_index, V, out.data_ptr(), counter.data_ptr(),
                                stream_ptr(labels.device)), "count_valid")
@@ -594,7 +696,8 @@ def format_timing(report: dict, top: int = 40) -> str:
 
 for _name in ("gemm", "flash_attn_fwd", "flash_attn_bwd", "rmsnorm_fwd", "rmsnorm_bwd", "rmsnorm_rope_fwd",
               "rmsnorm_rope_bwd", "layernorm_fwd", "layernorm_bwd",
-              "rope", "rope_pair", "glu_fwd", "glu_bwd", "embed_gather", "embed_scatter", "ce_fwd_bwd", "ce_vp_stats", "ce_vp_grad", "count_valid",
+              "rope", "rope_pair", "glu_fwd", "glu_bwd", "embed_gather", "embed_scatter", "ce_fwd_bwd", "ce_vp_stats", "ce_vp_grad", "token_log_probs_fwd", "token_log_probs_bwd",
+              "distill_fwd", "distill_bwd", "distill_reduce", "distill_count", "count_valid",
               "adamw", "sumsq",
               "clip_coef", "cast_f32_bf16", "gather_shards", "scatter_add_shards", "allreduce_p2p", "allreduce_multimem",
               "copy_bytes", "push_copy", "fold_slots_bf16", "reduce_slots", "peer_barrier", "peer_signal", "peer_wait"):

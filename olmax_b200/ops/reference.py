@@ -21,7 +21,7 @@ import torch.nn.functional as F
 
 __all__ = [
     "rms_norm", "layer_norm", "rope_tables", "apply_rope", "attention", "glu", "cross_entropy", "fused_cross_entropy",
-    "softcap", "activation",
+    "softcap", "activation", "token_log_probs", "token_log_probs_bwd", "distillation", "distillation_bwd",
 ]
 
 
@@ -177,3 +177,117 @@ def fused_cross_entropy(logits: torch.Tensor, labels: torch.Tensor, ignore_index
     if reduction == "sum":
         return per_tok.sum(), z.sum()
     return per_tok.view(labels.shape), z.view(labels.shape)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# The LM head's distribution p = softmax(y), y = softcap(z) / temperature of logits z [rows, V]
+# ----------------------------------------------------------------------------------------------------------------------
+def _distribution(z: torch.Tensor, cap: float, temperature: float):
+    """(y, dy/dz, lse) in fp32 (fp64 for fp64 logits)."""
+    zf = z if z.dtype == torch.float64 else z.float()
+    slope = torch.full_like(zf, 1.0 / temperature)
+    if cap and cap > 0:
+        t = torch.tanh(zf / cap)
+        zf, slope = cap * t, slope * (1.0 - t * t)
+    y = zf / temperature
+    return y, slope, torch.logsumexp(y, dim=-1)
+
+
+def _log_p(y: torch.Tensor, lse: torch.Tensor) -> torch.Tensor:
+    """log p; a row without any class (lse = -inf) has -inf everywhere."""
+    return y - torch.where(lse == -math.inf, torch.zeros_like(lse), lse).unsqueeze(-1)
+
+
+def token_log_probs(z: torch.Tensor, ids: Optional[torch.Tensor], top_k: int = 0, ignore_index: int = -100, cap: float = 0.0,
+                    temperature: float = 1.0):
+    """(log p of ids or None, entropy, lse, top log p or None, top ids or None) of logits z [rows, V]: the top classes are
+    those with the largest logits, equal ones in the order of their ids."""
+    V = z.shape[-1]
+    y, _, lse = _distribution(z, cap, temperature)
+    lp = _log_p(y, lse)
+    entropy = -torch.where(lp > -math.inf, lp.exp() * lp, torch.where(lp.isnan(), lp, torch.zeros_like(lp))).sum(-1)
+    taken = None
+    if ids is not None:
+        known = (ids != ignore_index) & (ids >= 0) & (ids < V)
+        taken = torch.where(known, lp.gather(-1, ids.clamp(0, V - 1).unsqueeze(-1)).squeeze(-1), torch.zeros_like(lse))
+    if not top_k:
+        return taken, entropy, lse, None, None
+    top_ids = z.sort(dim=-1, descending=True, stable=True).indices[:, :top_k].contiguous()
+    return taken, entropy, lse, lp.gather(-1, top_ids), top_ids
+
+
+def token_log_probs_bwd(z: torch.Tensor, ids: Optional[torch.Tensor], g_log_probs: Optional[torch.Tensor],
+                        g_entropy: Optional[torch.Tensor], ignore_index: int = -100, cap: float = 0.0,
+                        temperature: float = 1.0) -> torch.Tensor:
+    """d(sum g_log_probs log p + sum g_entropy H) / dz = dy/dz (g_lp (onehot - p) - g_H p (log p + H))."""
+    V = z.shape[-1]
+    y, slope, lse = _distribution(z, cap, temperature)
+    lp = _log_p(y, lse)
+    p = lp.exp()
+    d = torch.zeros_like(p)
+    if g_entropy is not None:
+        weighted = torch.where(p > 0, lp, torch.zeros_like(lp))
+        entropy = -(p * weighted).sum(-1, keepdim=True)
+        d = d - g_entropy.to(p.dtype).unsqueeze(-1) * p * torch.where(p > 0, lp + entropy, torch.zeros_like(lp))
+    if g_log_probs is not None:
+        known = (ids != ignore_index) & (ids >= 0) & (ids < V)
+        g = torch.where(known, g_log_probs.to(p.dtype), torch.zeros_like(lse)).unsqueeze(-1)
+        d = (d - g * p).scatter_add(-1, ids.clamp(0, V - 1).unsqueeze(-1), g)
+    return (torch.where((lse == -math.inf).unsqueeze(-1), torch.zeros_like(d), d) * slope).to(z.dtype)
+
+
+def _teacher(teacher_ids: torch.Tensor, values: torch.Tensor, V: int, renormalize: bool):
+    """(valid pairs, their masses, log of these, rows with a teacher): of several pairs with one id the first counts."""
+    ids = teacher_ids.long()
+    first = ~((ids.unsqueeze(-1) == ids.unsqueeze(-2)).tril(-1).any(-1))
+    valid = (ids >= 0) & (ids < V) & first
+    t = torch.where(valid, values.double(), torch.full_like(values, -math.inf, dtype=torch.float64))
+    some = (valid & ~(t == -math.inf)).any(-1) if renormalize else valid.any(-1)
+    log_q = t
+    if renormalize:
+        norm = torch.logsumexp(t, dim=-1, keepdim=True)
+        log_q = t - torch.where(norm == -math.inf, torch.zeros_like(norm), norm)
+    return valid, log_q.exp(), log_q, some
+
+
+def _distillation_parts(z, teacher_ids, values, renormalize, cap, temperature):
+    V = z.shape[-1]
+    y, slope, lse = _distribution(z, cap, temperature)
+    valid, q, log_q, some = _teacher(teacher_ids, values, V, renormalize)
+    at = torch.where(valid, teacher_ids.long(), torch.full_like(teacher_ids, V, dtype=torch.int64))
+    named = torch.zeros(z.shape[0], V + 1, dtype=torch.bool, device=z.device).scatter(-1, at, True)[:, :V]
+    rest_lse = torch.logsumexp(y.masked_fill(named, -math.inf), dim=-1)
+    rest = torch.zeros_like(q[:, 0])
+    if not renormalize:
+        rest = torch.where(rest_lse == -math.inf, rest, (1.0 - q.sum(-1)).clamp(min=0.0))
+    return y, slope, lse, valid, q, log_q, some, at, named, rest_lse, rest
+
+
+def distillation(z: torch.Tensor, teacher_ids: torch.Tensor, values: torch.Tensor, renormalize: bool, cap: float = 0.0,
+                 temperature: float = 1.0):
+    """(loss per row, rows with a teacher) for logits z [rows, V] and a teacher's [rows, k] pairs of class and log probability;
+    see ``ops/functional.py: distillation_loss``."""
+    y, _, lse, valid, q, log_q, some, at, _, rest_lse, rest = _distillation_parts(z, teacher_ids, values, renormalize, cap, temperature)
+    V = z.shape[-1]
+    lp = _log_p(y, lse).gather(-1, at.clamp(max=V - 1)).double()
+    terms = torch.where(valid & ~(q == 0), q * (log_q - lp), torch.zeros_like(q))
+    rest_lp = rest_lse.double() - lse.double()
+    loss = terms.sum(-1) + torch.where(rest > 0, rest * (rest.log() - rest_lp), torch.zeros_like(rest))
+    return torch.where(some, loss, torch.zeros_like(loss)).to(y.dtype), some
+
+
+def distillation_bwd(z: torch.Tensor, teacher_ids: torch.Tensor, values: torch.Tensor, g: torch.Tensor, renormalize: bool,
+                     cap: float = 0.0, temperature: float = 1.0) -> torch.Tensor:
+    """d(sum g loss) / dz: M p - q for the teacher's classes, e^(y - L) (M e^(L - lse) - rest) for the others, whose
+    log-sum-exp is L; M = sum q + rest."""
+    y, slope, lse, valid, q, _, some, at, named, rest_lse, rest = _distillation_parts(z, teacher_ids, values, renormalize, cap, temperature)
+    V = z.shape[-1]
+    total = q.sum(-1) + rest
+    p = _log_p(y, lse).exp()
+    safe = torch.where(rest_lse == -math.inf, torch.zeros_like(rest_lse), rest_lse)
+    coef = torch.where(rest_lse == -math.inf, torch.zeros_like(total), total * (safe - lse).double().exp() - rest).to(y.dtype)
+    others = (y - safe.unsqueeze(-1)).masked_fill(named, -math.inf).exp() * coef.unsqueeze(-1)
+    d = torch.where(named, total.to(y.dtype).unsqueeze(-1) * p, others)
+    d = d.scatter_add(-1, at.clamp(max=V - 1), torch.where(valid, -q, torch.zeros_like(q)).to(y.dtype))
+    alive = (some & (lse != -math.inf)).unsqueeze(-1)
+    return torch.where(alive, d * slope * g.to(y.dtype).unsqueeze(-1), torch.zeros_like(d)).to(z.dtype)

@@ -70,7 +70,8 @@ class Trainer:
     save_folder: PathOrStr
     optim: OptimConfig
     loss_fun: Optional[Callable[[Any, Any, Any], torch.Tensor]] = None
-    """``loss_fun(model, micro_batch, buffer_cache) -> scalar``; default: ``model(ids, labels, cache)[0]``."""
+    """``loss_fun(model, micro_batch, buffer_cache) -> scalar``; default: ``model(ids, labels, cache)[0]`` for a micro-batch of
+    two tensors, ``model.distillation_loss(ids, teacher_ids, teacher_log_probs, cache)`` for one of three."""
     mesh: Optional[MeshResource] = None
     grad_dtype: str = "float32"
     compute_dtype: str = "bfloat16"
@@ -283,6 +284,9 @@ class Trainer:
 
     # ------------------------------------------------------------------ the optimizer step
     def _default_loss(self, model, micro_batch, cache):
+        if len(micro_batch) == 3:
+            ids, teacher_ids, teacher_log_probs = micro_batch
+            return model.distillation_loss(ids, teacher_ids, teacher_log_probs, cache)
         ids, labels = micro_batch
         loss, z = model(ids, labels, cache, z_loss_multiplier=self.z_loss_multiplier)
         return loss
