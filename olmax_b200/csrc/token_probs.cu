@@ -1,7 +1,10 @@
 // The distribution of an LM head: log probabilities of given tokens, entropy and top classes; distillation from a teacher's top
 // classes; the gradients of both with respect to the logits.  See token_probs.h for the definitions.
 //
-// One block per row.  Statistics are kept as (maximum, sum of exponentials) so that a row is read once whatever its range is.
+// Everything here reads long rows of logits and is bound by HBM (a byte of logits costs 1.5 instructions at most if it is to be
+// read at full rate), so that a row is read once per direction: statistics are kept as (maximum, sums of exponentials relative to
+// it), and the top classes are found on the way.  All exponentials and logarithms are to the base 2, of differences t = (z - m) c of capped
+// logits with c = log2(e) / T: the difference is formed before the product, so that the lowest values of a type do not overflow.
 #include "token_probs.h"
 #include "host_common.h"
 
@@ -12,6 +15,7 @@
 namespace ob {
 
 constexpr int TP_THREADS = 512;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 template <class T>
 __device__ __forceinline__ float to_f(T x);
@@ -26,158 +30,459 @@ __device__ __forceinline__ float from_f<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16(x); }
 
-// y(z) and dy/dz.  tanh(u) = 1 - 2 r and 1 - tanh^2(u) = 4 r (1 - r) with r = 1 / (1 + e^2u): two hardware approximations, absolute error of
-// the tanh below 2e-7 (the approximate tanh instruction's 5e-4 would show in every log probability).
+// 2^x by the hardware (relative error 2^-22; 0 at -inf)
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The capped logit cap(z) = softcap * tanh(z / softcap).  tanh(u) = 1 - 2 r and 1 - tanh^2(u) = 4 r (1 - r) with r = 1 / (1 + e^2u): two
+// hardware approximations, absolute error of the tanh below 2e-7 (the approximate tanh instruction's 5e-4 would show in every
+// log probability).
 struct Scaling {
-  float cap, inv_cap, inv_temp;
-  __device__ __forceinline__ float y(float z) const {
-    if (cap > 0.f) z = cap * (1.f - 2.f * __fdividef(1.f, 1.f + __expf(2.f * z * inv_cap)));
-    return z * inv_temp;
+  float cap, inv_cap2;   // inv_cap2 = 2 log2(e) / cap
+  float c;               // log2(e) / T
+  float inv_temp;
+  // cap(z)
+  __device__ __forceinline__ float capped(float z) const {
+    return cap > 0.f ? cap * (1.f - 2.f * __fdividef(1.f, 1.f + exp2_fast(z * inv_cap2))) : z;
   }
-  __device__ __forceinline__ float y(float z, float* slope) const {
+  // cap(z) and dy / dz
+  __device__ __forceinline__ float capped(float z, float* slope) const {
     *slope = inv_temp;
     if (cap > 0.f) {
-      const float r = __fdividef(1.f, 1.f + __expf(2.f * z * inv_cap));
+      const float r = __fdividef(1.f, 1.f + exp2_fast(z * inv_cap2));
       z = cap * (1.f - 2.f * r);
       *slope *= 4.f * r * (1.f - r);
     }
-    return z * inv_temp;
+    return z;
   }
 };
 
-// (maximum, sum e^(y - m), sum e^(y - m) (y - m)): log-sum-exp = m + log s, entropy = log s - w / s
+// Of some classes: their largest capped logit m, s = sum 2^t, w = sum 2^t t with t = (z - m) c.
+// log p = ln 2 (t - log2 s), entropy = ln 2 (log2 s - w / s).
 struct Stats {
   float m, s, w;
 };
 __device__ __forceinline__ Stats empty_stats() { return Stats{-INFINITY, 0.f, 0.f}; }
 // the sums of `a` with respect to the maximum m >= a.m; m = -inf: no class has been seen
-__device__ __forceinline__ Stats shifted(Stats a, float m) {
+__device__ __forceinline__ Stats shifted(Stats a, float m, float c) {
   if (a.m == m || a.s == 0.f) return Stats{m, a.s, a.w};
-  const float d = fmaxf(a.m - m, -FLT_MAX), f = __expf(d);
+  const float d = fmaxf((a.m - m) * c, -FLT_MAX), f = exp2_fast(d);
   return Stats{m, a.s * f, f > 0.f ? (a.w + a.s * d) * f : 0.f};
 }
-__device__ __forceinline__ Stats combine(Stats a, Stats b) {
+__device__ __forceinline__ Stats combine(Stats a, Stats b, float c) {
   const float m = fmaxf(a.m, b.m);
-  a = shifted(a, m);
-  b = shifted(b, m);
+  a = shifted(a, m, c);
+  b = shifted(b, m, c);
   return Stats{m, a.s + b.s, a.w + b.w};
 }
-// a class that is masked (-inf) adds nothing, not a product of 0 and infinity
-__device__ __forceinline__ void add_class(Stats& a, float y) {
-  if (y > a.m) a = shifted(a, y);
-  const float d = fmaxf(y - (a.m == -INFINITY ? 0.f : a.m), -FLT_MAX), e = y == y ? __expf(d) : y;
-  a.s += e;
-  a.w += e * d;
+__device__ __forceinline__ bool no_class(Stats a) { return a.m == -INFINITY && a.s == 0.f; }   // (a NaN makes the sum NaN)
+
+// Adds E classes whose capped logits are f: their maximum first, then exponentials that do not wait for one another.  A masked
+// class (-inf) adds nothing: its exponent is kept finite where 0 * infinity would come up.
+template <bool W, int E>
+__device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], float c) {
+  float mx = f[0];
+#pragma unroll
+  for (int j = 1; j < E; ++j) mx = fmaxf(mx, f[j]);
+  if (mx > a.m) a = shifted(a, mx, c);
+  const float ref = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const float t = (f[j] - ref) * c, e = exp2_fast(t);
+    a.s += e;
+    if (W) a.w = fmaf(e, fmaxf(t, -FLT_MAX), a.w);
+  }
 }
 
-__device__ __forceinline__ Stats block_combine(Stats a, Stats* red) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1)
+__device__ __forceinline__ Stats shuffle_combine(Stats a, int first, float c) {
+  for (int off = first; off > 0; off >>= 1)
     a = combine(a, Stats{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.s, off),
-                         __shfl_xor_sync(0xffffffffu, a.w, off)});
+                         __shfl_xor_sync(0xffffffffu, a.w, off)}, c);
+  return a;
+}
+__device__ __forceinline__ Stats block_combine(Stats a, Stats* red, float c) {
+  a = shuffle_combine(a, 16, c);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
   __syncthreads();
-  a = red[0];
-  for (int i = 1; i < (int)blockDim.x / 32; ++i) a = combine(a, red[i]);
-  return a;
+  return shuffle_combine(red[threadIdx.x & 15], 8, c);
+}
+static_assert(TP_THREADS == 512, "block_combine joins 16 warps");
+
+// A row as 16-byte vectors between a head and a tail of single classes: rows start at any multiple of the element size.
+template <class T>
+struct Row {
+  static constexpr int N = 16 / sizeof(T);
+  const T* z;
+  int head, nvec, tail;   // classes, vectors, classes
+  __device__ __forceinline__ Row(const T* row, int V) : z(row) {
+    const int lead = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+    head = min(V, lead);
+    nvec = (V - head) / N;
+    tail = V - head - nvec * N;
+  }
+  __device__ __forceinline__ int class_of(int vec) const { return head + vec * N; }
+  __device__ __forceinline__ uint4 load(int vec) const { return reinterpret_cast<const uint4*>(z + head)[vec]; }
+  // the single class of thread t in the head (t < head) or the tail, or -1
+  __device__ __forceinline__ int single(int t, bool first, bool last) const {
+    if (t < N) return first && t < head ? t : -1;
+    t -= N;
+    return last && t < tail ? head + nvec * N + t : -1;
+  }
+};
+template <class T>
+__device__ __forceinline__ void unpack(uint4 v, float* f);
+template <>
+__device__ __forceinline__ void unpack<float>(uint4 v, float* f) {
+  f[0] = __uint_as_float(v.x);
+  f[1] = __uint_as_float(v.y);
+  f[2] = __uint_as_float(v.z);
+  f[3] = __uint_as_float(v.w);
+}
+template <>
+__device__ __forceinline__ void unpack<bf16>(uint4 v, float* f) {
+  const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(u[i] << 16);
+    f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+// sixteen bytes of -inf: classes that are not there
+template <class T>
+__device__ __forceinline__ uint4 no_vector() {
+  const unsigned u = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+  return make_uint4(u, u, u, u);
 }
 
-// Order of the classes: larger logits first (NaN before all, -0 equal to 0), then lower classes.
+// ---------------------------------------------------------------------------------------------------------------------
+// Top classes.  Order of the classes: larger logits first (NaN before all, -0 equal to 0), then lower classes.
+// ---------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned order_key(float z) {
   if (z != z) return 0xffffffffu;
   const unsigned u = __float_as_uint(z + 0.f);
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ float key_logit(unsigned key) {
+  return key == 0xffffffffu ? NAN : __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+}
+// Every class has a key above 0.
+
+// A row's (or slice's) candidates in shared memory.  A class enters if it does not come after (cut_key, cut_class); `n` have.
+// A batch of the row adds at most BATCH of them; before it there are at most KEEP.
+template <int BATCH>
+struct Candidates {
+  static constexpr int KEEP = 1024;
+  static constexpr int SIZE = KEEP + BATCH;
+  unsigned key[SIZE];
+  int cls[SIZE];
+  int n, kept;
+  int red[2][TP_THREADS / 32];
+};
 
 __device__ __forceinline__ int block_sum(int c, int* red) {
   c = __reduce_add_sync(0xffffffffu, c);
-  __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = c;
   __syncthreads();
-  int t = 0;
-  for (int i = 0; i < (int)blockDim.x / 32; ++i) t += red[i];
-  return t;
+  return __reduce_add_sync(0xffffffffu, (threadIdx.x & 31) < TP_THREADS / 32 ? red[threadIdx.x & 31] : 0);
 }
 
-template <class T>
-__global__ void __launch_bounds__(TP_THREADS)
-    token_log_probs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ ids,
-                               float* __restrict__ log_probs, float* __restrict__ entropy, float* __restrict__ lse_out,
-                               int top_k, float* __restrict__ top_log_probs, long long* __restrict__ top_ids, int V,
-                               int ignore_index, Scaling sc) {
-  __shared__ Stats red[TP_THREADS / 32];
-  __shared__ int redi[TP_THREADS / 32];
-  __shared__ unsigned keys[OB_TOP_K_MAX];
-  __shared__ int idx[OB_TOP_K_MAX];
-  __shared__ int found;
-  const long long row = blockIdx.x;
-  const T* z = logits + row * ld;
-  Stats a = empty_stats();
-  for (int i = threadIdx.x; i < V; i += TP_THREADS) add_class(a, sc.y(to_f(z[i])));
-  a = block_combine(a, red);
-  const float log_s = logf(a.s);
-  const bool none = a.m == -INFINITY && a.s == 0.f;   // (a NaN makes the sum NaN)
-  auto log_p = [&](float y) { return y == -INFINITY ? (log_s == log_s ? y : log_s) : (y - a.m) - log_s; };
-  if (threadIdx.x == 0) {
-    if (log_probs != nullptr) {
-      const long long id = ids[row];
-      log_probs[row] = id != (long long)ignore_index && id >= 0 && id < V ? log_p(sc.y(to_f(z[id]))) : 0.f;
+// Drops candidates that are certainly not among the first k of the n there are, and lowers the cut to what is kept: the k-th largest
+// key is searched bit by bit, 16 bits first, which leaves little more than k unless many logits are nearly equal; then the
+// other bits, then classes.  At most `most` (>= k) are kept.  All threads call it; it begins and ends with the block in step.
+template <class C>
+__device__ void compact(C& c, int n, int k, int most, unsigned& cut_key, int& cut_class) {
+  int turn = 0;
+  auto count = [&](auto pred) {
+    int x = 0;
+    for (int i = threadIdx.x; i < n; i += TP_THREADS) x += pred(c.key[i], c.cls[i]);
+    turn ^= 1;   // (two buffers: a thread is at most one sum ahead of the slowest reader)
+    return block_sum(x, c.red[turn]);
+  };
+  unsigned key = 0;
+  int stays = n;
+  for (int bit = 31; bit >= 0 && stays > k; --bit) {
+    if (bit == 15 && stays <= most) break;
+    const unsigned next = key | (1u << bit);
+    const int x = count([&](unsigned q, int) { return q >= next; });
+    if (x >= k) key = next, stays = x;
+  }
+  int cls = INT_MAX;
+  if (stays > most) {
+    // every bit of the key is fixed: more than `most` classes at or above it, so ties at it
+    const int above = count([&](unsigned q, int) { return q > key; });
+    int low = 0;   // fewer than k - above classes of that key lie below `low`
+    for (int bit = 30; bit >= 0; --bit) {
+      const int next = low | (1 << bit);
+      if (count([&](unsigned q, int i) { return q == key && i < next; }) < k - above) low = next;
     }
-    if (entropy != nullptr) entropy[row] = none ? 0.f : log_s - a.w / a.s;
-    if (lse_out != nullptr) lse_out[row] = none ? -INFINITY : a.m + log_s;
-    found = 0;
-  }
-  if (top_k <= 0) return;
-  // the top_k-th largest key, by bits
-  unsigned cut = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const unsigned c = cut | (1u << bit);
-    int n = 0;
-    for (int i = threadIdx.x; i < V; i += TP_THREADS) n += order_key(to_f(z[i])) >= c;
-    if (block_sum(n, redi) >= top_k) cut = c;
-  }
-  int n = 0;
-  for (int i = threadIdx.x; i < V; i += TP_THREADS) n += order_key(to_f(z[i])) > cut;
-  const int equal = top_k - block_sum(n, redi);
-  // the lowest class up to which `equal` classes have that key
-  int last = 0;
-  for (int bit = 30; bit >= 0; --bit) {
-    const int c = last | (1 << bit);   // classes below c
-    n = 0;
-    for (int i = threadIdx.x; i < V && i < c; i += TP_THREADS) n += order_key(to_f(z[i])) == cut;
-    if (block_sum(n, redi) < equal) last = c;
-  }
-  for (int i = threadIdx.x; i < V; i += TP_THREADS) {
-    const unsigned key = order_key(to_f(z[i]));
-    if (key > cut || (key == cut && i <= last)) {
-      const int at = atomicAdd(&found, 1);
-      keys[at] = key;
-      idx[at] = i;
-    }
+    cls = low;
   }
   __syncthreads();
-  if (threadIdx.x < top_k) {
-    const unsigned key = keys[threadIdx.x];
-    const int i = idx[threadIdx.x];
-    int rank = 0;
-    for (int j = 0; j < top_k; ++j) rank += keys[j] > key || (keys[j] == key && idx[j] < i);
-    top_log_probs[row * top_k + rank] = log_p(sc.y(to_f(z[i])));
-    top_ids[row * top_k + rank] = i;
+  if (threadIdx.x == 0) c.kept = 0;
+  // in place: a candidate moves to where an earlier chunk, or its own, has been read
+  for (int i0 = 0; i0 < n; i0 += TP_THREADS) {
+    const int i = i0 + threadIdx.x;
+    const unsigned q = i < n ? c.key[i] : 0u;
+    const int j = i < n ? c.cls[i] : INT_MAX;
+    __syncthreads();
+    if (i < n && (q > key || (q == key && j <= cls))) {
+      const int at = atomicAdd(&c.kept, 1);
+      c.key[at] = q;
+      c.cls[at] = j;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) c.n = c.kept;
+  if (key > cut_key || (key == cut_key && cls < cut_class)) cut_key = key, cut_class = cls;
+  __syncthreads();
+}
+
+// A lower bound of the k-th largest of one key per thread (0: none), exact in its upper 16 bits.
+__device__ __forceinline__ unsigned kth_of_threads(unsigned key, int k) {
+  unsigned cut = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 16; --bit) {
+    const unsigned next = cut | (1u << bit);
+    if (__syncthreads_count(key >= next) >= k) cut = next;
+  }
+  return cut;
+}
+
+struct ScoreArgs {
+  const long long* ids;
+  float *log_probs, *entropy, *norm;
+  int top_k;
+  float* top_log_probs;
+  long long* top_ids;
+  int V, ignore_index;
+  Scaling sc;
+};
+
+// What the CTAs of a row's cluster leave with the first one.
+struct Slices {
+  Stats stats[8];
+  unsigned key[8][OB_TOP_K_MAX];
+  int cls[8][OB_TOP_K_MAX];
+};
+
+// (forms that do not ask for a converged warp)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void store_cluster(uint32_t addr, float x) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(x) : "memory");
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, unsigned x) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
+}
+
+// Log probabilities, entropy and top classes.  A row belongs to a cluster of C CTAs (C = 1 but for few rows), a slice of its vectors to
+// each; the first CTA joins the slices' statistics and candidates through distributed shared memory.  Every thread has U 16-byte
+// loads in flight and takes the maximum of the batch before its exponentials.
+// Top classes in the same pass: from the first batch on, a class is a candidate if it is not below the k-th largest of the threads'
+// maxima over the first batch (a lower bound of the row's k-th largest logit that some k to 1.2 k classes of the batch reach); when
+// 1024 candidates have come together they are cut down, which raises the bound.  Most batches of a thread end at one comparison.
+template <class T, int U, bool CAP, bool TOP>
+__global__ void __launch_bounds__(TP_THREADS, 3)
+    token_log_probs_fwd_kernel(const T* __restrict__ logits, long long ld, int C, ScoreArgs p) {
+  constexpr int N = Row<T>::N, E = U * N;
+  typedef Candidates<TP_THREADS * E + 2 * N> Cand;
+  extern __shared__ __align__(16) char shared_bytes[];
+  Cand& cand = *reinterpret_cast<Cand*>(shared_bytes);
+  __shared__ Stats red[TP_THREADS / 32];
+  __shared__ Slices slices;
+  if (C > 1) cluster_arrive();
+  const long long row = blockIdx.x / (unsigned)C;
+  const int part = (int)(blockIdx.x - row * C);
+  const Row<T> r(logits + row * ld, p.V);
+  const int v0 = (int)((long long)r.nvec * part / C), v1 = (int)((long long)r.nvec * (part + 1) / C);
+  float taken = 0.f;
+  bool known = false;
+  if (part == 0 && threadIdx.x == 0 && p.log_probs != nullptr) {
+    const long long id = p.ids[row];
+    known = id != (long long)p.ignore_index && id >= 0 && id < p.V;
+    if (known) taken = to_f(r.z[id]);
+  }
+  Stats a = empty_stats();
+  unsigned cut_key = 0;
+  int cut_class = INT_MAX;
+  if (TOP && threadIdx.x == 0) cand.n = 0;
+  const int single = r.single(threadIdx.x, part == 0, part == C - 1);
+  const float single_z = single >= 0 ? to_f(r.z[single]) : -INFINITY;
+  if (single >= 0) {
+    const float f[1] = {CAP ? p.sc.capped(single_z) : single_z};
+    add_classes<true, 1>(a, f, p.sc.c);
+  }
+  for (int b = v0; b < v1 || (TOP && b == v0); b += TP_THREADS * U) {
+    uint4 v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = b + k * TP_THREADS + threadIdx.x;
+      v[k] = i < v1 ? r.load(i) : no_vector<T>();
+    }
+    float f[E];
+#pragma unroll
+    for (int k = 0; k < U; ++k) unpack<T>(v[k], f + k * N);
+    float mx = -INFINITY;
+    if (TOP) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) mx = fmaxf(mx, f[j]);
+    }
+    if (CAP) {
+      float y[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) y[j] = p.sc.capped(f[j]);
+      // (what is not there would come out as the lowest capped logit)
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (b + k * TP_THREADS + (int)threadIdx.x >= v1) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) y[k * N + j] = -INFINITY;
+        }
+      add_classes<true, E>(a, y, p.sc.c);
+    } else {
+      add_classes<true, E>(a, f, p.sc.c);
+    }
+    if (TOP) {
+      const bool some = b + (int)threadIdx.x < v1;
+      const bool nan = a.s != a.s;   // a NaN, in this batch or before, comes first but is no maximum
+      if (b == v0) {
+        unsigned best = some ? order_key(mx) : 0u;
+        if (nan) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) best = max(best, f[j] != f[j] ? 0xffffffffu : 0u);
+        }
+        if (single >= 0) best = max(best, order_key(single_z));
+        cut_key = kth_of_threads(best, p.top_k);
+      }
+      int end = 0;
+      auto enter = [&](auto&& each) {   // each(visit): visit(logit, class) for every class there is
+        int add = 0;
+        each([&](float z, int i) {
+          const unsigned key = order_key(z);
+          add += key > cut_key || (key == cut_key && i <= cut_class);
+        });
+        if (add == 0) return;
+        int at = atomicAdd(&cand.n, add);
+        end = at + add;
+        each([&](float z, int i) {
+          const unsigned key = order_key(z);
+          if (key > cut_key || (key == cut_key && i <= cut_class)) {
+            cand.key[at] = key;
+            cand.cls[at] = i;
+            ++at;
+          }
+        });
+      };
+      if (some && (nan || order_key(mx) >= cut_key))
+        enter([&](auto visit) {
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            const int i = b + k * TP_THREADS + threadIdx.x;
+            if (i < v1) {
+#pragma unroll
+              for (int j = 0; j < N; ++j) visit(f[k * N + j], r.class_of(i) + j);
+            }
+          }
+        });
+      if (b == v0 && single >= 0) enter([&](auto visit) { visit(single_z, single); });
+      // (every thread's last candidate, not the counter: a faster thread may already be adding to that)
+      if (__syncthreads_or(end > Cand::KEEP)) compact(cand, cand.n, p.top_k, Cand::KEEP / 2, cut_key, cut_class);
+    }
+  }
+  a = block_combine(a, red, p.sc.c);
+  if (C > 1) cluster_wait();   // the first CTA runs
+  if (TOP) {
+    // the slice's first k classes in order
+    int n = cand.n;
+    __syncthreads();
+    if (n > TP_THREADS / 2) {
+      compact(cand, n, p.top_k, TP_THREADS, cut_key, cut_class);
+      n = cand.n;
+    }
+    uint32_t keys = smem_u32(slices.key[part]), classes = smem_u32(slices.cls[part]);
+    if (C > 1) {
+      keys = mapa_shared(keys, 0);
+      classes = mapa_shared(classes, 0);
+    }
+    for (int t = threadIdx.x; t < n; t += TP_THREADS) {
+      const unsigned key = cand.key[t];
+      const int i = cand.cls[t];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += cand.key[j] > key || (cand.key[j] == key && cand.cls[j] < i);
+      if (rank < p.top_k) {
+        store_cluster(keys + rank * 4, key);
+        store_cluster(classes + rank * 4, (unsigned)i);
+      }
+    }
+    for (int t = n + threadIdx.x; t < p.top_k; t += TP_THREADS) store_cluster(keys + t * 4, 0u);
+  }
+  if (C > 1) {
+    if (threadIdx.x == 0) {
+      const uint32_t at = mapa_shared(smem_u32(&slices.stats[part]), 0);
+      store_cluster(at, a.m);
+      store_cluster(at + 4, a.s);
+      store_cluster(at + 8, a.w);
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (part != 0) return;
+    a = slices.stats[0];
+    for (int i = 1; i < C; ++i) a = combine(a, slices.stats[i], p.sc.c);
+  } else if (TOP) {
+    __syncthreads();
+  }
+  const float log_s = log2f(a.s);
+  auto log_p = [&](float z) {
+    const float y = CAP ? p.sc.capped(z) : z;
+    return y == -INFINITY ? (log_s == log_s ? y : log_s) : LN2 * ((y - a.m) * p.sc.c - log_s);
+  };
+  if (threadIdx.x == 0) {
+    if (p.log_probs != nullptr) p.log_probs[row] = known ? log_p(taken) : 0.f;
+    if (p.entropy != nullptr) p.entropy[row] = no_class(a) ? 0.f : LN2 * (log_s - a.w / a.s);
+    if (p.norm != nullptr) *reinterpret_cast<float2*>(p.norm + row * 2) = make_float2(a.m, log_s);
+  }
+  if (TOP) {
+    // the place of a class among all slices: its own in its list and, of every other, the number of classes before it
+    for (int t = threadIdx.x; t < C * p.top_k; t += TP_THREADS) {
+      const int own = t / p.top_k;
+      int rank = t - own * p.top_k;
+      const unsigned key = slices.key[own][rank];
+      if (key == 0) continue;
+      const int i = slices.cls[own][rank];
+      for (int s = 0; s < C; ++s) {
+        if (s == own) continue;
+        int lo = 0, hi = p.top_k;   // classes [0, lo) of the list come before, [hi, k) after
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          const unsigned q = slices.key[s][mid];
+          if (q > key || (q == key && q != 0 && slices.cls[s][mid] < i)) lo = mid + 1;
+          else hi = mid;
+        }
+        rank += lo;
+      }
+      if (rank < p.top_k) {
+        p.top_log_probs[row * p.top_k + rank] = log_p(key_logit(key));
+        p.top_ids[row * p.top_k + rank] = i;
+      }
+    }
   }
 }
 
 template <class T, class D>
 __global__ void __launch_bounds__(TP_THREADS)
     token_log_probs_bwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ ids,
-                               const float* __restrict__ lse_in, const float* __restrict__ entropy,
+                               const float2* __restrict__ norm, const float* __restrict__ entropy,
                                const float* __restrict__ g_log_probs, long long stride_lp,
                                const float* __restrict__ g_entropy, long long stride_ent, D* __restrict__ dlogits,
                                long long ld_d, int V, int ignore_index, Scaling sc) {
   const long long row = blockIdx.x;
   const T* z = logits + row * ld;
   D* d = dlogits + row * ld_d;
-  const float lse = lse_in[row];
+  const float2 lse = norm[row];
   const float ge = g_entropy != nullptr ? g_entropy[row * stride_ent] : 0.f;
   float gl = 0.f;
   long long id = -1;
@@ -186,13 +491,12 @@ __global__ void __launch_bounds__(TP_THREADS)
     if (id != (long long)ignore_index && id >= 0 && id < V) gl = g_log_probs[row * stride_lp];
     else id = -1;
   }
-  const bool none = lse == -INFINITY;
+  const bool none = lse.x == -INFINITY && lse.y == -INFINITY;
   const float h = entropy != nullptr ? entropy[row] : 0.f;
   for (int i = threadIdx.x; i < V; i += TP_THREADS) {
     float slope;
-    const float y = sc.y(to_f(z[i]), &slope);
-    const float lp = y - lse, p = __expf(lp);
-    float g = -p * (gl + ge * (p > 0.f ? lp + h : 0.f));
+    const float lp = (sc.capped(to_f(z[i]), &slope) - lse.x) * sc.c - lse.y, p = exp2_fast(lp);
+    float g = -p * (gl + ge * (p > 0.f ? fmaf(lp, LN2, h) : 0.f));
     if (i == id) g += gl;
     d[i] = from_f<D>(none ? 0.f : g * slope);
   }
@@ -240,8 +544,11 @@ __global__ void __launch_bounds__(TP_THREADS)
   if (threadIdx.x < k && !counts) id_s[threadIdx.x] = -1;
   Stats a = empty_stats();
   for (int i = threadIdx.x; i < V; i += TP_THREADS)
-    if (!((named[i >> 5] >> (i & 31)) & 1)) add_class(a, sc.y(to_f(z[i])));
-  a = block_combine(a, red);
+    if (!((named[i >> 5] >> (i & 31)) & 1)) {
+      const float f[1] = {sc.capped(to_f(z[i]))};
+      add_classes<false, 1>(a, f, sc.c);
+    }
+  a = block_combine(a, red, sc.c);
   if (threadIdx.x >= 32) return;
   // the first warp: up to four of the teacher's pairs per lane
   constexpr int N = OB_TOP_K_MAX / 32;
@@ -255,23 +562,21 @@ __global__ void __launch_bounds__(TP_THREADS)
     const int i = n * 32 + threadIdx.x;
     in[n] = i < k && id_s[i] >= 0;
     t[n] = in[n] ? teacher_log_probs[row * ld_t + i] : -INFINITY;
-    y[n] = in[n] ? sc.y(to_f(z[id_s[i]])) : -INFINITY;
-    if (in[n]) add_class(st, y[n]);
+    const float f[1] = {in[n] ? sc.capped(to_f(z[id_s[i]])) : -INFINITY};
+    y[n] = f[0];
+    if (in[n]) add_classes<false, 1>(st, f, sc.c);
     t_max = fmaxf(t_max, t[n]);
     any |= in[n] && !(renormalize && t[n] == -INFINITY);
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
-    st = combine(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, off), __shfl_xor_sync(0xffffffffu, st.s, off),
-                           __shfl_xor_sync(0xffffffffu, st.w, off)});
     t_max = fmaxf(t_max, __shfl_xor_sync(0xffffffffu, t_max, off));
   }
   any = __any_sync(0xffffffffu, any);
-  const Stats all = combine(st, a);
-  const bool none = all.m == -INFINITY && all.s == 0.f;
-  const float lse = none ? -INFINITY : all.m + logf(all.s);
-  const bool others = !(a.m == -INFINITY && a.s == 0.f);
-  const float rest_lse = others ? a.m + logf(a.s) : -INFINITY;
+  const Stats all = combine(shuffle_combine(st, 16, sc.c), a, sc.c);
+  const bool others = !no_class(a);
+  const float log_s = log2f(all.s), rest_log_s = log2f(a.s);
+  const double ln2 = 0.69314718055994530942;
   const double shift = renormalize && t_max > -INFINITY ? (double)t_max : 0.0;
   double q[N], sum = 0.0;
 #pragma unroll
@@ -291,19 +596,20 @@ __global__ void __launch_bounds__(TP_THREADS)
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     if (renormalize) q[n] /= sum;
-    const double lp = y[n] == -INFINITY ? -INFINITY : (double)y[n] - lse;
+    const double lp = y[n] == -INFINITY ? -INFINITY : (((double)y[n] - all.m) * sc.c - log_s) * ln2;
     if (in[n] && q[n] != 0.0) loss += q[n] * ((double)t[n] - log_norm - lp);
     const int i = n * 32 + threadIdx.x;
     if (i < k) q_out[row * k + i] = in[n] && any ? (float)q[n] : -1.f;
   }
   loss = warp_sum(loss);
   if (threadIdx.x == 0) {
-    const double rest_lp = (double)rest_lse - lse;
+    const double rest_lp = (((double)a.m - all.m) * sc.c + rest_log_s - log_s) * ln2;
     if (rest > 0.0) loss += rest * (log(rest) - rest_lp);
     row_loss[row] = any ? (float)loss : 0.f;
     const double total = mass + rest;
-    float4 o = make_float4(rest_lse, others && any ? (float)(total * exp(rest_lp) - rest) : 0.f, lse, any ? (float)total : -1.f);
-    *reinterpret_cast<float4*>(row_stats + row * 4) = o;
+    float4* o = reinterpret_cast<float4*>(row_stats + row * 8);
+    o[0] = make_float4(any ? (float)total : -1.f, others && any ? (float)(total * exp(rest_lp) - rest) : 0.f, 0.f, 0.f);
+    o[1] = make_float4(all.m, log_s, a.m, rest_log_s);
   }
 }
 
@@ -316,15 +622,15 @@ __global__ void __launch_bounds__(TP_THREADS)
   const long long row = blockIdx.x;
   const T* z = logits + row * ld;
   D* d = dlogits + row * ld_d;
-  const float4 st = *reinterpret_cast<const float4*>(row_stats + row * 4);
+  const float4 st = *reinterpret_cast<const float4*>(row_stats + row * 8), norm = *reinterpret_cast<const float4*>(row_stats + row * 8 + 4);
   const float gs = (g != nullptr ? g[row * stride_g] : 1.f) * scale * (inv_count != nullptr ? *inv_count : 1.f);
-  const bool nothing = st.w < 0.f || st.z == -INFINITY;
-  const float rest_lse = st.x == -INFINITY ? 0.f : st.x;
+  const bool nothing = st.x < 0.f || (norm.x == -INFINITY && norm.y == -INFINITY);
+  const bool others = !(norm.z == -INFINITY && norm.w == -INFINITY);
   const float coef = st.y * gs;
   for (int i = threadIdx.x; i < V; i += TP_THREADS) {
     float slope;
-    const float y = sc.y(to_f(z[i]), &slope);
-    d[i] = from_f<D>(nothing ? 0.f : __expf(y - rest_lse) * coef * slope);
+    const float y = sc.capped(to_f(z[i]), &slope);
+    d[i] = from_f<D>(nothing || !others ? 0.f : exp2_fast((y - norm.z) * sc.c - norm.w) * coef * slope);
   }
   __syncthreads();
   if (threadIdx.x < k && !nothing) {
@@ -332,8 +638,8 @@ __global__ void __launch_bounds__(TP_THREADS)
     if (!(qi < 0.f)) {
       const long long i = teacher_id(teacher_ids, ids_64, row * ld_t + threadIdx.x);
       float slope;
-      const float y = sc.y(to_f(z[i]), &slope);
-      d[i] = from_f<D>((st.w * __expf(y - st.z) - qi) * gs * slope);
+      const float y = sc.capped(to_f(z[i]), &slope);
+      d[i] = from_f<D>((st.x * exp2_fast((y - norm.x) * sc.c - norm.y) - qi) * gs * slope);
     }
   }
 }
@@ -347,7 +653,7 @@ __global__ void __launch_bounds__(1024)
   double sum = 0.0;
   int n = 0;
   for (long long r = threadIdx.x; r < rows; r += 1024) {
-    const bool counted = !(row_stats[r * 4 + 3] < 0.f);
+    const bool counted = !(row_stats[r * 8] < 0.f);
     if (counted) sum += (double)row_loss[r];
     n += counted;
   }
@@ -382,7 +688,10 @@ __global__ void __launch_bounds__(1024)
     }
     n += any;
   }
-  n = block_sum(n, redi);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) redi[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x < 32) n = __reduce_add_sync(0xffffffffu, redi[threadIdx.x]);
   if (threadIdx.x == 0) *inv_count = 1.f / (float)(n > 0 ? n : 1);
 }
 
@@ -394,7 +703,59 @@ static inline int check_logits(const char* what, const void* logits, int dtype, 
 }
 
 static inline Scaling scaling(float softcap, float inv_temp) {
-  return Scaling{softcap, softcap > 0.f ? 1.f / softcap : 0.f, inv_temp};
+  return Scaling{softcap, softcap > 0.f ? 2.f * LOG2E / softcap : 0.f, inv_temp * LOG2E, inv_temp};
+}
+
+// Shared memory beyond 48 KB is an attribute of a kernel on a device: set once for each.
+template <class K>
+static inline int allow_shared(K kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  OB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) OB_FAIL(-7, "device ordinal %d outside the supported range [0, 64)", dev);
+  if (!done[dev]) {
+    OB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done[dev] = true;
+  }
+  return 0;
+}
+
+// CTAs per row: a power of two up to the portable cluster size, as long as all CTAs run at once (three per SM) and a slice keeps a batch
+// or more of every thread.
+static inline int ctas_per_row(long long rows, int V, int per_batch) {
+  int C = 1;
+  while (C < 8 && rows * C * 2 <= 3ll * sm_count() && V / (2 * C) >= per_batch) C *= 2;
+  return C;
+}
+
+template <class K, class... Args>
+static int launch_clusters(K kernel, long long blocks, int C, int shared, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(TP_THREADS);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  OB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return 0;
+}
+
+template <class T, int U, bool CAP, bool TOP>
+static int launch_scores(const T* logits, long long ld, long long rows, const ScoreArgs& args, cudaStream_t stream) {
+  constexpr int per_batch = TP_THREADS * U * Row<T>::N;
+  auto kernel = token_log_probs_fwd_kernel<T, U, CAP, TOP>;
+  const int shared = TOP ? (int)sizeof(Candidates<per_batch + 2 * Row<T>::N>) : 0;
+  if (TOP) {
+    static bool done[64] = {};
+    if (int rc = allow_shared(kernel, shared, done)) return rc;
+  }
+  const int C = ctas_per_row(rows, args.V, per_batch);
+  return launch_clusters(kernel, rows * C, C, shared, stream, logits, ld, C, args);
 }
 
 }  // namespace ob
@@ -402,7 +763,7 @@ static inline Scaling scaling(float softcap, float inv_temp) {
 using namespace ob;
 
 extern "C" int ob_token_log_probs_fwd(const void* logits, int dtype, long long ld, const long long* ids, float* log_probs,
-                                      float* entropy, float* lse, int top_k, float* top_log_probs, long long* top_ids,
+                                      float* entropy, float* norm, int top_k, float* top_log_probs, long long* top_ids,
                                       long long rows, int V, int ignore_index, float softcap, float inv_temp,
                                       cudaStream_t stream) {
   if (rows <= 0) return 0;
@@ -410,29 +771,30 @@ extern "C" int ob_token_log_probs_fwd(const void* logits, int dtype, long long l
   if (top_k < 0 || top_k > OB_TOP_K_MAX || top_k > V) OB_FAIL(-4, "token_log_probs: top_k %d outside [0, min(%d, %d)]", top_k, OB_TOP_K_MAX, V);
   if ((log_probs != nullptr && ids == nullptr) || (top_k > 0 && (top_log_probs == nullptr || top_ids == nullptr)))
     OB_FAIL(-5, "token_log_probs: missing tensor");
-  const Scaling sc = scaling(softcap, inv_temp);
-  if (dtype == OB_F32)
-    token_log_probs_fwd_kernel<float><<<(unsigned)rows, TP_THREADS, 0, stream>>>(
-        (const float*)logits, ld, ids, log_probs, entropy, lse, top_k, top_log_probs, top_ids, V, ignore_index, sc);
-  else
-    token_log_probs_fwd_kernel<bf16><<<(unsigned)rows, TP_THREADS, 0, stream>>>(
-        (const bf16*)logits, ld, ids, log_probs, entropy, lse, top_k, top_log_probs, top_ids, V, ignore_index, sc);
-  OB_CUDA_OK(cudaGetLastError());
-  return 0;
+  const ScoreArgs args{ids, log_probs, entropy, norm, top_k, top_log_probs, top_ids, V, ignore_index, scaling(softcap, inv_temp)};
+  const bool cap = softcap > 0.f, top = top_k > 0;
+  if (dtype == OB_F32) {
+    auto* z = (const float*)logits;
+    if (top) return cap ? launch_scores<float, 2, true, true>(z, ld, rows, args, stream) : launch_scores<float, 2, false, true>(z, ld, rows, args, stream);
+    return cap ? launch_scores<float, 4, true, false>(z, ld, rows, args, stream) : launch_scores<float, 4, false, false>(z, ld, rows, args, stream);
+  }
+  auto* z = (const bf16*)logits;
+  if (top) return cap ? launch_scores<bf16, 1, true, true>(z, ld, rows, args, stream) : launch_scores<bf16, 1, false, true>(z, ld, rows, args, stream);
+  return cap ? launch_scores<bf16, 2, true, false>(z, ld, rows, args, stream) : launch_scores<bf16, 2, false, false>(z, ld, rows, args, stream);
 }
 
-extern "C" int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const long long* ids, const float* lse,
+extern "C" int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const long long* ids, const float* norm,
                                       const float* entropy, const float* g_log_probs, long long stride_lp,
                                       const float* g_entropy, long long stride_ent, void* dlogits, int dtype_d, long long ld_d,
                                       long long rows, int V, int ignore_index, float softcap, float inv_temp,
                                       cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (int rc = check_logits("token_log_probs backward", logits, dtype, ld, rows, V)) return rc;
-  if (lse == nullptr || dlogits == nullptr || (g_log_probs != nullptr && ids == nullptr) || (g_entropy != nullptr && entropy == nullptr))
+  if (norm == nullptr || dlogits == nullptr || (g_log_probs != nullptr && ids == nullptr) || (g_entropy != nullptr && entropy == nullptr))
     OB_FAIL(-5, "token_log_probs backward: missing tensor");
   const Scaling sc = scaling(softcap, inv_temp);
 #define OB_LAUNCH(T, D)                                                                                                     \
-  token_log_probs_bwd_kernel<T, D><<<(unsigned)rows, TP_THREADS, 0, stream>>>((const T*)logits, ld, ids, lse, entropy,      \
+  token_log_probs_bwd_kernel<T, D><<<(unsigned)rows, TP_THREADS, 0, stream>>>((const T*)logits, ld, ids, (const float2*)norm, entropy, \
                                                                               g_log_probs, stride_lp, g_entropy, stride_ent, \
                                                                               (D*)dlogits, ld_d, V, ignore_index, sc)
   if (dtype == OB_F32 && dtype_d == OB_F32) OB_LAUNCH(float, float);

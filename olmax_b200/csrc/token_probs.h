@@ -16,14 +16,14 @@ extern "C" {
 #define OB_TOP_K_MAX 128
 
 // log_probs[r] = log p of class ids[r] (0 where ids[r] == ignore_index or lies outside [0, V); both may be null), entropy[r],
-// lse[r] = log sum exp y (may be null).  top_k > 0: top_log_probs / top_ids [rows, top_k] = the classes with the largest logits
+// norm[r] = two floats (8-byte aligned) that the backward pass reads: the largest capped logit and log2 sum exp(y - its y) (may be null).  top_k > 0: top_log_probs / top_ids [rows, top_k] = the classes with the largest logits
 // in order, equal logits by their class (top_k <= min(V, OB_TOP_K_MAX)).
 int ob_token_log_probs_fwd(const void* logits, int dtype, long long ld, const long long* ids, float* log_probs, float* entropy,
-                           float* lse, int top_k, float* top_log_probs, long long* top_ids, long long rows, int V,
+                           float* norm, int top_k, float* top_log_probs, long long* top_ids, long long rows, int V,
                            int ignore_index, float softcap, float inv_temp, cudaStream_t stream);
 // dlogits (of dtype_d, row stride ld_d) = g_log_probs[r * stride_lp] * d log_probs[r] + g_entropy[r * stride_ent] * d entropy[r]
 // over d logits; either upstream gradient may be null.
-int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const long long* ids, const float* lse,
+int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const long long* ids, const float* norm,
                            const float* entropy, const float* g_log_probs, long long stride_lp, const float* g_entropy,
                            long long stride_ent, void* dlogits, int dtype_d, long long ld_d, long long rows, int V,
                            int ignore_index, float softcap, float inv_temp, cudaStream_t stream);
@@ -33,8 +33,9 @@ int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const lo
 //   renormalize != 0: q = softmax of the row's values;  loss = sum q (log q - log p)
 //   else:             q = exp(value); the classes the teacher does not name are one further class with what is left of one:
 //                     loss = sum q (log q - log p) + rest_q (log rest_q - log rest_p)
-// row_loss[r]; row_stats[r] = (log-sum-exp of the other classes, coefficient of their gradient, lse, total teacher mass or -1 for
-// a row without a teacher: loss 0, gradient 0); q [rows, k] = the teacher's masses, -1 for pairs that do not count.
+// row_loss[r]; row_stats[r] = eight floats (16-byte aligned): the teacher's total mass (-1 for a row without a teacher: loss 0, gradient 0), the
+// coefficient of the other classes' gradient, two unused, the largest capped logit and log2 sum exp(y - its y) of all classes, the same
+// of the other classes; q [rows, k] = the teacher's masses, -1 for pairs that do not count.
 int ob_distill_fwd(const void* logits, int dtype, long long ld, const void* teacher_ids, int ids_64,
                    const float* teacher_log_probs, long long ld_t, int k, int renormalize, float* row_loss, float* row_stats,
                    float* q, long long rows, int V, float softcap, float inv_temp, cudaStream_t stream);

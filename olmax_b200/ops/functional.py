@@ -1197,15 +1197,15 @@ class _TokenLogProbsFn(torch.autograd.Function):
         if z.is_cuda:
             log_probs = torch.empty(rows, dtype=torch.float32, device=z.device) if ids is not None else None
             entropy = torch.empty(rows, dtype=torch.float32, device=z.device)
-            lse = torch.empty_like(entropy) if ctx.needs_input_grad[0] else None
+            norm = torch.empty((rows, 2), dtype=torch.float32, device=z.device) if ctx.needs_input_grad[0] else None
             top = torch.empty((rows, top_k), dtype=torch.float32, device=z.device) if top_k else None
             top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=z.device) if top_k else None
             if rows:
-                K.token_log_probs_fwd(z, ids, log_probs, entropy, lse, top, top_ids, softcap=cap, **ctx.options)
+                K.token_log_probs_fwd(z, ids, log_probs, entropy, norm, top, top_ids, softcap=cap, **ctx.options)
         else:
-            log_probs, entropy, lse, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
+            log_probs, entropy, norm, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(z, ids, lse, entropy)
+            ctx.save_for_backward(z, ids, norm, entropy)
         ctx.mark_non_differentiable(*(t for t in (top, top_ids) if t is not None))
         return log_probs, entropy, top, top_ids
 
@@ -1214,11 +1214,11 @@ class _TokenLogProbsFn(torch.autograd.Function):
     def backward(ctx, g_log_probs, g_entropy, _top, _ids):
         if g_log_probs is None and g_entropy is None:
             return None, None, None, None, None, None
-        z, ids, lse, entropy = ctx.saved_tensors
+        z, ids, norm, entropy = ctx.saved_tensors
         if z.is_cuda:
             d = torch.empty(z.shape, dtype=z.dtype, device=z.device)
             if z.shape[0]:
-                K.token_log_probs_bwd(z, ids, lse, entropy, _upstream(g_log_probs), _upstream(g_entropy), d, softcap=ctx.cap,
+                K.token_log_probs_bwd(z, ids, norm, entropy, _upstream(g_log_probs), _upstream(g_entropy), d, softcap=ctx.cap,
                                       **ctx.options)
         else:
             d = ref.token_log_probs_bwd(z, ids, g_log_probs, g_entropy, cap=ctx.cap, **ctx.options)
@@ -1285,7 +1285,7 @@ class _DistillationFn(torch.autograd.Function):
         if z.is_cuda:
             dev = z.device
             loss = torch.empty(rows, dtype=torch.float32, device=dev)
-            stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+            stats = torch.empty((rows, 8), dtype=torch.float32, device=dev)
             q = torch.empty((rows, k), dtype=torch.float32, device=dev)
             total = torch.empty((), dtype=torch.float32, device=dev)
             inv = torch.empty((), dtype=torch.float32, device=dev)
@@ -1428,17 +1428,17 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
             dev = x2.device
             log_probs = torch.empty(M, dtype=torch.float32, device=dev) if ids is not None else None
             entropy = torch.empty(M, dtype=torch.float32, device=dev)
-            lse = torch.empty_like(entropy) if keep else None
+            norm = torch.empty((M, 2), dtype=torch.float32, device=dev) if keep else None
             top = torch.empty((M, top_k), dtype=torch.float32, device=dev) if top_k else None
             top_ids = torch.empty((M, top_k), dtype=torch.int64, device=dev) if top_k else None
             for r0, r1, _, z in _HeadChunks(x2, handle, chunk_rows):
-                cut = [t[r0:r1] if t is not None else None for t in (ids, log_probs, entropy, lse, top, top_ids)]
+                cut = [t[r0:r1] if t is not None else None for t in (ids, log_probs, entropy, norm, top, top_ids)]
                 K.token_log_probs_fwd(z, *cut, softcap=cap, **ctx.options)
         else:
             z = (x2 @ handle.full().t()).float()
-            log_probs, entropy, lse, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
+            log_probs, entropy, norm, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
         if keep:
-            ctx.save_for_backward(x2, ids, lse, entropy)
+            ctx.save_for_backward(x2, ids, norm, entropy)
         ctx.mark_non_differentiable(*(t for t in (top, top_ids) if t is not None))
         return log_probs, entropy, top, top_ids
 
@@ -1447,7 +1447,7 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
     def backward(ctx, g_log_probs, g_entropy, _top, _ids):
         if g_log_probs is None and g_entropy is None:
             return (None,) * 8
-        x2, ids, lse, entropy = ctx.saved_tensors
+        x2, ids, norm, entropy = ctx.saved_tensors
         handle = ctx.handle
         if _on_gpu(x2):
             gl, ge = _upstream(g_log_probs), _upstream(g_entropy)
@@ -1455,7 +1455,7 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
             dlogits, single = chunks.gradients()
             dx = torch.empty_like(x2)
             for r0, r1, xc, z in chunks:
-                cut = [t[r0:r1] if t is not None else None for t in (ids, lse, entropy, gl, ge)]
+                cut = [t[r0:r1] if t is not None else None for t in (ids, norm, entropy, gl, ge)]
                 K.token_log_probs_bwd(z, *cut, chunks.rows_of(dlogits, single, r0, r1), softcap=ctx.cap, **ctx.options)
                 chunks.chunk_gradient(dlogits, single, r0, r1, xc, dx)
             chunks.finish(dlogits, single)
@@ -1496,7 +1496,7 @@ class _LinearDistillationFn(torch.autograd.Function):
             inv = torch.empty((), dtype=torch.float32, device=dev)
             K.distill_count(ids, values, inv, renormalize=renormalize, V=V)
             loss = torch.empty(M, dtype=torch.float32, device=dev)
-            stats = torch.empty((M, 4), dtype=torch.float32, device=dev)
+            stats = torch.empty((M, 8), dtype=torch.float32, device=dev)
             chunks = _HeadChunks(x2, handle, chunk_rows)
             q = torch.empty((chunks.step, ids.shape[1]), dtype=torch.float32, device=dev)
             dx = torch.empty_like(x2) if need_grad else None

@@ -427,24 +427,24 @@ def _on(device: torch.device):
     return torch.cuda.device(device)
 
 
-def token_log_probs_fwd(logits, ids, log_probs, entropy, lse, top_log_probs, top_ids, *, ignore_index=-100, softcap=0.0,
+def token_log_probs_fwd(logits, ids, log_probs, entropy, norm, top_log_probs, top_ids, *, ignore_index=-100, softcap=0.0,
                         temperature=1.0) -> None:
-    """Any of the outputs but ``entropy`` may be None; the number of top classes is ``top_ids.shape[1]``."""
+    """Any of the outputs but ``entropy`` may be None; ``norm`` [rows, 2] is what :func:`token_log_probs_bwd` reads; the number of top classes is ``top_ids.shape[1]``."""
     rows, V = logits.shape
     with _on(logits.device):
         check(lib().ob_token_log_probs_fwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), _ptr(ids), _ptr(log_probs),
-                                           entropy.data_ptr(), _ptr(lse), 0 if top_ids is None else top_ids.shape[1],
+                                           entropy.data_ptr(), _ptr(norm), 0 if top_ids is None else top_ids.shape[1],
                                            _ptr(top_log_probs), _ptr(top_ids), rows, V, ignore_index, softcap,
                                            1.0 / temperature, stream_ptr(logits.device)), "token_log_probs_fwd")
     _count()
 
 
-def token_log_probs_bwd(logits, ids, lse, entropy, g_log_probs, g_entropy, dlogits, *, ignore_index=-100, softcap=0.0,
+def token_log_probs_bwd(logits, ids, norm, entropy, g_log_probs, g_entropy, dlogits, *, ignore_index=-100, softcap=0.0,
                         temperature=1.0) -> None:
     """``g_log_probs`` / ``g_entropy``: fp32 [rows] of any stride, or None."""
     rows, V = logits.shape
     with _on(logits.device):
-        check(lib().ob_token_log_probs_bwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), _ptr(ids), lse.data_ptr(),
+        check(lib().ob_token_log_probs_bwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), _ptr(ids), norm.data_ptr(),
                                            entropy.data_ptr(), _ptr(g_log_probs), 0 if g_log_probs is None else g_log_probs.stride(0),
                                            _ptr(g_entropy), 0 if g_entropy is None else g_entropy.stride(0), dlogits.data_ptr(),
                                            _logits_dtype(dlogits), dlogits.stride(0), rows, V, ignore_index, softcap,
@@ -461,7 +461,7 @@ def _teacher_ids(t: torch.Tensor) -> int:
 def distill_fwd(logits, teacher_ids, teacher_log_probs, row_loss, row_stats, q, *, renormalize, softcap=0.0,
                 temperature=1.0) -> None:
     """``teacher_ids`` (int32 / int64) and ``teacher_log_probs`` (fp32) [rows, k] with one row stride; row_loss [rows], row_stats
-    [rows, 4] and q [rows, k] are fp32 outputs that :func:`distill_bwd` reads."""
+    [rows, 8] and q [rows, k] are fp32 outputs that :func:`distill_bwd` reads."""
     rows, V = logits.shape
     if teacher_log_probs.stride() != teacher_ids.stride() or teacher_log_probs.dtype != torch.float32:
         raise KernelError("distillation: fp32 teacher values laid out like the teacher's ids are needed")

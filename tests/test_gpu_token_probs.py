@@ -448,3 +448,18 @@ def test_refusals_reach_no_kernel():
         _bf16_head(64, 64).token_log_probs(torch.zeros(4, 64, device=DEV))
     out = F.token_log_probs(z[:0], torch.zeros(0, dtype=torch.int64, device=DEV), top_k=2)
     assert out.top_ids.shape == (0, 2) and K.launch_count() == before
+
+
+def test_infinite_logits():
+    """+inf has no distribution (NaN, as the formula gives it), but an order."""
+    for V in (40, 9000):
+        z = _logits(3, V)
+        z[0, 5] = math.inf
+        z[1, V - 1] = z[1, 7] = math.inf
+        z[1, 20] = math.nan
+        out = F.token_log_probs(z, torch.tensor([5, 7, 3], device=DEV), top_k=3)
+        assert out.log_probs[:2].isnan().all() and out.entropy[:2].isnan().all() and out.log_probs[2].isfinite()
+        best = z.clone()
+        best[0, 5] = -math.inf
+        assert out.top_ids[0].tolist() == [5, *best[0].topk(2).indices.tolist()]
+        assert out.top_ids[1].tolist() == [20, 7, V - 1]
