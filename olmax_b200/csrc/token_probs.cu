@@ -10,6 +10,7 @@
 
 #include <float.h>
 #include <limits.h>
+#include <type_traits>
 #include "sm100.cuh"
 
 namespace ob {
@@ -472,34 +473,101 @@ __global__ void __launch_bounds__(TP_THREADS, 3)
   }
 }
 
-template <class T, class D>
-__global__ void __launch_bounds__(TP_THREADS)
-    token_log_probs_bwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ ids,
-                               const float2* __restrict__ norm, const float* __restrict__ entropy,
-                               const float* __restrict__ g_log_probs, long long stride_lp,
-                               const float* __restrict__ g_entropy, long long stride_ent, D* __restrict__ dlogits,
-                               long long ld_d, int V, int ignore_index, Scaling sc) {
-  const long long row = blockIdx.x;
-  const T* z = logits + row * ld;
-  D* d = dlogits + row * ld_d;
-  const float2 lse = norm[row];
-  const float ge = g_entropy != nullptr ? g_entropy[row * stride_ent] : 0.f;
+// ---------------------------------------------------------------------------------------------------------------------
+// Gradients: every class's from its logit and a few numbers of the row.  A block takes a span of a row, blocks in launch order.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int GRAD_THREADS = 256, GRAD_UNROLL = 4;
+
+// N gradients to where they lie side by side, N * sizeof(D) bytes aligned alike
+template <class D, int N>
+__device__ __forceinline__ void store_vector(D* d, const float (&g)[N]);
+template <>
+__device__ __forceinline__ void store_vector<float, 4>(float* d, const float (&g)[4]) {
+  *reinterpret_cast<float4*>(d) = make_float4(g[0], g[1], g[2], g[3]);
+}
+template <>
+__device__ __forceinline__ void store_vector<bf16, 4>(bf16* d, const float (&g)[4]) {
+  *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]));
+}
+template <>
+__device__ __forceinline__ void store_vector<bf16, 8>(bf16* d, const float (&g)[8]) {
+  *reinterpret_cast<uint4*>(d) = make_uint4(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7]));
+}
+
+// The span `part` of `per_block` vectors of a row and its gradient: d[i] = grad(z[i], i) for its classes [lo, hi), which it returns.
+// The gradient is written in vectors where its row is aligned like the logits', else class by class.
+template <class T, class D, class F>
+__device__ __forceinline__ int2 map_span(const T* z, D* d, int V, int part, int parts, int per_block, F grad) {
+  constexpr int N = Row<T>::N;
+  const Row<T> r(z, V);
+  const int v0 = min(r.nvec, part * per_block), v1 = part == parts - 1 ? r.nvec : min(r.nvec, v0 + per_block);
+  const int lo = part == 0 ? 0 : r.class_of(v0), hi = part == parts - 1 ? V : r.class_of(v1);
+  if ((reinterpret_cast<uintptr_t>(d + r.head) & (N * sizeof(D) - 1)) != 0) {
+    for (int i = lo + threadIdx.x; i < hi; i += GRAD_THREADS) d[i] = from_f<D>(grad(to_f(z[i]), i));
+    return make_int2(lo, hi);
+  }
+  for (int b = v0 + threadIdx.x; b < v1; b += GRAD_THREADS * GRAD_UNROLL) {
+    uint4 v[GRAD_UNROLL];
+#pragma unroll
+    for (int k = 0; k < GRAD_UNROLL; ++k)
+      if (b + k * GRAD_THREADS < v1) v[k] = r.load(b + k * GRAD_THREADS);
+#pragma unroll
+    for (int k = 0; k < GRAD_UNROLL; ++k) {
+      const int i = b + k * GRAD_THREADS;
+      if (i >= v1) break;
+      float f[N];
+      unpack<T>(v[k], f);
+      const int cls = r.class_of(i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = grad(f[j], cls + j);
+      store_vector<D, N>(d + cls, f);
+    }
+  }
+  const int single = r.single(threadIdx.x, part == 0, part == parts - 1);
+  if (single >= 0) d[single] = from_f<D>(grad(to_f(z[single]), single));
+  return make_int2(lo, hi);
+}
+
+struct ScoreGradArgs {
+  const long long* ids;
+  const float2* norm;
+  const float *entropy, *g_log_probs, *g_entropy;
+  long long stride_lp, stride_ent;
+  int V, ignore_index;
+  Scaling sc;
+};
+
+// dz = dy/dz (g_lp (onehot - p) - g_H p (log p + H)) = dy/dz (g_lp onehot - p (k0 + k1 t)) with t = log2 p.
+template <class T, class D, bool CAP>
+__global__ void __launch_bounds__(GRAD_THREADS)
+    token_log_probs_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts,
+                               int per_block, ScoreGradArgs p) {
+  const long long row = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x - row * parts);
+  const float2 norm = p.norm[row];
+  const float ge = p.g_entropy != nullptr ? p.g_entropy[row * p.stride_ent] : 0.f;
   float gl = 0.f;
-  long long id = -1;
-  if (g_log_probs != nullptr) {
-    id = ids[row];
-    if (id != (long long)ignore_index && id >= 0 && id < V) gl = g_log_probs[row * stride_lp];
-    else id = -1;
+  int id = -1;
+  if (p.g_log_probs != nullptr) {
+    const long long i = p.ids[row];
+    if (i != (long long)p.ignore_index && i >= 0 && i < p.V) {
+      gl = p.g_log_probs[row * p.stride_lp];
+      id = (int)i;
+    }
   }
-  const bool none = lse.x == -INFINITY && lse.y == -INFINITY;
-  const float h = entropy != nullptr ? entropy[row] : 0.f;
-  for (int i = threadIdx.x; i < V; i += TP_THREADS) {
-    float slope;
-    const float lp = (sc.capped(to_f(z[i]), &slope) - lse.x) * sc.c - lse.y, p = exp2_fast(lp);
-    float g = -p * (gl + ge * (p > 0.f ? fmaf(lp, LN2, h) : 0.f));
+  const bool none = norm.x == -INFINITY && norm.y == -INFINITY;
+  const float scale = CAP ? 1.f : p.sc.inv_temp;
+  const float k0 = (gl + ge * (ge != 0.f ? p.entropy[row] : 0.f)) * scale, k1 = ge * LN2 * scale;
+  gl *= scale;
+  map_span<T, D>(logits + row * ld, dlogits + row * ld_d, p.V, part, parts, per_block, [&](float z, int i) {
+    float slope = 1.f;
+    if (CAP) z = p.sc.capped(z, &slope);
+    const float t = (z - norm.x) * p.sc.c - norm.y, e = exp2_fast(t);
+    // (2^t is 0 from -150 on; what it is multiplied by stays finite)
+    float g = -e * fmaf(k1, fmaxf(t, -1024.f), k0);
     if (i == id) g += gl;
-    d[i] = from_f<D>(none ? 0.f : g * slope);
-  }
+    return none ? 0.f : g * slope;
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -519,39 +587,27 @@ __device__ __forceinline__ double warp_sum(double x) {
   return x;
 }
 
-template <class T>
-__global__ void __launch_bounds__(TP_THREADS)
-    distill_fwd_kernel(const T* __restrict__ logits, long long ld, const void* __restrict__ teacher_ids, int ids_64,
-                       const float* __restrict__ teacher_log_probs, long long ld_t, int k, int renormalize,
-                       float* __restrict__ row_loss, float* __restrict__ row_stats, float* __restrict__ q_out, int V,
-                       Scaling sc) {
-  extern __shared__ unsigned named[];   // one bit per class
-  __shared__ Stats red[TP_THREADS / 32];
-  __shared__ long long id_s[OB_TOP_K_MAX];
-  const long long row = blockIdx.x;
-  const T* z = logits + row * ld;
-  for (int i = threadIdx.x; i < (V + 31) / 32; i += TP_THREADS) named[i] = 0;
-  if (threadIdx.x < k) id_s[threadIdx.x] = teacher_id(teacher_ids, ids_64, row * ld_t + threadIdx.x);
-  __syncthreads();
-  bool counts = false;
-  if (threadIdx.x < k) {
-    const long long id = id_s[threadIdx.x];
-    counts = id >= 0 && id < V;
-    for (int j = 0; j < (int)threadIdx.x; ++j) counts &= id_s[j] != id;
-    if (counts) atomicOr(&named[id >> 5], 1u << (id & 31));
-  }
-  __syncthreads();
-  if (threadIdx.x < k && !counts) id_s[threadIdx.x] = -1;
-  Stats a = empty_stats();
-  for (int i = threadIdx.x; i < V; i += TP_THREADS)
-    if (!((named[i >> 5] >> (i & 31)) & 1)) {
-      const float f[1] = {sc.capped(to_f(z[i]))};
-      add_classes<false, 1>(a, f, sc.c);
-    }
-  a = block_combine(a, red, sc.c);
-  if (threadIdx.x >= 32) return;
-  // the first warp: up to four of the teacher's pairs per lane
+struct DistillArgs {
+  const void* teacher_ids;
+  const float* teacher_log_probs;
+  int ids_64, k, renormalize;
+  long long ld_t;
+  float *row_loss, *row_stats, *q;
+  int V;
+  Scaling sc;
+};
+
+// The teacher's pairs of a row in shared memory: class (-1: does not count), value, student's capped logit.
+struct Pairs {
+  int cls[OB_TOP_K_MAX], repeated[OB_TOP_K_MAX];
+  float t[OB_TOP_K_MAX], y[OB_TOP_K_MAX];
+};
+
+// The row's loss and what its gradient needs, by one warp: `others` = statistics of the classes outside the teacher's.
+__device__ __forceinline__ void distill_row(const Pairs& pairs, Stats others_stats, long long row, const DistillArgs& p) {
+  const int lane = threadIdx.x & 31;
   constexpr int N = OB_TOP_K_MAX / 32;
+  const double ln2 = 0.69314718055994530942;
   float t[N], y[N];
   bool in[N];
   Stats st = empty_stats();
@@ -559,25 +615,22 @@ __global__ void __launch_bounds__(TP_THREADS)
   bool any = false;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    const int i = n * 32 + threadIdx.x;
-    in[n] = i < k && id_s[i] >= 0;
-    t[n] = in[n] ? teacher_log_probs[row * ld_t + i] : -INFINITY;
-    const float f[1] = {in[n] ? sc.capped(to_f(z[id_s[i]])) : -INFINITY};
+    const int i = n * 32 + lane;
+    in[n] = i < p.k && pairs.cls[i] >= 0;
+    t[n] = in[n] ? pairs.t[i] : -INFINITY;
+    const float f[1] = {in[n] ? pairs.y[i] : -INFINITY};
     y[n] = f[0];
-    if (in[n]) add_classes<false, 1>(st, f, sc.c);
+    if (in[n]) add_classes<false, 1>(st, f, p.sc.c);
     t_max = fmaxf(t_max, t[n]);
-    any |= in[n] && !(renormalize && t[n] == -INFINITY);
+    any |= in[n] && !(p.renormalize && t[n] == -INFINITY);
   }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    t_max = fmaxf(t_max, __shfl_xor_sync(0xffffffffu, t_max, off));
-  }
+  for (int off = 16; off > 0; off >>= 1) t_max = fmaxf(t_max, __shfl_xor_sync(0xffffffffu, t_max, off));
   any = __any_sync(0xffffffffu, any);
-  const Stats all = combine(shuffle_combine(st, 16, sc.c), a, sc.c);
+  const Stats a = others_stats, all = combine(shuffle_combine(st, 16, p.sc.c), a, p.sc.c);
   const bool others = !no_class(a);
   const float log_s = log2f(all.s), rest_log_s = log2f(a.s);
-  const double ln2 = 0.69314718055994530942;
-  const double shift = renormalize && t_max > -INFINITY ? (double)t_max : 0.0;
+  const double shift = p.renormalize && t_max > -INFINITY ? (double)t_max : 0.0;
   double q[N], sum = 0.0;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -586,7 +639,7 @@ __global__ void __launch_bounds__(TP_THREADS)
   }
   sum = warp_sum(sum);
   double log_norm = shift, mass = sum, rest = 0.0;
-  if (renormalize) {
+  if (p.renormalize) {
     log_norm += log(sum);
     mass = 1.0;
   } else if (others) {
@@ -595,54 +648,172 @@ __global__ void __launch_bounds__(TP_THREADS)
   double loss = 0.0;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    if (renormalize) q[n] /= sum;
-    const double lp = y[n] == -INFINITY ? -INFINITY : (((double)y[n] - all.m) * sc.c - log_s) * ln2;
+    if (p.renormalize) q[n] /= sum;
+    const double lp = y[n] == -INFINITY ? -INFINITY : (((double)y[n] - all.m) * p.sc.c - log_s) * ln2;
     if (in[n] && q[n] != 0.0) loss += q[n] * ((double)t[n] - log_norm - lp);
-    const int i = n * 32 + threadIdx.x;
-    if (i < k) q_out[row * k + i] = in[n] && any ? (float)q[n] : -1.f;
+    const int i = n * 32 + lane;
+    if (i < p.k) p.q[row * p.k + i] = in[n] && any ? (float)q[n] : -1.f;
   }
   loss = warp_sum(loss);
-  if (threadIdx.x == 0) {
-    const double rest_lp = (((double)a.m - all.m) * sc.c + rest_log_s - log_s) * ln2;
+  if (lane == 0) {
+    const double rest_lp = (((double)a.m - all.m) * p.sc.c + rest_log_s - log_s) * ln2;
     if (rest > 0.0) loss += rest * (log(rest) - rest_lp);
-    row_loss[row] = any ? (float)loss : 0.f;
+    p.row_loss[row] = any ? (float)loss : 0.f;
     const double total = mass + rest;
-    float4* o = reinterpret_cast<float4*>(row_stats + row * 8);
+    float4* o = reinterpret_cast<float4*>(p.row_stats + row * 8);
     o[0] = make_float4(any ? (float)total : -1.f, others && any ? (float)(total * exp(rest_lp) - rest) : 0.f, 0.f, 0.f);
     o[1] = make_float4(all.m, log_s, a.m, rest_log_s);
   }
 }
 
-template <class T, class D>
-__global__ void __launch_bounds__(TP_THREADS)
-    distill_bwd_kernel(const T* __restrict__ logits, long long ld, const void* __restrict__ teacher_ids, int ids_64,
-                       long long ld_t, int k, const float* __restrict__ row_stats, const float* __restrict__ q,
-                       const float* __restrict__ g, long long stride_g, const float* __restrict__ inv_count, float scale,
-                       D* __restrict__ dlogits, long long ld_d, int V, Scaling sc) {
-  const long long row = blockIdx.x;
-  const T* z = logits + row * ld;
-  D* d = dlogits + row * ld_d;
-  const float4 st = *reinterpret_cast<const float4*>(row_stats + row * 8), norm = *reinterpret_cast<const float4*>(row_stats + row * 8 + 4);
-  const float gs = (g != nullptr ? g[row * stride_g] : 1.f) * scale * (inv_count != nullptr ? *inv_count : 1.f);
-  const bool nothing = st.x < 0.f || (norm.x == -INFINITY && norm.y == -INFINITY);
-  const bool others = !(norm.z == -INFINITY && norm.w == -INFINITY);
-  const float coef = st.y * gs;
-  for (int i = threadIdx.x; i < V; i += TP_THREADS) {
-    float slope;
-    const float y = sc.capped(to_f(z[i]), &slope);
-    d[i] = from_f<D>(nothing || !others ? 0.f : exp2_fast((y - norm.z) * sc.c - norm.w) * coef * slope);
-  }
-  __syncthreads();
-  if (threadIdx.x < k && !nothing) {
-    const float qi = q[row * k + threadIdx.x];
-    if (!(qi < 0.f)) {
-      const long long i = teacher_id(teacher_ids, ids_64, row * ld_t + threadIdx.x);
-      float slope;
-      const float y = sc.capped(to_f(z[i]), &slope);
-      d[i] = from_f<D>((st.x * exp2_fast((y - norm.x) * sc.c - norm.y) - qi) * gs * slope);
+// A row belongs to a cluster of C CTAs as in the log probabilities.  A bit of shared memory per class of the slice says which the teacher
+// names; four or eight of them, one vector's, cost one look per 16 bytes.
+template <class T, int U, bool CAP>
+__global__ void __launch_bounds__(TP_THREADS, 3)
+    distill_fwd_kernel(const T* __restrict__ logits, long long ld, int C, DistillArgs p) {
+  constexpr int N = Row<T>::N, E = U * N;
+  extern __shared__ __align__(16) char shared_bytes[];
+  unsigned* named = reinterpret_cast<unsigned*>(shared_bytes);
+  __shared__ Stats red[TP_THREADS / 32], slices[8];
+  __shared__ Pairs pairs;
+  if (C > 1) cluster_arrive();
+  const long long row = blockIdx.x / (unsigned)C;
+  const int part = (int)(blockIdx.x - row * C);
+  const Row<T> r(logits + row * ld, p.V);
+  const int v0 = (int)((long long)r.nvec * part / C), v1 = (int)((long long)r.nvec * (part + 1) / C);
+  const int lo = part == 0 ? 0 : r.class_of(v0), hi = part == C - 1 ? p.V : r.class_of(v1);
+  // the bit of class i: vectors begin at multiples of N, the row's head lies in front of the first
+  const int shift = N - r.class_of(v0);
+  long long id = -1;
+  if ((int)threadIdx.x < p.k) {
+    id = teacher_id(p.teacher_ids, p.ids_64, row * p.ld_t + threadIdx.x);
+    if (id < 0 || id >= p.V) id = -1;
+    if (part == 0) {
+      pairs.t[threadIdx.x] = p.teacher_log_probs[row * p.ld_t + threadIdx.x];
+      if (id >= 0) pairs.y[threadIdx.x] = p.sc.capped(to_f(r.z[id]));
     }
   }
+  if (threadIdx.x < OB_TOP_K_MAX) {
+    pairs.cls[threadIdx.x] = (int)id;
+    pairs.repeated[threadIdx.x] = 0;
+  }
+  for (int i = threadIdx.x; i < (hi + shift + 31) / 32; i += TP_THREADS) named[i] = 0;
+  __syncthreads();
+  {
+    // four threads look for an earlier pair with the class of one
+    const int i = threadIdx.x % OB_TOP_K_MAX, j0 = threadIdx.x / OB_TOP_K_MAX * (OB_TOP_K_MAX / 4);
+    const int mine = pairs.cls[i];
+    bool before = false;
+    if (mine >= 0 && j0 < i) {
+#pragma unroll
+      for (int j = 0; j < OB_TOP_K_MAX / 4; ++j) before |= pairs.cls[j0 + j] == mine && j0 + j < i;
+    }
+    if (before) pairs.repeated[i] = 1;
+  }
+  __syncthreads();
+  if (threadIdx.x < OB_TOP_K_MAX) {
+    if (pairs.repeated[threadIdx.x]) pairs.cls[threadIdx.x] = -1;
+    else if (id >= lo && id < hi) atomicOr(&named[((int)id + shift) >> 5], 1u << (((int)id + shift) & 31));
+  }
+  __syncthreads();
+  Stats a = empty_stats();
+  const int single = r.single(threadIdx.x, part == 0, part == C - 1);
+  if (single >= 0 && !((named[(single + shift) >> 5] >> ((single + shift) & 31)) & 1)) {
+    const float f[1] = {p.sc.capped(to_f(r.z[single]))};
+    add_classes<false, 1>(a, f, p.sc.c);
+  }
+  for (int b = v0; b < v1; b += TP_THREADS * U) {
+    uint4 v[U];
+    unsigned out[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = b + k * TP_THREADS + threadIdx.x;
+      v[k] = i < v1 ? r.load(i) : no_vector<T>();
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = b + k * TP_THREADS + threadIdx.x, bit = (i - v0 + 1) * N;
+      out[k] = i < v1 ? (named[bit >> 5] >> (bit & 31)) & ((1u << N) - 1) : (1u << N) - 1;
+    }
+    float f[E];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      unpack<T>(v[k], f + k * N);
+      if (CAP) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[k * N + j] = p.sc.capped(f[k * N + j]);
+      }
+      if (out[k]) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if ((out[k] >> j) & 1) f[k * N + j] = -INFINITY;
+      }
+    }
+    add_classes<false, E>(a, f, p.sc.c);
+  }
+  a = block_combine(a, red, p.sc.c);
+  if (C > 1) {
+    cluster_wait();   // the first CTA runs
+    if (threadIdx.x == 0) {
+      const uint32_t at = mapa_shared(smem_u32(&slices[part]), 0);
+      store_cluster(at, a.m);
+      store_cluster(at + 4, a.s);
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (part != 0) return;
+    a = Stats{slices[0].m, slices[0].s, 0.f};
+    for (int i = 1; i < C; ++i) a = combine(a, Stats{slices[i].m, slices[i].s, 0.f}, p.sc.c);
+  }
+  if (threadIdx.x < 32) distill_row(pairs, a, row, p);
 }
+
+struct DistillGradArgs {
+  const void* teacher_ids;
+  int ids_64, k;
+  long long ld_t;
+  const float *row_stats, *q, *g;
+  long long stride_g;
+  const float* inv_count;
+  float scale;
+  int V;
+  Scaling sc;
+};
+
+template <class T, class D, bool CAP>
+__global__ void __launch_bounds__(GRAD_THREADS)
+    distill_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts, int per_block,
+                       DistillGradArgs p) {
+  const long long row = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x - row * parts);
+  const T* z = logits + row * ld;
+  D* d = dlogits + row * ld_d;
+  const float2 st = *reinterpret_cast<const float2*>(p.row_stats + row * 8);
+  const float4 norm = *reinterpret_cast<const float4*>(p.row_stats + row * 8 + 4);
+  long long id = -1;
+  float q = -1.f;
+  if ((int)threadIdx.x < p.k) {
+    q = p.q[row * p.k + threadIdx.x];
+    id = teacher_id(p.teacher_ids, p.ids_64, row * p.ld_t + threadIdx.x);
+  }
+  const float gs = (p.g != nullptr ? p.g[row * p.stride_g] : 1.f) * p.scale * (p.inv_count != nullptr ? *p.inv_count : 1.f);
+  const bool nothing = st.x < 0.f || (norm.x == -INFINITY && norm.y == -INFINITY);
+  const bool zero = nothing || (norm.z == -INFINITY && norm.w == -INFINITY);   // no class outside the teacher's
+  const float coef = st.y * gs * (CAP ? 1.f : p.sc.inv_temp);
+  const int2 span = map_span<T, D>(z, d, p.V, part, parts, per_block, [&](float x, int) {
+    float slope = 1.f;
+    if (CAP) x = p.sc.capped(x, &slope);
+    return zero ? 0.f : exp2_fast((x - norm.z) * p.sc.c - norm.w) * coef * slope;
+  });
+  // the teacher's classes, over what has just been written for them
+  __syncthreads();
+  if (!nothing && !(q < 0.f) && id >= span.x && id < span.y) {
+    float slope;
+    const float x = p.sc.capped(to_f(z[id]), &slope);
+    d[id] = from_f<D>((st.x * exp2_fast((x - norm.x) * p.sc.c - norm.y) - q) * gs * slope);
+  }
+}
+static_assert(OB_TOP_K_MAX <= GRAD_THREADS, "one thread per class of the teacher");
 
 // One block: the order of the sum does not depend on the launch.
 __global__ void __launch_bounds__(1024)
@@ -758,6 +929,39 @@ static int launch_scores(const T* logits, long long ld, long long rows, const Sc
   return launch_clusters(kernel, rows * C, C, shared, stream, logits, ld, C, args);
 }
 
+template <class T, int U, bool CAP>
+static int launch_distill(const T* logits, long long ld, long long rows, const DistillArgs& args, cudaStream_t stream) {
+  constexpr int N = Row<T>::N, LIMIT = 160 * 1024;
+  auto kernel = distill_fwd_kernel<T, U, CAP>;
+  const int C = ctas_per_row(rows, args.V, TP_THREADS * U * N);
+  // a bit for each class of a slice, with the row's head, tail and the rounding of its vectors
+  const int bytes = (args.V / C + 4 * N + 31) / 32 * 4;
+  if (bytes > LIMIT) OB_FAIL(-6, "distillation: %d classes are more than %d", args.V, LIMIT * 8);
+  static bool done[64] = {};
+  if (int rc = allow_shared(kernel, LIMIT, done)) return rc;
+  return launch_clusters(kernel, rows * C, C, bytes, stream, logits, ld, C, args);
+}
+
+// Calls launch(z, d, parts, per_block) with the types of the logits and of their gradient and the spans of a row.
+template <class F>
+static int launch_gradient(const char* what, const void* z, int dtype, long long ld, void* d, int dtype_d, long long ld_d,
+                           long long rows, int V, cudaStream_t stream, F launch) {
+  const int N = dtype == OB_F32 ? 4 : 8;
+  // two batches of every thread to a block, more where the grid would not hold the blocks
+  long long per_block = 2ll * GRAD_THREADS * GRAD_UNROLL, parts = 0;
+  for (;; per_block *= 2) {
+    parts = (V / N + per_block - 1) / per_block;
+    if (parts < 1) parts = 1;
+    if (rows * parts <= INT_MAX) break;
+  }
+  if (dtype == OB_F32 && dtype_d == OB_F32) launch((const float*)z, (float*)d, (int)parts, (int)per_block);
+  else if (dtype == OB_F32 && dtype_d == OB_BF16) launch((const float*)z, (bf16*)d, (int)parts, (int)per_block);
+  else if (dtype == OB_BF16 && dtype_d == OB_BF16) launch((const bf16*)z, (bf16*)d, (int)parts, (int)per_block);
+  else OB_FAIL(-2, "%s: no gradient of type %d for logits of type %d", what, dtype_d, dtype);
+  OB_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
 }  // namespace ob
 
 using namespace ob;
@@ -793,17 +997,15 @@ extern "C" int ob_token_log_probs_bwd(const void* logits, int dtype, long long l
   if (norm == nullptr || dlogits == nullptr || (g_log_probs != nullptr && ids == nullptr) || (g_entropy != nullptr && entropy == nullptr))
     OB_FAIL(-5, "token_log_probs backward: missing tensor");
   const Scaling sc = scaling(softcap, inv_temp);
-#define OB_LAUNCH(T, D)                                                                                                     \
-  token_log_probs_bwd_kernel<T, D><<<(unsigned)rows, TP_THREADS, 0, stream>>>((const T*)logits, ld, ids, (const float2*)norm, entropy, \
-                                                                              g_log_probs, stride_lp, g_entropy, stride_ent, \
-                                                                              (D*)dlogits, ld_d, V, ignore_index, sc)
-  if (dtype == OB_F32 && dtype_d == OB_F32) OB_LAUNCH(float, float);
-  else if (dtype == OB_F32 && dtype_d == OB_BF16) OB_LAUNCH(float, bf16);
-  else if (dtype == OB_BF16 && dtype_d == OB_BF16) OB_LAUNCH(bf16, bf16);
-  else OB_FAIL(-2, "token_log_probs backward: no gradient of type %d for logits of type %d", dtype_d, dtype);
-#undef OB_LAUNCH
-  OB_CUDA_OK(cudaGetLastError());
-  return 0;
+  const ScoreGradArgs args{ids, (const float2*)norm, entropy, g_log_probs, g_entropy, stride_lp, stride_ent, V, ignore_index, sc};
+  return launch_gradient("token_log_probs backward", logits, dtype, ld, dlogits, dtype_d, ld_d, rows, V, stream,
+                         [&](auto* z, auto* d, int parts, int per_block) {
+    typedef std::remove_const_t<std::remove_pointer_t<decltype(z)>> T;
+    typedef std::remove_pointer_t<decltype(d)> D;
+    const unsigned blocks = (unsigned)(rows * parts);
+    if (softcap > 0.f) token_log_probs_bwd_kernel<T, D, true><<<blocks, GRAD_THREADS, 0, stream>>>(z, ld, d, ld_d, parts, per_block, args);
+    else token_log_probs_bwd_kernel<T, D, false><<<blocks, GRAD_THREADS, 0, stream>>>(z, ld, d, ld_d, parts, per_block, args);
+  });
 }
 
 extern "C" int ob_distill_fwd(const void* logits, int dtype, long long ld, const void* teacher_ids, int ids_64,
@@ -815,18 +1017,12 @@ extern "C" int ob_distill_fwd(const void* logits, int dtype, long long ld, const
   if (k < 1 || k > OB_TOP_K_MAX) OB_FAIL(-4, "distillation: %d teacher classes outside [1, %d]", k, OB_TOP_K_MAX);
   if (teacher_ids == nullptr || teacher_log_probs == nullptr || row_loss == nullptr || row_stats == nullptr || q == nullptr)
     OB_FAIL(-5, "distillation: missing tensor");
-  const int bytes = (V + 31) / 32 * 4;
-  if (bytes > 160 * 1024) OB_FAIL(-6, "distillation: more than %d classes", 160 * 1024 * 8);
-  const Scaling sc = scaling(softcap, inv_temp);
-  auto launch = [&](auto kernel, auto* z) -> int {
-    OB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-    kernel<<<(unsigned)rows, TP_THREADS, bytes, stream>>>(z, ld, teacher_ids, ids_64, teacher_log_probs, ld_t, k, renormalize,
-                                                          row_loss, row_stats, q, V, sc);
-    OB_CUDA_OK(cudaGetLastError());
-    return 0;
-  };
-  return dtype == OB_F32 ? launch(distill_fwd_kernel<float>, (const float*)logits)
-                         : launch(distill_fwd_kernel<bf16>, (const bf16*)logits);
+  const DistillArgs args{teacher_ids, teacher_log_probs, ids_64, k, renormalize, ld_t, row_loss, row_stats, q, V, scaling(softcap, inv_temp)};
+  if (dtype == OB_F32)
+    return softcap > 0.f ? launch_distill<float, 4, true>((const float*)logits, ld, rows, args, stream)
+                         : launch_distill<float, 4, false>((const float*)logits, ld, rows, args, stream);
+  return softcap > 0.f ? launch_distill<bf16, 2, true>((const bf16*)logits, ld, rows, args, stream)
+                       : launch_distill<bf16, 2, false>((const bf16*)logits, ld, rows, args, stream);
 }
 
 extern "C" int ob_distill_bwd(const void* logits, int dtype, long long ld, const void* teacher_ids, int ids_64, long long ld_t,
@@ -839,17 +1035,15 @@ extern "C" int ob_distill_bwd(const void* logits, int dtype, long long ld, const
   if (teacher_ids == nullptr || row_stats == nullptr || q == nullptr || dlogits == nullptr)
     OB_FAIL(-5, "distillation backward: missing tensor");
   const Scaling sc = scaling(softcap, inv_temp);
-#define OB_LAUNCH(T, D)                                                                                                   \
-  distill_bwd_kernel<T, D><<<(unsigned)rows, TP_THREADS, 0, stream>>>((const T*)logits, ld, teacher_ids, ids_64, ld_t, k, \
-                                                                      row_stats, q, g, stride_g, inv_count, scale,        \
-                                                                      (D*)dlogits, ld_d, V, sc)
-  if (dtype == OB_F32 && dtype_d == OB_F32) OB_LAUNCH(float, float);
-  else if (dtype == OB_F32 && dtype_d == OB_BF16) OB_LAUNCH(float, bf16);
-  else if (dtype == OB_BF16 && dtype_d == OB_BF16) OB_LAUNCH(bf16, bf16);
-  else OB_FAIL(-2, "distillation backward: no gradient of type %d for logits of type %d", dtype_d, dtype);
-#undef OB_LAUNCH
-  OB_CUDA_OK(cudaGetLastError());
-  return 0;
+  const DistillGradArgs args{teacher_ids, ids_64, k, ld_t, row_stats, q, g, stride_g, inv_count, scale, V, sc};
+  return launch_gradient("distillation backward", logits, dtype, ld, dlogits, dtype_d, ld_d, rows, V, stream,
+                         [&](auto* z, auto* d, int parts, int per_block) {
+    typedef std::remove_const_t<std::remove_pointer_t<decltype(z)>> T;
+    typedef std::remove_pointer_t<decltype(d)> D;
+    const unsigned blocks = (unsigned)(rows * parts);
+    if (softcap > 0.f) distill_bwd_kernel<T, D, true><<<blocks, GRAD_THREADS, 0, stream>>>(z, ld, d, ld_d, parts, per_block, args);
+    else distill_bwd_kernel<T, D, false><<<blocks, GRAD_THREADS, 0, stream>>>(z, ld, d, ld_d, parts, per_block, args);
+  });
 }
 
 extern "C" int ob_distill_reduce(const float* row_loss, const float* row_stats, long long rows, int mean, float* loss,
