@@ -38,26 +38,54 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// The capped logit cap(z) = softcap * tanh(z / softcap).  tanh(u) = 1 - 2 r and 1 - tanh^2(u) = 4 r (1 - r) with r = 1 / (1 + e^2u): two
-// hardware approximations, absolute error of the tanh below 2e-7 (the approximate tanh instruction's 5e-4 would show in every
-// log probability).
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// (fminf would drop a NaN)
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float z;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
+// The capped logit cap(z) = softcap * tanh(z / softcap).  tanh(u) = 1 - 2 r and 1 - tanh^2(u) = 4 r (1 - r) with r = 1 / a, a = 1 + e^2u: the
+// approximate tanh instruction's error of 5e-4 would show in every log probability, this form's is below 6e-7 (the roundings of r <= 1 and the
+// exponential's).  It takes two special-function operations beside the exponential of the softmax, of which an SM does sixteen a clock: they
+// bound the kernels.  So two classes share a reciprocal, 1 / (a b); a <= 2^30 changes no tanh and keeps the product finite.  What follows is
+// linear in r: t = (cap(z) - m) c is one multiply-add.
 struct Scaling {
-  float cap, inv_cap2;   // inv_cap2 = 2 log2(e) / cap
-  float c;               // log2(e) / T
+  float cap, k;     // k = 2 log2(e) / cap
+  float c;          // log2(e) / T
   float inv_temp;
-  // cap(z)
-  __device__ __forceinline__ float capped(float z) const {
-    return cap > 0.f ? cap * (1.f - 2.f * __fdividef(1.f, 1.f + exp2_fast(z * inv_cap2))) : z;
+
+  // f <- r of the logits f
+  template <int E>
+  __device__ __forceinline__ void reciprocals(float (&f)[E]) const {
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[j] = 1.f + exp2_fast(min_nan(f[j] * k, 30.f));
+#pragma unroll
+    for (int j = 0; j + 1 < E; j += 2) {
+      const float both = rcp_fast(f[j] * f[j + 1]), r = both * f[j + 1];
+      f[j + 1] = both * f[j];
+      f[j] = r;
+    }
+    if (E % 2) f[E - 1] = rcp_fast(f[E - 1]);
   }
-  // cap(z) and dy / dz
+  __device__ __forceinline__ float of_r(float r) const { return fmaf(-2.f * cap, r, cap); }
+  // one class, whether there is a cap or not: its capped logit, and dy / dz
   __device__ __forceinline__ float capped(float z, float* slope) const {
     *slope = inv_temp;
-    if (cap > 0.f) {
-      const float r = __fdividef(1.f, 1.f + exp2_fast(z * inv_cap2));
-      z = cap * (1.f - 2.f * r);
-      *slope *= 4.f * r * (1.f - r);
-    }
-    return z;
+    if (!(cap > 0.f)) return z;
+    float f[1] = {z};
+    reciprocals(f);
+    *slope *= 4.f * fmaf(-f[0], f[0], f[0]);
+    return of_r(f[0]);
+  }
+  __device__ __forceinline__ float capped(float z) const {
+    float slope;
+    return capped(z, &slope);
   }
 };
 
@@ -81,21 +109,28 @@ __device__ __forceinline__ Stats combine(Stats a, Stats b, float c) {
 }
 __device__ __forceinline__ bool no_class(Stats a) { return a.m == -INFINITY && a.s == 0.f; }   // (a NaN makes the sum NaN)
 
-// Adds E classes whose capped logits are f: their maximum first, then exponentials that do not wait for one another.  A masked
-// class (-inf) adds nothing: its exponent is kept finite where 0 * infinity would come up.
-template <bool W, int E>
-__device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], float c) {
+// Adds E classes of logits f: their maximum first, then exponentials that do not wait for one another.  A masked class (-inf) adds nothing: its
+// exponent is kept finite where 0 * infinity would come up.  With CAP f are the classes' r (infinite for one that is not there).
+template <bool CAP, bool W, int E>
+__device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], const Scaling& sc) {
   float mx = f[0];
 #pragma unroll
-  for (int j = 1; j < E; ++j) mx = fmaxf(mx, f[j]);
-  if (mx > a.m) a = shifted(a, mx, c);
+  for (int j = 1; j < E; ++j) mx = CAP ? fminf(mx, f[j]) : fmaxf(mx, f[j]);
+  if (CAP) mx = sc.of_r(mx);
+  if (mx > a.m) a = shifted(a, mx, sc.c);
   const float ref = a.m == -INFINITY ? 0.f : a.m;
+  const float t0 = (sc.cap - ref) * sc.c, t1 = -2.f * sc.cap * sc.c;
 #pragma unroll
   for (int j = 0; j < E; ++j) {
-    const float t = (f[j] - ref) * c, e = exp2_fast(t);
+    const float t = CAP ? fmaf(f[j], t1, t0) : (f[j] - ref) * sc.c, e = exp2_fast(t);
     a.s += e;
     if (W) a.w = fmaf(e, fmaxf(t, -FLT_MAX), a.w);
   }
+}
+// one class of capped logit y
+__device__ __forceinline__ void add_class(Stats& a, float y, const Scaling& sc) {
+  const float f[1] = {y};
+  add_classes<false, true, 1>(a, f, sc);
 }
 
 __device__ __forceinline__ Stats shuffle_combine(Stats a, int first, float c) {
@@ -176,7 +211,7 @@ __device__ __forceinline__ float key_logit(unsigned key) {
 // A batch of the row adds at most BATCH of them; before it there are at most KEEP.
 template <int BATCH>
 struct Candidates {
-  static constexpr int KEEP = 1024;
+  static constexpr int KEEP = 512;
   static constexpr int SIZE = KEEP + BATCH;
   unsigned key[SIZE];
   int cls[SIZE];
@@ -282,12 +317,13 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, unsigned x) {
 
 // Log probabilities, entropy and top classes.  A row belongs to a cluster of C CTAs (C = 1 but for few rows), a slice of its vectors to
 // each; the first CTA joins the slices' statistics and candidates through distributed shared memory.  Every thread has U 16-byte
-// loads in flight and takes the maximum of the batch before its exponentials.
+// loads in flight (TOP: those of the next batch) and takes the maximum of the batch before its exponentials.
 // Top classes in the same pass: from the first batch on, a class is a candidate if it is not below the k-th largest of the threads'
-// maxima over the first batch (a lower bound of the row's k-th largest logit that some k to 1.2 k classes of the batch reach); when
-// 1024 candidates have come together they are cut down, which raises the bound.  Most batches of a thread end at one comparison.
+// maxima over the first batch (a lower bound of the row's k-th largest logit that some k to 1.2 k classes of the batch reach).  Whenever 256 + 2 k
+// candidates have come together they are cut down, which raises the bound: the longer a row, the fewer batches have a candidate
+// at all, and a thread's batch ends at one comparison with its maximum.
 template <class T, int U, bool CAP, bool TOP>
-__global__ void __launch_bounds__(TP_THREADS, 3)
+__global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 2 : 3)
     token_log_probs_fwd_kernel(const T* __restrict__ logits, long long ld, int C, ScoreArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
   typedef Candidates<TP_THREADS * E + 2 * N> Cand;
@@ -300,6 +336,15 @@ __global__ void __launch_bounds__(TP_THREADS, 3)
   const int part = (int)(blockIdx.x - row * C);
   const Row<T> r(logits + row * ld, p.V);
   const int v0 = (int)((long long)r.nvec * part / C), v1 = (int)((long long)r.nvec * (part + 1) / C);
+  uint4 v[U];
+  auto load = [&](int b) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = b + k * TP_THREADS + threadIdx.x;
+      v[k] = i < v1 ? r.load(i) : no_vector<T>();
+    }
+  };
+  load(v0);
   float taken = 0.f;
   bool known = false;
   if (part == 0 && threadIdx.x == 0 && p.log_probs != nullptr) {
@@ -310,23 +355,19 @@ __global__ void __launch_bounds__(TP_THREADS, 3)
   Stats a = empty_stats();
   unsigned cut_key = 0;
   int cut_class = INT_MAX;
+  const int limit = 256 + 2 * p.top_k;   // <= Cand::KEEP
   if (TOP && threadIdx.x == 0) cand.n = 0;
   const int single = r.single(threadIdx.x, part == 0, part == C - 1);
   const float single_z = single >= 0 ? to_f(r.z[single]) : -INFINITY;
   if (single >= 0) {
-    const float f[1] = {CAP ? p.sc.capped(single_z) : single_z};
-    add_classes<true, 1>(a, f, p.sc.c);
+    add_class(a, CAP ? p.sc.capped(single_z) : single_z, p.sc);
   }
   for (int b = v0; b < v1 || (TOP && b == v0); b += TP_THREADS * U) {
-    uint4 v[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int i = b + k * TP_THREADS + threadIdx.x;
-      v[k] = i < v1 ? r.load(i) : no_vector<T>();
-    }
     float f[E];
+    if (!TOP && b > v0) load(b);
 #pragma unroll
     for (int k = 0; k < U; ++k) unpack<T>(v[k], f + k * N);
+    if (TOP) load(b + TP_THREADS * U);
     float mx = -INFINITY;
     if (TOP) {
 #pragma unroll
@@ -335,20 +376,20 @@ __global__ void __launch_bounds__(TP_THREADS, 3)
     if (CAP) {
       float y[E];
 #pragma unroll
-      for (int j = 0; j < E; ++j) y[j] = p.sc.capped(f[j]);
-      // (what is not there would come out as the lowest capped logit)
+      for (int j = 0; j < E; ++j) y[j] = f[j];
+      p.sc.reciprocals(y);
+      if (b + TP_THREADS * U > v1) {
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (b + k * TP_THREADS + (int)threadIdx.x >= v1) {
-#pragma unroll
-          for (int j = 0; j < N; ++j) y[k * N + j] = -INFINITY;
-        }
-      add_classes<true, E>(a, y, p.sc.c);
+        for (int j = 0; j < E; ++j)
+          if (b + j / N * TP_THREADS + (int)threadIdx.x >= v1) y[j] = INFINITY;
+      }
+      add_classes<true, true, E>(a, y, p.sc);
     } else {
-      add_classes<true, E>(a, f, p.sc.c);
+      add_classes<false, true, E>(a, f, p.sc);
     }
     if (TOP) {
-      const bool some = b + (int)threadIdx.x < v1;
+      const int first = b + (int)threadIdx.x;
+      const bool some = first < v1;
       const bool nan = a.s != a.s;   // a NaN, in this batch or before, comes first but is no maximum
       if (b == v0) {
         unsigned best = some ? order_key(mx) : 0u;
@@ -360,38 +401,29 @@ __global__ void __launch_bounds__(TP_THREADS, 3)
         cut_key = kth_of_threads(best, p.top_k);
       }
       int end = 0;
-      auto enter = [&](auto&& each) {   // each(visit): visit(logit, class) for every class there is
-        int add = 0;
-        each([&](float z, int i) {
-          const unsigned key = order_key(z);
-          add += key > cut_key || (key == cut_key && i <= cut_class);
-        });
-        if (add == 0) return;
-        int at = atomicAdd(&cand.n, add);
-        end = at + add;
-        each([&](float z, int i) {
-          const unsigned key = order_key(z);
-          if (key > cut_key || (key == cut_key && i <= cut_class)) {
-            cand.key[at] = key;
-            cand.cls[at] = i;
-            ++at;
-          }
-        });
+      auto enter = [&](float z, int i) {
+        const unsigned key = order_key(z);
+        if (key > cut_key || (key == cut_key && i <= cut_class)) {
+          const int at = atomicAdd(&cand.n, 1);
+          cand.key[at] = key;
+          cand.cls[at] = i;
+          end = at + 1;
+        }
       };
-      if (some && (nan || order_key(mx) >= cut_key))
-        enter([&](auto visit) {
+      // Behind the cut's class a logit has to be above the cut's.  (The bound of a cut_key of 0 is NaN, below which nothing is.)
+      const float bound = key_logit(cut_key + (cut_key > 0 && r.class_of(first) > cut_class ? 1u : 0u));
+      if (some && (nan || !(mx < bound))) {
+        unsigned over = 0;
 #pragma unroll
-          for (int k = 0; k < U; ++k) {
-            const int i = b + k * TP_THREADS + threadIdx.x;
-            if (i < v1) {
-#pragma unroll
-              for (int j = 0; j < N; ++j) visit(f[k * N + j], r.class_of(i) + j);
-            }
-          }
-        });
-      if (b == v0 && single >= 0) enter([&](auto visit) { visit(single_z, single); });
+        for (int j = 0; j < E; ++j) over |= !(f[j] < bound) && first + j / N * TP_THREADS < v1 ? 1u << j : 0u;
+        for (; over != 0; over &= over - 1) {   // few: read again
+          const int j = __ffs(over) - 1, i = r.class_of(first + j / N * TP_THREADS) + j % N;
+          enter(to_f(r.z[i]), i);
+        }
+      }
+      if (b == v0 && single >= 0) enter(single_z, single);
       // (every thread's last candidate, not the counter: a faster thread may already be adding to that)
-      if (__syncthreads_or(end > Cand::KEEP)) compact(cand, cand.n, p.top_k, Cand::KEEP / 2, cut_key, cut_class);
+      if (__syncthreads_or(end > limit)) compact(cand, cand.n, p.top_k, limit / 2, cut_key, cut_class);
     }
   }
   a = block_combine(a, red, p.sc.c);
@@ -400,8 +432,8 @@ __global__ void __launch_bounds__(TP_THREADS, 3)
     // the slice's first k classes in order
     int n = cand.n;
     __syncthreads();
-    if (n > TP_THREADS / 2) {
-      compact(cand, n, p.top_k, TP_THREADS, cut_key, cut_class);
+    if (n > limit / 2) {
+      compact(cand, n, p.top_k, limit / 2, cut_key, cut_class);
       n = cand.n;
     }
     uint32_t keys = smem_u32(slices.key[part]), classes = smem_u32(slices.cls[part]);
@@ -494,7 +526,8 @@ __device__ __forceinline__ void store_vector<bf16, 8>(bf16* d, const float (&g)[
   *reinterpret_cast<uint4*>(d) = make_uint4(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7]));
 }
 
-// The span `part` of `per_block` vectors of a row and its gradient: d[i] = grad(z[i], i) for its classes [lo, hi), which it returns.
+// The span `part` of `per_block` vectors of a row and its gradient, for the classes [lo, hi), which it returns: grad(f, i) turns
+// an array f of the logits of classes i, i + 1, ... into their gradients.
 // The gradient is written in vectors where its row is aligned like the logits', else class by class.
 template <class T, class D, class F>
 __device__ __forceinline__ int2 map_span(const T* z, D* d, int V, int part, int parts, int per_block, F grad) {
@@ -503,7 +536,11 @@ __device__ __forceinline__ int2 map_span(const T* z, D* d, int V, int part, int 
   const int v0 = min(r.nvec, part * per_block), v1 = part == parts - 1 ? r.nvec : min(r.nvec, v0 + per_block);
   const int lo = part == 0 ? 0 : r.class_of(v0), hi = part == parts - 1 ? V : r.class_of(v1);
   if ((reinterpret_cast<uintptr_t>(d + r.head) & (N * sizeof(D) - 1)) != 0) {
-    for (int i = lo + threadIdx.x; i < hi; i += GRAD_THREADS) d[i] = from_f<D>(grad(to_f(z[i]), i));
+    for (int i = lo + threadIdx.x; i < hi; i += GRAD_THREADS) {
+      float f[1] = {to_f(z[i])};
+      grad(f, i);
+      d[i] = from_f<D>(f[0]);
+    }
     return make_int2(lo, hi);
   }
   for (int b = v0 + threadIdx.x; b < v1; b += GRAD_THREADS * GRAD_UNROLL) {
@@ -518,13 +555,16 @@ __device__ __forceinline__ int2 map_span(const T* z, D* d, int V, int part, int 
       float f[N];
       unpack<T>(v[k], f);
       const int cls = r.class_of(i);
-#pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = grad(f[j], cls + j);
+      grad(f, cls);
       store_vector<D, N>(d + cls, f);
     }
   }
   const int single = r.single(threadIdx.x, part == 0, part == parts - 1);
-  if (single >= 0) d[single] = from_f<D>(grad(to_f(z[single]), single));
+  if (single >= 0) {
+    float f[1] = {to_f(z[single])};
+    grad(f, single);
+    d[single] = from_f<D>(f[0]);
+  }
   return make_int2(lo, hi);
 }
 
@@ -544,7 +584,7 @@ __global__ void __launch_bounds__(GRAD_THREADS)
                                int per_block, ScoreGradArgs p) {
   const long long row = blockIdx.x / (unsigned)parts;
   const int part = (int)(blockIdx.x - row * parts);
-  const float2 norm = p.norm[row];
+  float2 norm = p.norm[row];
   const float ge = p.g_entropy != nullptr ? p.g_entropy[row * p.stride_ent] : 0.f;
   float gl = 0.f;
   int id = -1;
@@ -555,18 +595,25 @@ __global__ void __launch_bounds__(GRAD_THREADS)
       id = (int)i;
     }
   }
-  const bool none = norm.x == -INFINITY && norm.y == -INFINITY;
-  const float scale = CAP ? 1.f : p.sc.inv_temp;
-  const float k0 = (gl + ge * (ge != 0.f ? p.entropy[row] : 0.f)) * scale, k1 = ge * LN2 * scale;
-  gl *= scale;
-  map_span<T, D>(logits + row * ld, dlogits + row * ld_d, p.V, part, parts, per_block, [&](float z, int i) {
-    float slope = 1.f;
-    if (CAP) z = p.sc.capped(z, &slope);
-    const float t = (z - norm.x) * p.sc.c - norm.y, e = exp2_fast(t);
-    // (2^t is 0 from -150 on; what it is multiplied by stays finite)
-    float g = -e * fmaf(k1, fmaxf(t, -1024.f), k0);
-    if (i == id) g += gl;
-    return none ? 0.f : g * slope;
+  float k0 = (gl + ge * (ge != 0.f ? p.entropy[row] : 0.f)) * p.sc.inv_temp, k1 = ge * LN2 * p.sc.inv_temp;
+  gl *= p.sc.inv_temp;
+  if (norm.x == -INFINITY && norm.y == -INFINITY) {   // no class: exponents of -inf and factors of 0
+    norm = make_float2(0.f, 0.f);
+    k0 = k1 = gl = 0.f;
+  }
+  if (CAP) k0 *= 4.f, k1 *= 4.f, gl *= 4.f;   // of the slope 4 r (1 - r)
+  const float t0 = (p.sc.cap - norm.x) * p.sc.c - norm.y, t1 = -2.f * p.sc.cap * p.sc.c;
+  map_span<T, D>(logits + row * ld, dlogits + row * ld_d, p.V, part, parts, per_block, [&](auto& f, int i) {
+    constexpr int M = sizeof(f) / sizeof(float);
+    if (CAP) p.sc.reciprocals(f);
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const float t = CAP ? fmaf(f[j], t1, t0) : fmaf(f[j] - norm.x, p.sc.c, -norm.y), e = exp2_fast(t);
+      // (2^t is 0 from -150 on; what it is multiplied by stays finite)
+      float g = -e * fmaf(k1, fmaxf(t, -1024.f), k0);
+      if (i + j == id) g += gl;
+      f[j] = CAP ? g * fmaf(-f[j], f[j], f[j]) : g;
+    }
   });
 }
 
@@ -618,9 +665,8 @@ __device__ __forceinline__ void distill_row(const Pairs& pairs, Stats others_sta
     const int i = n * 32 + lane;
     in[n] = i < p.k && pairs.cls[i] >= 0;
     t[n] = in[n] ? pairs.t[i] : -INFINITY;
-    const float f[1] = {in[n] ? pairs.y[i] : -INFINITY};
-    y[n] = f[0];
-    if (in[n]) add_classes<false, 1>(st, f, p.sc.c);
+    y[n] = in[n] ? pairs.y[i] : -INFINITY;
+    if (in[n]) add_class(st, y[n], p.sc);
     t_max = fmaxf(t_max, t[n]);
     any |= in[n] && !(p.renormalize && t[n] == -INFINITY);
   }
@@ -669,7 +715,7 @@ __device__ __forceinline__ void distill_row(const Pairs& pairs, Stats others_sta
 // A row belongs to a cluster of C CTAs as in the log probabilities.  A bit of shared memory per class of the slice says which the teacher
 // names; four or eight of them, one vector's, cost one look per 16 bytes.
 template <class T, int U, bool CAP>
-__global__ void __launch_bounds__(TP_THREADS, 3)
+__global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
     distill_fwd_kernel(const T* __restrict__ logits, long long ld, int C, DistillArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
   extern __shared__ __align__(16) char shared_bytes[];
@@ -719,8 +765,7 @@ __global__ void __launch_bounds__(TP_THREADS, 3)
   Stats a = empty_stats();
   const int single = r.single(threadIdx.x, part == 0, part == C - 1);
   if (single >= 0 && !((named[(single + shift) >> 5] >> ((single + shift) & 31)) & 1)) {
-    const float f[1] = {p.sc.capped(to_f(r.z[single]))};
-    add_classes<false, 1>(a, f, p.sc.c);
+    add_class(a, p.sc.capped(to_f(r.z[single])), p.sc);
   }
   for (int b = v0; b < v1; b += TP_THREADS * U) {
     uint4 v[U];
@@ -739,17 +784,17 @@ __global__ void __launch_bounds__(TP_THREADS, 3)
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       unpack<T>(v[k], f + k * N);
-      if (CAP) {
+    }
+    if (CAP) p.sc.reciprocals(f);
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[k * N + j] = p.sc.capped(f[k * N + j]);
-      }
+    for (int k = 0; k < U; ++k) {
       if (out[k]) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          if ((out[k] >> j) & 1) f[k * N + j] = -INFINITY;
+          if ((out[k] >> j) & 1) f[k * N + j] = CAP ? INFINITY : -INFINITY;
       }
     }
-    add_classes<false, E>(a, f, p.sc.c);
+    add_classes<CAP, false, E>(a, f, p.sc);
   }
   a = block_combine(a, red, p.sc.c);
   if (C > 1) {
@@ -799,11 +844,16 @@ __global__ void __launch_bounds__(GRAD_THREADS)
   const float gs = (p.g != nullptr ? p.g[row * p.stride_g] : 1.f) * p.scale * (p.inv_count != nullptr ? *p.inv_count : 1.f);
   const bool nothing = st.x < 0.f || (norm.x == -INFINITY && norm.y == -INFINITY);
   const bool zero = nothing || (norm.z == -INFINITY && norm.w == -INFINITY);   // no class outside the teacher's
-  const float coef = st.y * gs * (CAP ? 1.f : p.sc.inv_temp);
-  const int2 span = map_span<T, D>(z, d, p.V, part, parts, per_block, [&](float x, int) {
-    float slope = 1.f;
-    if (CAP) x = p.sc.capped(x, &slope);
-    return zero ? 0.f : exp2_fast((x - norm.z) * p.sc.c - norm.w) * coef * slope;
+  const float coef = st.y * gs * p.sc.inv_temp * (CAP ? 4.f : 1.f);
+  const float t0 = (p.sc.cap - norm.z) * p.sc.c - norm.w, t1 = -2.f * p.sc.cap * p.sc.c;
+  const int2 span = map_span<T, D>(z, d, p.V, part, parts, per_block, [&](auto& f, int) {
+    constexpr int M = sizeof(f) / sizeof(float);
+    if (CAP) p.sc.reciprocals(f);
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const float g = exp2_fast(CAP ? fmaf(f[j], t1, t0) : fmaf(f[j] - norm.z, p.sc.c, -norm.w)) * coef;
+      f[j] = zero ? 0.f : CAP ? g * fmaf(-f[j], f[j], f[j]) : g;
+    }
   });
   // the teacher's classes, over what has just been written for them
   __syncthreads();
@@ -890,11 +940,11 @@ static inline int allow_shared(K kernel, int bytes, bool (&done)[64]) {
   return 0;
 }
 
-// CTAs per row: a power of two up to the portable cluster size, as long as all CTAs run at once (three per SM) and a slice keeps a batch
+// CTAs per row: a power of two up to the portable cluster size, as long as all CTAs run at once (two per SM) and a slice keeps a batch
 // or more of every thread.
 static inline int ctas_per_row(long long rows, int V, int per_batch) {
   int C = 1;
-  while (C < 8 && rows * C * 2 <= 3ll * sm_count() && V / (2 * C) >= per_batch) C *= 2;
+  while (C < 8 && rows * C * 2 <= 2ll * sm_count() && V / (2 * C) >= per_batch) C *= 2;
   return C;
 }
 
@@ -979,11 +1029,11 @@ extern "C" int ob_token_log_probs_fwd(const void* logits, int dtype, long long l
   const bool cap = softcap > 0.f, top = top_k > 0;
   if (dtype == OB_F32) {
     auto* z = (const float*)logits;
-    if (top) return cap ? launch_scores<float, 2, true, true>(z, ld, rows, args, stream) : launch_scores<float, 2, false, true>(z, ld, rows, args, stream);
+    if (top) return cap ? launch_scores<float, 4, true, true>(z, ld, rows, args, stream) : launch_scores<float, 4, false, true>(z, ld, rows, args, stream);
     return cap ? launch_scores<float, 4, true, false>(z, ld, rows, args, stream) : launch_scores<float, 4, false, false>(z, ld, rows, args, stream);
   }
   auto* z = (const bf16*)logits;
-  if (top) return cap ? launch_scores<bf16, 1, true, true>(z, ld, rows, args, stream) : launch_scores<bf16, 1, false, true>(z, ld, rows, args, stream);
+  if (top) return cap ? launch_scores<bf16, 2, true, true>(z, ld, rows, args, stream) : launch_scores<bf16, 2, false, true>(z, ld, rows, args, stream);
   return cap ? launch_scores<bf16, 2, true, false>(z, ld, rows, args, stream) : launch_scores<bf16, 2, false, false>(z, ld, rows, args, stream);
 }
 
