@@ -109,14 +109,18 @@ __device__ __forceinline__ Stats combine(Stats a, Stats b, float c) {
 }
 __device__ __forceinline__ bool no_class(Stats a) { return a.m == -INFINITY && a.s == 0.f; }   // (a NaN makes the sum NaN)
 
-// Adds E classes of logits f: their maximum first, then exponentials that do not wait for one another.  A masked class (-inf) adds nothing: its
-// exponent is kept finite where 0 * infinity would come up.  With CAP f are the classes' r (infinite for one that is not there).
-template <bool CAP, bool W, int E>
-__device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], const Scaling& sc) {
+template <int E>
+__device__ __forceinline__ float largest(const float (&f)[E]) {
   float mx = f[0];
 #pragma unroll
-  for (int j = 1; j < E; ++j) mx = CAP ? fminf(mx, f[j]) : fmaxf(mx, f[j]);
-  if (CAP) mx = sc.of_r(mx);
+  for (int j = 1; j < E; ++j) mx = fmaxf(mx, f[j]);
+  return mx;
+}
+// Adds E classes of logits f with the largest (capped) logit mx, known first so that the exponentials do not wait for one another.  A masked class
+// (-inf) adds nothing: its exponent is kept finite where 0 * infinity would come up.  With CAP f are the classes' r (infinite for one that is
+// not there).
+template <bool CAP, bool W, int E>
+__device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], float mx, const Scaling& sc) {
   if (mx > a.m) a = shifted(a, mx, sc.c);
   const float ref = a.m == -INFINITY ? 0.f : a.m;
   const float t0 = (sc.cap - ref) * sc.c, t1 = -2.f * sc.cap * sc.c;
@@ -130,7 +134,7 @@ __device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], const
 // one class of capped logit y
 __device__ __forceinline__ void add_class(Stats& a, float y, const Scaling& sc) {
   const float f[1] = {y};
-  add_classes<false, true, 1>(a, f, sc);
+  add_classes<false, true, 1>(a, f, y, sc);
 }
 
 __device__ __forceinline__ Stats shuffle_combine(Stats a, int first, float c) {
@@ -193,6 +197,17 @@ __device__ __forceinline__ uint4 no_vector() {
   const unsigned u = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
   return make_uint4(u, u, u, u);
 }
+// the vectors first, first + TP_THREADS, ... below `end`; `whole`: the batch has all of them, for every thread
+template <class T, int U>
+__device__ __forceinline__ void load_batch(const Row<T>& r, int first, bool whole, int end, uint4 (&v)[U]) {
+  if (whole) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = r.load(first + k * TP_THREADS);
+  } else {
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = first + k * TP_THREADS < end ? r.load(first + k * TP_THREADS) : no_vector<T>();
+  }
+}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Top classes.  Order of the classes: larger logits first (NaN before all, -0 equal to 0), then lower classes.
@@ -207,15 +222,18 @@ __device__ __forceinline__ float key_logit(unsigned key) {
 }
 // Every class has a key above 0.
 
-// A row's (or slice's) candidates in shared memory.  A class enters if it does not come after (cut_key, cut_class); `n` have.
-// A batch of the row adds at most BATCH of them; before it there are at most KEEP.
-template <int BATCH>
-struct Candidates {
-  static constexpr int KEEP = 512;
-  static constexpr int SIZE = KEEP + BATCH;
-  unsigned key[SIZE];
-  int cls[SIZE];
-  int n, kept;
+// What a row's (or slice's) top classes are found from, in shared memory.  The row is read in batches; what a thread reads of a batch is a group,
+// known by its largest logit.  Group g is the batch g / TP_THREADS of thread g % TP_THREADS.
+struct TopWork {
+  static constexpr int LIMIT = TP_THREADS + 2 * OB_TOP_K_MAX;   // groups kept from one batch to the next
+  static constexpr int GROUPS = LIMIT + TP_THREADS;             // ... and those of one batch
+  static constexpr int STEP = 192;
+  static constexpr int CLASSES = 1024;
+  unsigned group_key[GROUPS];
+  int group[GROUPS];
+  unsigned key[CLASSES];
+  int cls[CLASSES];
+  int groups, classes, kept;
   int red[2][TP_THREADS / 32];
 };
 
@@ -226,66 +244,124 @@ __device__ __forceinline__ int block_sum(int c, int* red) {
   return __reduce_add_sync(0xffffffffu, (threadIdx.x & 31) < TP_THREADS / 32 ? red[threadIdx.x & 31] : 0);
 }
 
-// Drops candidates that are certainly not among the first k of the n there are, and lowers the cut to what is kept: the k-th largest
-// key is searched bit by bit, 16 bits first, which leaves little more than k unless many logits are nearly equal; then the
-// other bits, then classes.  At most `most` (>= k) are kept.  All threads call it; it begins and ends with the block in step.
-template <class C>
-__device__ void compact(C& c, int n, int k, int most, unsigned& cut_key, int& cut_class) {
-  int turn = 0;
-  auto count = [&](auto pred) {
-    int x = 0;
-    for (int i = threadIdx.x; i < n; i += TP_THREADS) x += pred(c.key[i], c.cls[i]);
-    turn ^= 1;   // (two buffers: a thread is at most one sum ahead of the slowest reader)
-    return block_sum(x, c.red[turn]);
-  };
-  unsigned key = 0;
-  int stays = n;
-  for (int bit = 31; bit >= 0 && stays > k; --bit) {
-    if (bit == 15 && stays <= most) break;
+// The k-th in order of the members that count(pred) counts with pred(key, place): its key and the last place of that key among the first k.
+// There are k of them.  All threads call it.
+template <class F>
+__device__ void kth_in_order(F count, int k, unsigned& key, int& place) {
+  key = 0;
+  for (int bit = 31; bit >= 0; --bit) {
     const unsigned next = key | (1u << bit);
-    const int x = count([&](unsigned q, int) { return q >= next; });
-    if (x >= k) key = next, stays = x;
+    if (count([&](unsigned q, int) { return q >= next; }) >= k) key = next;
   }
-  int cls = INT_MAX;
-  if (stays > most) {
-    // every bit of the key is fixed: more than `most` classes at or above it, so ties at it
-    const int above = count([&](unsigned q, int) { return q > key; });
-    int low = 0;   // fewer than k - above classes of that key lie below `low`
-    for (int bit = 30; bit >= 0; --bit) {
-      const int next = low | (1 << bit);
-      if (count([&](unsigned q, int i) { return q == key && i < next; }) < k - above) low = next;
-    }
-    cls = low;
+  const int above = count([&](unsigned q, int) { return q > key; });
+  place = 0;
+  for (int bit = 30; bit >= 0; --bit) {
+    const int next = place | (1 << bit);
+    if (count([&](unsigned q, int i) { return q == key && i < next; }) < k - above) place = next;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) c.kept = 0;
-  // in place: a candidate moves to where an earlier chunk, or its own, has been read
+}
+
+// The groups of a batch have been too many (rising logits, or the same ones over and over): drops those that hold none of the first k classes.  The
+// k-th largest of the groups' maxima is a bound that k classes reach, none of them behind the batch up to which k groups reach it;
+// groups of later batches have to be above it.  What stays are fewer than k groups above, fewer than k at the bound of earlier batches
+// and the groups of one batch; their number is returned.
+__device__ __noinline__ int drop_groups(TopWork& w, int k, unsigned& cut) {
+  const int n = w.groups;
+  int turn = 0;
+  unsigned key;
+  int batch;
+  kth_in_order(
+      [&](auto pred) {
+        int x = 0;
+        for (int i = threadIdx.x; i < n; i += TP_THREADS) x += pred(w.group_key[i], w.group[i] / TP_THREADS);
+        turn ^= 1;   // (two buffers: a thread is at most one sum ahead of the slowest reader)
+        return block_sum(x, w.red[turn]);
+      },
+      k, key, batch);
+  if (threadIdx.x == 0) w.kept = 0;
+  // in place: a group moves to where an earlier chunk, or its own, has been read
   for (int i0 = 0; i0 < n; i0 += TP_THREADS) {
     const int i = i0 + threadIdx.x;
-    const unsigned q = i < n ? c.key[i] : 0u;
-    const int j = i < n ? c.cls[i] : INT_MAX;
+    const unsigned q = i < n ? w.group_key[i] : 0u;
+    const int g = i < n ? w.group[i] : 0;
     __syncthreads();
-    if (i < n && (q > key || (q == key && j <= cls))) {
-      const int at = atomicAdd(&c.kept, 1);
-      c.key[at] = q;
-      c.cls[at] = j;
+    if (i < n && (q > key || (q == key && g / TP_THREADS <= batch))) {
+      const int at = atomicAdd(&w.kept, 1);
+      w.group_key[at] = q;
+      w.group[at] = g;
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) c.n = c.kept;
-  if (key > cut_key || (key == cut_key && cls < cut_class)) cut_key = key, cut_class = cls;
+  if (threadIdx.x == 0) w.groups = w.kept;
+  cut = max(cut, key);
   __syncthreads();
+  return w.kept;
 }
 
 // A lower bound of the k-th largest of one key per thread (0: none), exact in its upper 16 bits.
 __device__ __forceinline__ unsigned kth_of_threads(unsigned key, int k) {
   unsigned cut = 0;
-#pragma unroll 1
+#pragma unroll
   for (int bit = 31; bit >= 16; --bit) {
     const unsigned next = cut | (1u << bit);
     if (__syncthreads_count(key >= next) >= k) cut = next;
   }
   return cut;
+}
+
+// The classes of the groups at or above `cut` that reach it themselves, and those of the row's head and tail (`single` of this thread, or -1), as
+// w.key / w.cls: at most CLASSES, and the first k among them.  Returns how many.
+template <class T, int U>
+__device__ int collect_classes(TopWork& w, const Row<T>& r, int v0, int v1, int single, int k, unsigned cut) {
+  constexpr int N = Row<T>::N;
+  const int n = w.groups;
+  // visit(key, class) for this thread's share of the classes
+  auto each = [&](auto visit) {
+    for (int t = threadIdx.x; t < n * U; t += TP_THREADS) {
+      if (w.group_key[t / U] < cut) continue;
+      const int g = w.group[t / U], vec = v0 + (g / TP_THREADS * U + t % U) * TP_THREADS + g % TP_THREADS;
+      if (vec >= v1) continue;
+      float f[N];
+      unpack<T>(r.load(vec), f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) visit(order_key(f[j]), r.class_of(vec) + j);
+    }
+    if (single >= 0) visit(order_key(to_f(r.z[single])), single);
+  };
+  if (threadIdx.x == 0) w.classes = 0;
+  __syncthreads();
+  each([&](unsigned key, int i) {
+    if (key < cut) return;
+    const int at = atomicAdd(&w.classes, 1);
+    if (at < TopWork::CLASSES) {
+      w.key[at] = key;
+      w.cls[at] = i;
+    }
+  });
+  __syncthreads();
+  int found = w.classes;
+  if (found <= TopWork::CLASSES) return found;
+  // more equal or nearly equal logits than there is room for: the k-th class exactly, then the first k
+  unsigned key;
+  int cls, turn = 0;
+  kth_in_order(
+      [&](auto pred) {
+        int x = 0;
+        each([&](unsigned q, int i) { x += pred(q, i); });
+        turn ^= 1;
+        return block_sum(x, w.red[turn]);
+      },
+      k, key, cls);
+  if (threadIdx.x == 0) w.classes = 0;
+  __syncthreads();
+  each([&](unsigned q, int i) {
+    if (q < key || (q == key && i > cls)) return;
+    const int at = atomicAdd(&w.classes, 1);
+    w.key[at] = q;
+    w.cls[at] = i;
+  });
+  __syncthreads();
+  return w.classes;
 }
 
 struct ScoreArgs {
@@ -316,19 +392,20 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, unsigned x) {
 }
 
 // Log probabilities, entropy and top classes.  A row belongs to a cluster of C CTAs (C = 1 but for few rows), a slice of its vectors to
-// each; the first CTA joins the slices' statistics and candidates through distributed shared memory.  Every thread has U 16-byte
-// loads in flight (TOP: those of the next batch) and takes the maximum of the batch before its exponentials.
-// Top classes in the same pass: from the first batch on, a class is a candidate if it is not below the k-th largest of the threads'
-// maxima over the first batch (a lower bound of the row's k-th largest logit that some k to 1.2 k classes of the batch reach).  Whenever 256 + 2 k
-// candidates have come together they are cut down, which raises the bound: the longer a row, the fewer batches have a candidate
-// at all, and a thread's batch ends at one comparison with its maximum.
+// each; the first CTA joins the slices' statistics and top classes through distributed shared memory.  Every thread has U 16-byte
+// loads in flight (AHEAD: those of the next batch) and takes the maximum of the batch before its exponentials.
+// Top classes in the same pass, at one comparison per thread and batch: a group (TopWork) is kept if its largest logit is above `cut`, a
+// lower bound of the row's k-th largest logit that k classes of earlier batches reach, so that no class of a later one at the bound is among the
+// first k.  The bound is the k-th largest of the threads' maxima so far, which no more than 1.2 k classes reach if they are spread over the
+// threads by chance; it is looked for at the first batch, whenever STEP more groups have come together, and at the end, when the
+// classes of the groups above it are read again and put in order.
 template <class T, int U, bool CAP, bool TOP>
-__global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 2 : 3)
+__global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
     token_log_probs_fwd_kernel(const T* __restrict__ logits, long long ld, int C, ScoreArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
-  typedef Candidates<TP_THREADS * E + 2 * N> Cand;
+  constexpr bool AHEAD = CAP;
   extern __shared__ __align__(16) char shared_bytes[];
-  Cand& cand = *reinterpret_cast<Cand*>(shared_bytes);
+  TopWork& work = *reinterpret_cast<TopWork*>(shared_bytes);   // TOP
   __shared__ Stats red[TP_THREADS / 32];
   __shared__ Slices slices;
   if (C > 1) cluster_arrive();
@@ -337,13 +414,7 @@ __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 2 : 3)
   const Row<T> r(logits + row * ld, p.V);
   const int v0 = (int)((long long)r.nvec * part / C), v1 = (int)((long long)r.nvec * (part + 1) / C);
   uint4 v[U];
-  auto load = [&](int b) {
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int i = b + k * TP_THREADS + threadIdx.x;
-      v[k] = i < v1 ? r.load(i) : no_vector<T>();
-    }
-  };
+  auto load = [&](int b) { load_batch<T, U>(r, b + threadIdx.x, b + TP_THREADS * U <= v1, v1, v); };
   load(v0);
   float taken = 0.f;
   bool known = false;
@@ -353,26 +424,19 @@ __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 2 : 3)
     if (known) taken = to_f(r.z[id]);
   }
   Stats a = empty_stats();
-  unsigned cut_key = 0;
-  int cut_class = INT_MAX;
-  const int limit = 256 + 2 * p.top_k;   // <= Cand::KEEP
-  if (TOP && threadIdx.x == 0) cand.n = 0;
+  unsigned cut = 0, best = 0;
+  int limit = TopWork::STEP;
+  if (TOP && threadIdx.x == 0) work.groups = 0;
+  if (TOP) __syncthreads();
   const int single = r.single(threadIdx.x, part == 0, part == C - 1);
-  const float single_z = single >= 0 ? to_f(r.z[single]) : -INFINITY;
-  if (single >= 0) {
-    add_class(a, CAP ? p.sc.capped(single_z) : single_z, p.sc);
-  }
-  for (int b = v0; b < v1 || (TOP && b == v0); b += TP_THREADS * U) {
+  if (single >= 0) add_class(a, p.sc.capped(to_f(r.z[single])), p.sc);
+  for (int b = v0, batch = 0; b < v1; b += TP_THREADS * U, ++batch) {
     float f[E];
-    if (!TOP && b > v0) load(b);
+    if (!AHEAD && b > v0) load(b);
 #pragma unroll
     for (int k = 0; k < U; ++k) unpack<T>(v[k], f + k * N);
-    if (TOP) load(b + TP_THREADS * U);
-    float mx = -INFINITY;
-    if (TOP) {
-#pragma unroll
-      for (int j = 0; j < E; ++j) mx = fmaxf(mx, f[j]);
-    }
+    if (AHEAD) load(b + TP_THREADS * U);
+    const float mx = largest(f);
     if (CAP) {
       float y[E];
 #pragma unroll
@@ -383,69 +447,55 @@ __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 2 : 3)
         for (int j = 0; j < E; ++j)
           if (b + j / N * TP_THREADS + (int)threadIdx.x >= v1) y[j] = INFINITY;
       }
-      add_classes<true, true, E>(a, y, p.sc);
+      add_classes<true, true, E>(a, y, b + (int)threadIdx.x < v1 ? p.sc.capped(mx) : -INFINITY, p.sc);
     } else {
-      add_classes<false, true, E>(a, f, p.sc);
+      add_classes<false, true, E>(a, f, mx, p.sc);
     }
     if (TOP) {
-      const int first = b + (int)threadIdx.x;
-      const bool some = first < v1;
-      const bool nan = a.s != a.s;   // a NaN, in this batch or before, comes first but is no maximum
-      if (b == v0) {
-        unsigned best = some ? order_key(mx) : 0u;
-        if (nan) {
-#pragma unroll
-          for (int j = 0; j < E; ++j) best = max(best, f[j] != f[j] ? 0xffffffffu : 0u);
+      const int first = b + threadIdx.x;
+      unsigned key = first < v1 ? order_key(mx) : 0u;
+      if (a.s != a.s) {   // a NaN, in this batch or before, comes first but is no maximum
+        for (int k = 0; k < U && first + k * TP_THREADS < v1; ++k) {
+          float x[N];
+          unpack<T>(r.load(first + k * TP_THREADS), x);
+          for (int j = 0; j < N; ++j)
+            if (x[j] != x[j]) key = 0xffffffffu;
         }
-        if (single >= 0) best = max(best, order_key(single_z));
-        cut_key = kth_of_threads(best, p.top_k);
       }
+      best = max(best, key);
+      if (b == v0) cut = kth_of_threads(best, p.top_k);
       int end = 0;
-      auto enter = [&](float z, int i) {
-        const unsigned key = order_key(z);
-        if (key > cut_key || (key == cut_key && i <= cut_class)) {
-          const int at = atomicAdd(&cand.n, 1);
-          cand.key[at] = key;
-          cand.cls[at] = i;
-          end = at + 1;
-        }
-      };
-      // Behind the cut's class a logit has to be above the cut's.  (The bound of a cut_key of 0 is NaN, below which nothing is.)
-      const float bound = key_logit(cut_key + (cut_key > 0 && r.class_of(first) > cut_class ? 1u : 0u));
-      if (some && (nan || !(mx < bound))) {
-        unsigned over = 0;
-#pragma unroll
-        for (int j = 0; j < E; ++j) over |= !(f[j] < bound) && first + j / N * TP_THREADS < v1 ? 1u << j : 0u;
-        for (; over != 0; over &= over - 1) {   // few: read again
-          const int j = __ffs(over) - 1, i = r.class_of(first + j / N * TP_THREADS) + j % N;
-          enter(to_f(r.z[i]), i);
-        }
+      if (b == v0 ? key != 0u && key >= cut : key > cut) {
+        const int at = atomicAdd(&work.groups, 1);
+        work.group_key[at] = key;
+        work.group[at] = batch * TP_THREADS + threadIdx.x;
+        end = at + 1;
       }
-      if (b == v0 && single >= 0) enter(single_z, single);
-      // (every thread's last candidate, not the counter: a faster thread may already be adding to that)
-      if (__syncthreads_or(end > limit)) compact(cand, cand.n, p.top_k, limit / 2, cut_key, cut_class);
+      // (every thread's last group, not the counter: a faster thread may already be adding to that)
+      if (__syncthreads_or(end > limit)) {
+        int n = work.groups;
+        if (n > TopWork::LIMIT) n = drop_groups(work, p.top_k, cut);
+        else cut = max(cut, kth_of_threads(best, p.top_k));
+        limit = min(n + TopWork::STEP, TopWork::LIMIT);
+      }
     }
   }
+  if (TOP) cut = max(cut, kth_of_threads(best, p.top_k));
   a = block_combine(a, red, p.sc.c);
   if (C > 1) cluster_wait();   // the first CTA runs
   if (TOP) {
     // the slice's first k classes in order
-    int n = cand.n;
-    __syncthreads();
-    if (n > limit / 2) {
-      compact(cand, n, p.top_k, limit / 2, cut_key, cut_class);
-      n = cand.n;
-    }
+    const int n = collect_classes<T, U>(work, r, v0, v1, single, p.top_k, cut);
     uint32_t keys = smem_u32(slices.key[part]), classes = smem_u32(slices.cls[part]);
     if (C > 1) {
       keys = mapa_shared(keys, 0);
       classes = mapa_shared(classes, 0);
     }
     for (int t = threadIdx.x; t < n; t += TP_THREADS) {
-      const unsigned key = cand.key[t];
-      const int i = cand.cls[t];
+      const unsigned key = work.key[t];
+      const int i = work.cls[t];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += cand.key[j] > key || (cand.key[j] == key && cand.cls[j] < i);
+      for (int j = 0; j < n; ++j) rank += work.key[j] > key || (work.key[j] == key && work.cls[j] < i);
       if (rank < p.top_k) {
         store_cluster(keys + rank * 4, key);
         store_cluster(classes + rank * 4, (unsigned)i);
@@ -508,7 +558,7 @@ __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 2 : 3)
 // ---------------------------------------------------------------------------------------------------------------------
 // Gradients: every class's from its logit and a few numbers of the row.  A block takes a span of a row, blocks in launch order.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int GRAD_THREADS = 256, GRAD_UNROLL = 4;
+constexpr int GRAD_THREADS = 256, GRAD_UNROLL = 2;
 
 // N gradients to where they lie side by side, N * sizeof(D) bytes aligned alike
 template <class D, int N>
@@ -543,11 +593,18 @@ __device__ __forceinline__ int2 map_span(const T* z, D* d, int V, int part, int 
     }
     return make_int2(lo, hi);
   }
+  uint4 next[GRAD_UNROLL];
+  auto load = [&](int b) {
+#pragma unroll
+    for (int k = 0; k < GRAD_UNROLL; ++k)
+      if (b + k * GRAD_THREADS < v1) next[k] = r.load(b + k * GRAD_THREADS);
+  };
+  load(v0 + threadIdx.x);
   for (int b = v0 + threadIdx.x; b < v1; b += GRAD_THREADS * GRAD_UNROLL) {
     uint4 v[GRAD_UNROLL];
 #pragma unroll
-    for (int k = 0; k < GRAD_UNROLL; ++k)
-      if (b + k * GRAD_THREADS < v1) v[k] = r.load(b + k * GRAD_THREADS);
+    for (int k = 0; k < GRAD_UNROLL; ++k) v[k] = next[k];
+    load(b + GRAD_THREADS * GRAD_UNROLL);
 #pragma unroll
     for (int k = 0; k < GRAD_UNROLL; ++k) {
       const int i = b + k * GRAD_THREADS;
@@ -579,7 +636,7 @@ struct ScoreGradArgs {
 
 // dz = dy/dz (g_lp (onehot - p) - g_H p (log p + H)) = dy/dz (g_lp onehot - p (k0 + k1 t)) with t = log2 p.
 template <class T, class D, bool CAP>
-__global__ void __launch_bounds__(GRAD_THREADS)
+__global__ void __launch_bounds__(GRAD_THREADS, 6)
     token_log_probs_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts,
                                int per_block, ScoreGradArgs p) {
   const long long row = blockIdx.x / (unsigned)parts;
@@ -770,11 +827,7 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
   for (int b = v0; b < v1; b += TP_THREADS * U) {
     uint4 v[U];
     unsigned out[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int i = b + k * TP_THREADS + threadIdx.x;
-      v[k] = i < v1 ? r.load(i) : no_vector<T>();
-    }
+    load_batch<T, U>(r, b + threadIdx.x, b + TP_THREADS * U <= v1, v1, v);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int i = b + k * TP_THREADS + threadIdx.x, bit = (i - v0 + 1) * N;
@@ -794,7 +847,14 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
           if ((out[k] >> j) & 1) f[k * N + j] = CAP ? INFINITY : -INFINITY;
       }
     }
-    add_classes<CAP, false, E>(a, f, p.sc);
+    if (CAP) {
+      float least = f[0];
+#pragma unroll
+      for (int j = 1; j < E; ++j) least = fminf(least, f[j]);
+      add_classes<true, false, E>(a, f, p.sc.of_r(least), p.sc);
+    } else {
+      add_classes<false, false, E>(a, f, largest(f), p.sc);
+    }
   }
   a = block_combine(a, red, p.sc.c);
   if (C > 1) {
@@ -826,7 +886,7 @@ struct DistillGradArgs {
 };
 
 template <class T, class D, bool CAP>
-__global__ void __launch_bounds__(GRAD_THREADS)
+__global__ void __launch_bounds__(GRAD_THREADS, 6)
     distill_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts, int per_block,
                        DistillGradArgs p) {
   const long long row = blockIdx.x / (unsigned)parts;
@@ -970,11 +1030,8 @@ template <class T, int U, bool CAP, bool TOP>
 static int launch_scores(const T* logits, long long ld, long long rows, const ScoreArgs& args, cudaStream_t stream) {
   constexpr int per_batch = TP_THREADS * U * Row<T>::N;
   auto kernel = token_log_probs_fwd_kernel<T, U, CAP, TOP>;
-  const int shared = TOP ? (int)sizeof(Candidates<per_batch + 2 * Row<T>::N>) : 0;
-  if (TOP) {
-    static bool done[64] = {};
-    if (int rc = allow_shared(kernel, shared, done)) return rc;
-  }
+  const int shared = TOP ? (int)sizeof(TopWork) : 0;   // (with the static part below the 48 KB that need no attribute)
+  static_assert(sizeof(TopWork) + sizeof(Slices) + 1024 <= 48 * 1024, "shared memory of the top classes");
   const int C = ctas_per_row(rows, args.V, per_batch);
   return launch_clusters(kernel, rows * C, C, shared, stream, logits, ld, C, args);
 }
@@ -997,8 +1054,8 @@ template <class F>
 static int launch_gradient(const char* what, const void* z, int dtype, long long ld, void* d, int dtype_d, long long ld_d,
                            long long rows, int V, cudaStream_t stream, F launch) {
   const int N = dtype == OB_F32 ? 4 : 8;
-  // two batches of every thread to a block, more where the grid would not hold the blocks
-  long long per_block = 2ll * GRAD_THREADS * GRAD_UNROLL, parts = 0;
+  // four batches of every thread to a block, more where the grid would not hold the blocks
+  long long per_block = 4ll * GRAD_THREADS * GRAD_UNROLL, parts = 0;
   for (;; per_block *= 2) {
     parts = (V / N + per_block - 1) / per_block;
     if (parts < 1) parts = 1;

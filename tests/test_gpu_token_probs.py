@@ -463,3 +463,24 @@ def test_infinite_logits():
         best[0, 5] = -math.inf
         assert out.top_ids[0].tolist() == [5, *best[0].topk(2).indices.tolist()]
         assert out.top_ids[1].tolist() == [20, 7, V - 1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_classes_of_long_rows_in_bad_orders(dtype):
+    """Rows that keep giving new largest logits, that keep repeating them, or whose largest ones all fall to the same few threads."""
+    V = 260011
+    i = torch.arange(V, device=DEV)
+    z = _logits(7, V)
+    z[0] = i                                                        # ascending (in steps of a rounding for bf16)
+    z[1] = 7.0
+    z[2] = (i // 50000).float()                                     # long runs, ascending
+    z[3] = torch.where(i % 2048 < 200, 50.0 + i / V, z[3])          # the largest in the same places of every stretch
+    z[4] = (i % 3).float()
+    z[5] = torch.where(i > V - 300, 1.0, -1.0)
+    z[6] = torch.where(i % 8192 < 8, (i // 8192).float(), -3.0)     # few threads, ascending
+    z = z.to(dtype)
+    for part in (z, z[:, 1:], z[:1]):                               # (one row: shared by a cluster)
+        for k in (1, 64, 128):
+            out = F.token_log_probs(part, top_k=k)
+            want = part.sort(dim=-1, descending=True, stable=True).indices[:, :k]
+            assert torch.equal(out.top_ids, want)
