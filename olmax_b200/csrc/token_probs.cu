@@ -15,7 +15,7 @@
 
 namespace ob {
 
-constexpr int TP_THREADS = 512;
+constexpr int TP_THREADS = 256;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 template <class T>
@@ -148,9 +148,8 @@ __device__ __forceinline__ Stats block_combine(Stats a, Stats* red, float c) {
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
   __syncthreads();
-  return shuffle_combine(red[threadIdx.x & 15], 8, c);
+  return shuffle_combine(red[threadIdx.x % (TP_THREADS / 32)], TP_THREADS / 64, c);
 }
-static_assert(TP_THREADS == 512, "block_combine joins 16 warps");
 
 // A row as 16-byte vectors between a head and a tail of single classes: rows start at any multiple of the element size.
 template <class T>
@@ -225,17 +224,23 @@ __device__ __forceinline__ float key_logit(unsigned key) {
 // What a row's (or slice's) top classes are found from, in shared memory.  The row is read in batches; what a thread reads of a batch is a group,
 // known by its largest logit.  Group g is the batch g / TP_THREADS of thread g % TP_THREADS.
 struct TopWork {
-  static constexpr int LIMIT = TP_THREADS + 2 * OB_TOP_K_MAX;   // groups kept from one batch to the next
-  static constexpr int GROUPS = LIMIT + TP_THREADS;             // ... and those of one batch
+  static constexpr int EVERY = 4;                          // batches between two looks at the number of groups, but for the first ones
+  static constexpr int LIMIT = 1536;                       // groups kept from one look to the next
+  static constexpr int GROUPS = LIMIT + EVERY * TP_THREADS;   // ... and those that come until then
   static constexpr int STEP = 192;
-  static constexpr int CLASSES = 1024;
+  static constexpr int CLASSES = 512;
   unsigned group_key[GROUPS];
   int group[GROUPS];
-  unsigned key[CLASSES];
-  int cls[CLASSES];
+  unsigned long long code[CLASSES];   // in order of the classes: order_code
   int groups, classes, kept;
   int red[2][TP_THREADS / 32];
 };
+static_assert(TopWork::LIMIT >= TP_THREADS + OB_TOP_K_MAX && TopWork::CLASSES > OB_TOP_K_MAX, "what drop_groups and collect_classes leave");
+
+// Larger codes come first.
+__device__ __forceinline__ unsigned long long order_code(unsigned key, int cls) {
+  return (unsigned long long)key << 32 | (unsigned)~cls;
+}
 
 __device__ __forceinline__ int block_sum(int c, int* red) {
   c = __reduce_add_sync(0xffffffffu, c);
@@ -310,7 +315,7 @@ __device__ __forceinline__ unsigned kth_of_threads(unsigned key, int k) {
 }
 
 // The classes of the groups at or above `cut` that reach it themselves, and those of the row's head and tail (`single` of this thread, or -1), as
-// w.key / w.cls: at most CLASSES, and the first k among them.  Returns how many.
+// w.code: at most CLASSES, and the first k among them.  Returns how many.
 template <class T, int U>
 __device__ int collect_classes(TopWork& w, const Row<T>& r, int v0, int v1, int single, int k, unsigned cut) {
   constexpr int N = Row<T>::N;
@@ -333,10 +338,7 @@ __device__ int collect_classes(TopWork& w, const Row<T>& r, int v0, int v1, int 
   each([&](unsigned key, int i) {
     if (key < cut) return;
     const int at = atomicAdd(&w.classes, 1);
-    if (at < TopWork::CLASSES) {
-      w.key[at] = key;
-      w.cls[at] = i;
-    }
+    if (at < TopWork::CLASSES) w.code[at] = order_code(key, i);
   });
   __syncthreads();
   int found = w.classes;
@@ -356,9 +358,7 @@ __device__ int collect_classes(TopWork& w, const Row<T>& r, int v0, int v1, int 
   __syncthreads();
   each([&](unsigned q, int i) {
     if (q < key || (q == key && i > cls)) return;
-    const int at = atomicAdd(&w.classes, 1);
-    w.key[at] = q;
-    w.cls[at] = i;
+    w.code[atomicAdd(&w.classes, 1)] = order_code(q, i);
   });
   __syncthreads();
   return w.classes;
@@ -374,11 +374,9 @@ struct ScoreArgs {
   Scaling sc;
 };
 
-// What the CTAs of a row's cluster leave with the first one.
-struct Slices {
-  Stats stats[8];
-  unsigned key[8][OB_TOP_K_MAX];
-  int cls[8][OB_TOP_K_MAX];
+// What a CTA of a row's cluster leaves with the first one.
+struct Slice {
+  unsigned long long code[OB_TOP_K_MAX];   // 0: no class
 };
 
 // (forms that do not ask for a converged warp)
@@ -387,8 +385,8 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ void store_cluster(uint32_t addr, float x) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(x) : "memory");
 }
-__device__ __forceinline__ void store_cluster(uint32_t addr, unsigned x) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
+__device__ __forceinline__ void store_cluster(uint32_t addr, unsigned long long x) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(x) : "memory");
 }
 
 // Log probabilities, entropy and top classes.  A row belongs to a cluster of C CTAs (C = 1 but for few rows), a slice of its vectors to
@@ -397,17 +395,17 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, unsigned x) {
 // Top classes in the same pass, at one comparison per thread and batch: a group (TopWork) is kept if its largest logit is above `cut`, a
 // lower bound of the row's k-th largest logit that k classes of earlier batches reach, so that no class of a later one at the bound is among the
 // first k.  The bound is the k-th largest of the threads' maxima so far, which no more than 1.2 k classes reach if they are spread over the
-// threads by chance; it is looked for at the first batch, whenever STEP more groups have come together, and at the end, when the
+// threads by chance; it is looked for at the first batch, whenever STEP more groups have come together, and at the end if there are many.  Then the
 // classes of the groups above it are read again and put in order.
 template <class T, int U, bool CAP, bool TOP>
-__global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
+__global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 4 : 6)
     token_log_probs_fwd_kernel(const T* __restrict__ logits, long long ld, int C, ScoreArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
-  constexpr bool AHEAD = CAP;
+  constexpr bool AHEAD = TOP || CAP;
   extern __shared__ __align__(16) char shared_bytes[];
-  TopWork& work = *reinterpret_cast<TopWork*>(shared_bytes);   // TOP
-  __shared__ Stats red[TP_THREADS / 32];
-  __shared__ Slices slices;
+  TopWork& work = *reinterpret_cast<TopWork*>(shared_bytes);                     // TOP
+  Slice* slices = reinterpret_cast<Slice*>(shared_bytes + sizeof(TopWork));      // TOP, one per CTA of the cluster
+  __shared__ Stats red[TP_THREADS / 32], parts[8];
   if (C > 1) cluster_arrive();
   const long long row = blockIdx.x / (unsigned)C;
   const int part = (int)(blockIdx.x - row * C);
@@ -425,7 +423,7 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
   }
   Stats a = empty_stats();
   unsigned cut = 0, best = 0;
-  int limit = TopWork::STEP;
+  int limit = TopWork::STEP, end = 0;
   if (TOP && threadIdx.x == 0) work.groups = 0;
   if (TOP) __syncthreads();
   const int single = r.single(threadIdx.x, part == 0, part == C - 1);
@@ -464,7 +462,6 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
       }
       best = max(best, key);
       if (b == v0) cut = kth_of_threads(best, p.top_k);
-      int end = 0;
       if (b == v0 ? key != 0u && key >= cut : key > cut) {
         const int at = atomicAdd(&work.groups, 1);
         work.group_key[at] = key;
@@ -472,40 +469,38 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
         end = at + 1;
       }
       // (every thread's last group, not the counter: a faster thread may already be adding to that)
-      if (__syncthreads_or(end > limit)) {
+      if ((batch < TopWork::EVERY || batch % TopWork::EVERY == TopWork::EVERY - 1) && __syncthreads_or(end > limit)) {
         int n = work.groups;
-        if (n > TopWork::LIMIT) n = drop_groups(work, p.top_k, cut);
-        else cut = max(cut, kth_of_threads(best, p.top_k));
+        if (n > TopWork::LIMIT) {
+          n = drop_groups(work, p.top_k, cut);
+          end = 0;
+        } else {
+          cut = max(cut, kth_of_threads(best, p.top_k));
+        }
         limit = min(n + TopWork::STEP, TopWork::LIMIT);
       }
     }
   }
-  if (TOP) cut = max(cut, kth_of_threads(best, p.top_k));
   a = block_combine(a, red, p.sc.c);
   if (C > 1) cluster_wait();   // the first CTA runs
   if (TOP) {
-    // the slice's first k classes in order
+    // the slice's first k classes in order; few groups are not worth a better bound
+    if (work.groups > TopWork::STEP) cut = max(cut, kth_of_threads(best, p.top_k));
     const int n = collect_classes<T, U>(work, r, v0, v1, single, p.top_k, cut);
-    uint32_t keys = smem_u32(slices.key[part]), classes = smem_u32(slices.cls[part]);
-    if (C > 1) {
-      keys = mapa_shared(keys, 0);
-      classes = mapa_shared(classes, 0);
-    }
+    uint32_t codes = smem_u32(slices[part].code);
+    if (C > 1) codes = mapa_shared(codes, 0);
     for (int t = threadIdx.x; t < n; t += TP_THREADS) {
-      const unsigned key = work.key[t];
-      const int i = work.cls[t];
+      const unsigned long long code = work.code[t];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += work.key[j] > key || (work.key[j] == key && work.cls[j] < i);
-      if (rank < p.top_k) {
-        store_cluster(keys + rank * 4, key);
-        store_cluster(classes + rank * 4, (unsigned)i);
-      }
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += work.code[j] > code;
+      if (rank < p.top_k) store_cluster(codes + rank * 8, code);
     }
-    for (int t = n + threadIdx.x; t < p.top_k; t += TP_THREADS) store_cluster(keys + t * 4, 0u);
+    for (int t = n + threadIdx.x; t < p.top_k; t += TP_THREADS) store_cluster(codes + t * 8, 0ull);
   }
   if (C > 1) {
     if (threadIdx.x == 0) {
-      const uint32_t at = mapa_shared(smem_u32(&slices.stats[part]), 0);
+      const uint32_t at = mapa_shared(smem_u32(&parts[part]), 0);
       store_cluster(at, a.m);
       store_cluster(at + 4, a.s);
       store_cluster(at + 8, a.w);
@@ -513,8 +508,8 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
     cluster_arrive();
     cluster_wait();
     if (part != 0) return;
-    a = slices.stats[0];
-    for (int i = 1; i < C; ++i) a = combine(a, slices.stats[i], p.sc.c);
+    a = parts[0];
+    for (int i = 1; i < C; ++i) a = combine(a, parts[i], p.sc.c);
   } else if (TOP) {
     __syncthreads();
   }
@@ -533,23 +528,21 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
     for (int t = threadIdx.x; t < C * p.top_k; t += TP_THREADS) {
       const int own = t / p.top_k;
       int rank = t - own * p.top_k;
-      const unsigned key = slices.key[own][rank];
-      if (key == 0) continue;
-      const int i = slices.cls[own][rank];
+      const unsigned long long code = slices[own].code[rank];
+      if (code == 0) continue;
       for (int s = 0; s < C; ++s) {
         if (s == own) continue;
         int lo = 0, hi = p.top_k;   // classes [0, lo) of the list come before, [hi, k) after
         while (lo < hi) {
           const int mid = (lo + hi) / 2;
-          const unsigned q = slices.key[s][mid];
-          if (q > key || (q == key && q != 0 && slices.cls[s][mid] < i)) lo = mid + 1;
+          if (slices[s].code[mid] > code) lo = mid + 1;
           else hi = mid;
         }
         rank += lo;
       }
       if (rank < p.top_k) {
-        p.top_log_probs[row * p.top_k + rank] = log_p(key_logit(key));
-        p.top_ids[row * p.top_k + rank] = i;
+        p.top_log_probs[row * p.top_k + rank] = log_p(key_logit((unsigned)(code >> 32)));
+        p.top_ids[row * p.top_k + rank] = ~(unsigned)code;
       }
     }
   }
@@ -772,7 +765,7 @@ __device__ __forceinline__ void distill_row(const Pairs& pairs, Stats others_sta
 // A row belongs to a cluster of C CTAs as in the log probabilities.  A bit of shared memory per class of the slice says which the teacher
 // names; four or eight of them, one vector's, cost one look per 16 bytes.
 template <class T, int U, bool CAP>
-__global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
+__global__ void __launch_bounds__(TP_THREADS, CAP ? 4 : 6)
     distill_fwd_kernel(const T* __restrict__ logits, long long ld, int C, DistillArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
   extern __shared__ __align__(16) char shared_bytes[];
@@ -803,13 +796,14 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 2 : 3)
   for (int i = threadIdx.x; i < (hi + shift + 31) / 32; i += TP_THREADS) named[i] = 0;
   __syncthreads();
   {
-    // four threads look for an earlier pair with the class of one
-    const int i = threadIdx.x % OB_TOP_K_MAX, j0 = threadIdx.x / OB_TOP_K_MAX * (OB_TOP_K_MAX / 4);
+    // some threads look for an earlier pair with the class of one, each among a share of them
+    constexpr int SHARE = OB_TOP_K_MAX * OB_TOP_K_MAX / TP_THREADS;
+    const int i = threadIdx.x % OB_TOP_K_MAX, j0 = threadIdx.x / OB_TOP_K_MAX * SHARE;
     const int mine = pairs.cls[i];
     bool before = false;
     if (mine >= 0 && j0 < i) {
 #pragma unroll
-      for (int j = 0; j < OB_TOP_K_MAX / 4; ++j) before |= pairs.cls[j0 + j] == mine && j0 + j < i;
+      for (int j = 0; j < SHARE; ++j) before |= pairs.cls[j0 + j] == mine && j0 + j < i;
     }
     if (before) pairs.repeated[i] = 1;
   }
@@ -1000,7 +994,7 @@ static inline int allow_shared(K kernel, int bytes, bool (&done)[64]) {
   return 0;
 }
 
-// CTAs per row: a power of two up to the portable cluster size, as long as all CTAs run at once (two per SM) and a slice keeps a batch
+// CTAs per row: a power of two up to the portable cluster size, as long as there are no more than two CTAs per SM and a slice keeps a batch
 // or more of every thread.
 static inline int ctas_per_row(long long rows, int V, int per_batch) {
   int C = 1;
@@ -1030,9 +1024,9 @@ template <class T, int U, bool CAP, bool TOP>
 static int launch_scores(const T* logits, long long ld, long long rows, const ScoreArgs& args, cudaStream_t stream) {
   constexpr int per_batch = TP_THREADS * U * Row<T>::N;
   auto kernel = token_log_probs_fwd_kernel<T, U, CAP, TOP>;
-  const int shared = TOP ? (int)sizeof(TopWork) : 0;   // (with the static part below the 48 KB that need no attribute)
-  static_assert(sizeof(TopWork) + sizeof(Slices) + 1024 <= 48 * 1024, "shared memory of the top classes");
   const int C = ctas_per_row(rows, args.V, per_batch);
+  static_assert(sizeof(TopWork) + 8 * sizeof(Slice) + 1024 <= 48 * 1024, "shared memory that needs no attribute, with the static part");
+  const int shared = TOP ? (int)(sizeof(TopWork) + C * sizeof(Slice)) : 0;
   return launch_clusters(kernel, rows * C, C, shared, stream, logits, ld, C, args);
 }
 

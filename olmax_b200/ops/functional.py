@@ -1165,7 +1165,7 @@ def _logit_rows(logits: torch.Tensor) -> torch.Tensor:
     allowed = (torch.float32, torch.bfloat16) if logits.is_cuda else (torch.float32, torch.bfloat16, torch.float64)
     if logits.dtype not in allowed:
         raise K.KernelError(f"logits must be fp32 or bf16, got {logits.dtype}")
-    z = logits.reshape(math.prod(logits.shape[:-1]), logits.shape[-1])
+    z = logits if logits.dim() == 2 else logits.reshape(math.prod(logits.shape[:-1]), logits.shape[-1])
     return z if z.stride(-1) == 1 else z.contiguous()
 
 
@@ -1174,17 +1174,43 @@ def _token_rows(ids: torch.Tensor, shape, device) -> torch.Tensor:
         raise ValueError(f"token ids must be int64 or int32, got {ids.dtype}")
     if tuple(ids.shape) != tuple(shape) or ids.device != device:
         raise ValueError(f"token ids of shape {tuple(ids.shape)} on {ids.device} do not fit rows of shape {tuple(shape)} on {device}")
+    if ids.dtype == torch.int64 and ids.dim() == 1 and ids.is_contiguous():
+        return ids
     return ids.reshape(-1).long().contiguous()
 
 
 def _upstream(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """An upstream gradient as fp32 [rows]; one that is a broadcast scalar (the gradient of a sum) stays one."""
+    """An upstream gradient as fp32 [rows], or one value for all rows (a scalar, or the gradient of a sum): stride 0."""
     if g is None:
         return None
     g = g.float()
     if g.dim() and not any(g.stride()):
         return g.as_strided((g.numel(),), (0,))
-    return g.reshape(-1)
+    return g.reshape(-1) if g.dim() > 1 else g
+
+
+def _refuse_double_backward() -> None:
+    """The gradients below are kernels' results, not functions of the upstream gradient that autograd could go through again (grad mode is
+    only on in a backward pass with ``create_graph``)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("log probabilities and distillation losses can be differentiated once: create_graph is not supported")
+
+
+def _scores(z: torch.Tensor, ids: Optional[torch.Tensor], top_k: int, ignore_index: int, cap: float, temperature: float, keep: bool):
+    """(log probabilities, entropy, top log probabilities, top ids, what the backward pass reads if ``keep``) of logits [rows, V]."""
+    if not z.is_cuda:
+        log_probs, entropy, norm, top, top_ids = ref.token_log_probs(z, ids, top_k, ignore_index, cap, temperature)
+        return log_probs, entropy, top, top_ids, norm
+    rows, dev = z.shape[0], z.device
+    log_probs = torch.empty(rows, dtype=torch.float32, device=dev) if ids is not None else None
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    norm = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev) if top_k else None
+    top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev) if top_k else None
+    if rows:
+        K.token_log_probs_fwd(z, ids, log_probs, entropy, norm, top, top_ids, ignore_index=ignore_index, softcap=cap,
+                              temperature=temperature)
+    return log_probs, entropy, top, top_ids, norm
 
 
 class _TokenLogProbsFn(torch.autograd.Function):
@@ -1193,25 +1219,14 @@ class _TokenLogProbsFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.options = dict(ignore_index=ignore_index, temperature=temperature)
         ctx.cap = cap
-        rows = z.shape[0]
-        if z.is_cuda:
-            log_probs = torch.empty(rows, dtype=torch.float32, device=z.device) if ids is not None else None
-            entropy = torch.empty(rows, dtype=torch.float32, device=z.device)
-            norm = torch.empty((rows, 2), dtype=torch.float32, device=z.device) if ctx.needs_input_grad[0] else None
-            top = torch.empty((rows, top_k), dtype=torch.float32, device=z.device) if top_k else None
-            top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=z.device) if top_k else None
-            if rows:
-                K.token_log_probs_fwd(z, ids, log_probs, entropy, norm, top, top_ids, softcap=cap, **ctx.options)
-        else:
-            log_probs, entropy, norm, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(z, ids, norm, entropy)
+        log_probs, entropy, top, top_ids, norm = _scores(z, ids, top_k, ignore_index, cap, temperature, True)
+        ctx.save_for_backward(z, ids, norm, entropy)
         ctx.mark_non_differentiable(*(t for t in (top, top_ids) if t is not None))
         return log_probs, entropy, top, top_ids
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_log_probs, g_entropy, _top, _ids):
+        _refuse_double_backward()
         if g_log_probs is None and g_entropy is None:
             return None, None, None, None, None, None
         z, ids, norm, entropy = ctx.saved_tensors
@@ -1244,7 +1259,18 @@ def token_log_probs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, *,
     z = _logit_rows(logits)
     shape = logits.shape[:-1]
     lab = _token_rows(ids, shape, logits.device) if ids is not None else None
-    log_probs, entropy, top, top_ids = _TokenLogProbsFn.apply(z, lab, int(top_k), int(ignore_index), cap, float(temperature))
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = _TokenLogProbsFn.apply(z, lab, int(top_k), int(ignore_index), cap, float(temperature))
+    else:
+        out = _scores(z, lab, int(top_k), int(ignore_index), cap, float(temperature), False)[:4]
+    return _shaped(out, shape, top_k)
+
+
+def _shaped(out, shape, top_k: int) -> TokenLogProbs:
+    """Results of rows as those of tokens of any shape."""
+    if len(shape) == 1:
+        return TokenLogProbs(*out)
+    log_probs, entropy, top, top_ids = out
     return TokenLogProbs(log_probs.view(shape) if log_probs is not None else None, entropy.view(shape),
                          top.view(*shape, top_k) if top_k else None, top_ids.view(*shape, top_k) if top_k else None)
 
@@ -1283,19 +1309,16 @@ class _DistillationFn(torch.autograd.Function):
         rows, k = ids.shape
         keep = ctx.needs_input_grad[0]
         if z.is_cuda:
-            dev = z.device
-            loss = torch.empty(rows, dtype=torch.float32, device=dev)
-            stats = torch.empty((rows, 8), dtype=torch.float32, device=dev)
-            q = torch.empty((rows, k), dtype=torch.float32, device=dev)
-            total = torch.empty((), dtype=torch.float32, device=dev)
-            inv = torch.empty((), dtype=torch.float32, device=dev)
+            work = K.distill_work(rows, k, z.device)
+            loss = torch.empty(rows if reduction == "none" else (), dtype=torch.float32, device=z.device)
             if rows:
-                K.distill_fwd(z, ids, values, loss, stats, q, renormalize=renormalize, softcap=cap, temperature=temperature)
+                K.distill_fwd(z, ids, values, work, renormalize=renormalize, softcap=cap, temperature=temperature,
+                              row_loss=loss if reduction == "none" else None)
             if reduction != "none":
-                K.distill_reduce(loss, stats, total, inv, mean=reduction == "mean")
+                K.distill_reduce(work, rows, k, loss, mean=reduction == "mean")
             if keep:
-                ctx.save_for_backward(z, ids, stats, q, inv)
-            return loss if reduction == "none" else total
+                ctx.save_for_backward(z, ids, work)
+            return loss
         loss, some = ref.distillation(z, ids, values, renormalize, cap, temperature)
         inv = 1.0 / some.sum().clamp(min=1).to(loss.dtype) if reduction == "mean" else torch.ones((), dtype=loss.dtype)
         if keep:
@@ -1303,19 +1326,17 @@ class _DistillationFn(torch.autograd.Function):
         return loss if reduction == "none" else loss.sum() * inv
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _refuse_double_backward()
         renormalize, cap, temperature, reduction = ctx.options
         if not ctx.needs_input_grad[0]:
             return (None,) * 7
         z, ids = ctx.saved_tensors[:2]
         rows = z.shape[0]
         if z.is_cuda:
-            stats, q, inv = ctx.saved_tensors[2:]
             d = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-            g = g.expand(rows) if reduction != "none" else g
             if rows:
-                K.distill_bwd(z, ids, stats, q, _upstream(g), inv if reduction == "mean" else None, d, softcap=cap,
+                K.distill_bwd(z, ids, ctx.saved_tensors[2], _upstream(g), d, mean=reduction == "mean", softcap=cap,
                               temperature=temperature)
         else:
             values, inv = ctx.saved_tensors[2:]
@@ -1443,8 +1464,8 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
         return log_probs, entropy, top, top_ids
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_log_probs, g_entropy, _top, _ids):
+        _refuse_double_backward()
         if g_log_probs is None and g_entropy is None:
             return (None,) * 8
         x2, ids, norm, entropy = ctx.saved_tensors
@@ -1475,10 +1496,8 @@ def linear_token_log_probs(x: torch.Tensor, handle, ids: Optional[torch.Tensor] 
     shape = x.shape[:-1]
     lab = _token_rows(ids, shape, x.device) if ids is not None else None
     x2 = x.reshape(math.prod(shape), x.shape[-1]).contiguous()
-    log_probs, entropy, top, top_ids = _LinearTokenLogProbsFn.apply(x2, handle, lab, int(top_k), int(ignore_index), cap,
-                                                                    float(temperature), int(chunk_rows))
-    return TokenLogProbs(log_probs.view(shape) if log_probs is not None else None, entropy.view(shape),
-                         top.view(*shape, top_k) if top_k else None, top_ids.view(*shape, top_k) if top_k else None)
+    return _shaped(_LinearTokenLogProbsFn.apply(x2, handle, lab, int(top_k), int(ignore_index), cap, float(temperature),
+                                                int(chunk_rows)), shape, top_k)
 
 
 class _LinearDistillationFn(torch.autograd.Function):
@@ -1492,25 +1511,23 @@ class _LinearDistillationFn(torch.autograd.Function):
         M, V = x2.shape[0], handle.tp_shape[0]
         if _on_gpu(x2):
             dev = x2.device
+            k = ids.shape[1]
             total = torch.empty((), dtype=torch.float32, device=dev)
-            inv = torch.empty((), dtype=torch.float32, device=dev)
-            K.distill_count(ids, values, inv, renormalize=renormalize, V=V)
-            loss = torch.empty(M, dtype=torch.float32, device=dev)
-            stats = torch.empty((M, 8), dtype=torch.float32, device=dev)
+            work = K.distill_work(M, k, dev)
+            K.distill_count(ids, values, work, renormalize=renormalize, V=V)
             chunks = _HeadChunks(x2, handle, chunk_rows)
-            q = torch.empty((chunks.step, ids.shape[1]), dtype=torch.float32, device=dev)
             dx = torch.empty_like(x2) if need_grad else None
             dlogits, single = chunks.gradients() if need_grad else (None, False)
             for r0, r1, xc, z in chunks:
-                K.distill_fwd(z, ids[r0:r1], values[r0:r1], loss[r0:r1], stats[r0:r1], q[: r1 - r0], renormalize=renormalize,
-                              softcap=cap, temperature=temperature)
+                K.distill_fwd(z, ids[r0:r1], values[r0:r1], work, row0=r0, total_rows=M, renormalize=renormalize, softcap=cap,
+                              temperature=temperature)
                 if need_grad:
-                    K.distill_bwd(z, ids[r0:r1], stats[r0:r1], q[: r1 - r0], None, inv,
-                                  chunks.rows_of(dlogits, single, r0, r1), scale=weight, softcap=cap, temperature=temperature)
+                    K.distill_bwd(z, ids[r0:r1], work, None, chunks.rows_of(dlogits, single, r0, r1), row0=r0, total_rows=M, mean=True,
+                                  scale=weight, softcap=cap, temperature=temperature)
                     chunks.chunk_gradient(dlogits, single, r0, r1, xc, dx)
             if need_grad:
                 chunks.finish(dlogits, single)
-            K.distill_reduce(loss, stats, total, None, mean=True)
+            K.distill_reduce(work, M, k, total, mean=True)
             total = total * weight if weight != 1.0 else total
         else:
             w = handle.full()
@@ -1528,8 +1545,8 @@ class _LinearDistillationFn(torch.autograd.Function):
         return total
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _refuse_double_backward()
         (dx,) = ctx.saved_tensors
         # g is 1 for loss.backward(); the weight gradient was already accumulated under that assumption
         return (dx * g.to(dx.dtype),) + (None,) * 8

@@ -28,7 +28,7 @@ __all__ = [
     "embed_gather", "embed_scatter", "ce_fwd_bwd", "ce_vp_stats", "ce_vp_grad", "count_valid", "adamw", "sumsq", "clip_coef", "cast_f32_bf16",
     "layernorm_fwd", "layernorm_bwd", "gather_shards", "scatter_add_shards", "allreduce_p2p", "allreduce_multimem",
     "peer_barrier", "peer_signal", "peer_wait", "copy_bytes", "push_copy", "fold_slots_bf16", "reduce_slots",
-    "token_log_probs_fwd", "token_log_probs_bwd", "distill_fwd", "distill_bwd", "distill_reduce", "distill_count", "TOP_K_MAX",
+    "token_log_probs_fwd", "token_log_probs_bwd", "distill_work", "distill_fwd", "distill_bwd", "distill_reduce", "distill_count", "TOP_K_MAX",
     "launch_count", "reset_launch_count", "pointer_table",
     "timing_enabled", "set_timing", "timed_region", "timing_report", "format_timing",
 ]
@@ -420,11 +420,12 @@ def _logits_dtype(t: torch.Tensor) -> int:
     return _LOGITS_DTYPE[t.dtype]
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """Make ``device`` current for a launch (nothing to do where it is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def token_log_probs_fwd(logits, ids, log_probs, entropy, norm, top_log_probs, top_ids, *, ignore_index=-100, softcap=0.0,
@@ -458,47 +459,67 @@ def _teacher_ids(t: torch.Tensor) -> int:
     return int(t.dtype == torch.int64)
 
 
-def distill_fwd(logits, teacher_ids, teacher_log_probs, row_loss, row_stats, q, *, renormalize, softcap=0.0,
+def distill_work(rows: int, k: int, device: torch.device) -> torch.Tensor:
+    """What the distillation kernels leave for one another of ``rows`` rows and ``k`` teacher classes, fp32: 1 / counted rows (16 bytes),
+    row statistics [rows, 8], teacher masses [rows, k], row losses [rows]."""
+    return torch.empty(4 + rows * (9 + k), dtype=torch.float32, device=device)
+
+
+def _work_ptrs(work: torch.Tensor, rows: int, k: int, row0: int = 0):
+    """(1 / counted rows, statistics, masses, losses) of the rows from ``row0`` on."""
+    base = work.data_ptr()
+    stats = base + 16
+    q = stats + 32 * rows
+    loss = q + 4 * k * rows
+    return base, stats + 32 * row0, q + 4 * k * row0, loss + 4 * row0
+
+
+def distill_fwd(logits, teacher_ids, teacher_log_probs, work, *, renormalize, row0=0, total_rows=None, row_loss=None, softcap=0.0,
                 temperature=1.0) -> None:
-    """``teacher_ids`` (int32 / int64) and ``teacher_log_probs`` (fp32) [rows, k] with one row stride; row_loss [rows], row_stats
-    [rows, 8] and q [rows, k] are fp32 outputs that :func:`distill_bwd` reads."""
+    """``teacher_ids`` (int32 / int64) and ``teacher_log_probs`` (fp32) [rows, k] with one row stride, for rows ``row0``, ... of the ``total_rows`` that
+    ``work`` (:func:`distill_work`) is for; ``row_loss``: where the losses go instead of into ``work``."""
     rows, V = logits.shape
+    k = teacher_ids.shape[1]
     if teacher_log_probs.stride() != teacher_ids.stride() or teacher_log_probs.dtype != torch.float32:
         raise KernelError("distillation: fp32 teacher values laid out like the teacher's ids are needed")
+    _, stats, q, loss = _work_ptrs(work, rows if total_rows is None else total_rows, k, row0)
     with _on(logits.device):
         check(lib().ob_distill_fwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), teacher_ids.data_ptr(),
-                                   _teacher_ids(teacher_ids), teacher_log_probs.data_ptr(), teacher_ids.stride(0),
-                                   teacher_ids.shape[1], int(renormalize), row_loss.data_ptr(), row_stats.data_ptr(), q.data_ptr(),
-                                   rows, V, softcap, 1.0 / temperature, stream_ptr(logits.device)), "distill_fwd")
+                                   _teacher_ids(teacher_ids), teacher_log_probs.data_ptr(), teacher_ids.stride(0), k, int(renormalize),
+                                   loss if row_loss is None else row_loss.data_ptr(), stats, q, rows, V, softcap, 1.0 / temperature,
+                                   stream_ptr(logits.device)), "distill_fwd")
     _count()
 
 
-def distill_bwd(logits, teacher_ids, row_stats, q, g, inv_count, dlogits, *, scale=1.0, softcap=0.0, temperature=1.0) -> None:
-    """``g``: fp32 [rows] of any stride (0: one value for all rows) or None; ``inv_count``: device scalar or None."""
+def distill_bwd(logits, teacher_ids, work, g, dlogits, *, mean, row0=0, total_rows=None, scale=1.0, softcap=0.0, temperature=1.0) -> None:
+    """``g``: fp32 [rows], or one value for all rows, or None; ``mean``: divide by the number of rows with a teacher."""
     rows, V = logits.shape
+    k = teacher_ids.shape[1]
+    inv_count, stats, q, _ = _work_ptrs(work, rows if total_rows is None else total_rows, k, row0)
     with _on(logits.device):
         check(lib().ob_distill_bwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), teacher_ids.data_ptr(),
-                                   _teacher_ids(teacher_ids), teacher_ids.stride(0), teacher_ids.shape[1], row_stats.data_ptr(),
-                                   q.data_ptr(), _ptr(g), 0 if g is None else g.stride(0), _ptr(inv_count), scale,
+                                   _teacher_ids(teacher_ids), teacher_ids.stride(0), k, stats, q, _ptr(g),
+                                   0 if g is None or g.dim() == 0 else g.stride(0), inv_count if mean else None, scale,
                                    dlogits.data_ptr(), _logits_dtype(dlogits), dlogits.stride(0), rows, V, softcap,
                                    1.0 / temperature, stream_ptr(logits.device)), "distill_bwd")
     _count()
 
 
-def distill_reduce(row_loss, row_stats, loss, inv_count, *, mean: bool) -> None:
-    """loss = sum (or mean over the rows with a teacher) of ``row_loss``; inv_count (or None) = 1 / max(1, these rows)."""
-    with _on(row_loss.device):
-        check(lib().ob_distill_reduce(row_loss.data_ptr(), row_stats.data_ptr(), row_loss.shape[0], int(mean), loss.data_ptr(),
-                                      _ptr(inv_count), stream_ptr(row_loss.device)), "distill_reduce")
+def distill_reduce(work, rows, k, loss, *, mean: bool) -> None:
+    """loss = sum (or mean over the rows with a teacher) of the row losses in ``work``, into which goes 1 / max(1, these rows)."""
+    inv_count, stats, _, row_loss = _work_ptrs(work, rows, k)
+    with _on(work.device):
+        check(lib().ob_distill_reduce(row_loss, stats, rows, int(mean), loss.data_ptr(), inv_count, stream_ptr(work.device)),
+              "distill_reduce")
     _count()
 
 
-def distill_count(teacher_ids, teacher_log_probs, inv_count, *, renormalize, V) -> None:
-    """inv_count = 1 / max(1, rows with a teacher), before the student's logits are there."""
+def distill_count(teacher_ids, teacher_log_probs, work, *, renormalize, V) -> None:
+    """1 / max(1, rows with a teacher) into ``work``, before the student's logits are there."""
     with _on(teacher_ids.device):
         check(lib().ob_distill_count(teacher_ids.data_ptr(), _teacher_ids(teacher_ids), teacher_log_probs.data_ptr(),
                                      teacher_ids.stride(0), teacher_ids.shape[1], int(renormalize), teacher_ids.shape[0], V,
-                                     inv_count.data_ptr(), stream_ptr(teacher_ids.device)), "distill_count")
+                                     work.data_ptr(), stream_ptr(teacher_ids.device)), "distill_count")
     _count()
 
 

@@ -313,3 +313,13 @@ def test_empty_batches():
     z = torch.zeros(0, 10, requires_grad=True)
     loss = F.distillation_loss(z, torch.zeros((0, 2), dtype=torch.int64), torch.zeros(0, 2))
     assert float(loss) == 0 and torch.autograd.grad(loss, z)[0].shape == (0, 10)
+
+
+def test_second_derivatives_are_refused():
+    z = _rows(3, 9).requires_grad_(True)
+    out = F.token_log_probs(z, torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out.log_probs.sum(), z, create_graph=True)
+    loss = F.distillation_loss(z, torch.zeros((3, 1), dtype=torch.int64), torch.zeros(3, 1))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, z, create_graph=True)
