@@ -51,27 +51,38 @@ __device__ __forceinline__ float min_nan(float x, float y) {
 }
 
 // The capped logit cap(z) = softcap * tanh(z / softcap).  tanh(u) = 1 - 2 r and 1 - tanh^2(u) = 4 r (1 - r) with r = 1 / a, a = 1 + e^2u: the
-// approximate tanh instruction's error of 5e-4 would show in every log probability, this form's is below 6e-7 (the roundings of r <= 1 and the
+// approximate tanh instruction's error of 5e-4 would show in every log probability, this form's is below 8e-7 (the roundings of r <= 1 and the
 // exponential's).  It takes two special-function operations beside the exponential of the softmax, of which an SM does sixteen a clock: they
-// bound the kernels.  So two classes share a reciprocal, 1 / (a b); a <= 2^30 changes no tanh and keeps the product finite.  What follows is
-// linear in r: t = (cap(z) - m) c is one multiply-add.
+// bound the kernels.  So four classes share a reciprocal, that of the product of their a; a <= 2^30 changes no tanh and keeps the product
+// finite.  What follows is linear in r: t = (cap(z) - m) c is one multiply-add.
 struct Scaling {
   float cap, k;     // k = 2 log2(e) / cap
   float c;          // log2(e) / T
   float inv_temp;
 
-  // f <- r of the logits f
+  __device__ __forceinline__ float2 denominators(float z0, float z1) const {
+    const float2 x = mul2(make_float2(z0, z1), make_float2(k, k));
+    return add2(make_float2(exp2_fast(min_nan(x.x, 30.f)), exp2_fast(min_nan(x.y, 30.f))), make_float2(1.f, 1.f));
+  }
+  // f <- r of the logits f (one, or a multiple of four)
   template <int E>
   __device__ __forceinline__ void reciprocals(float (&f)[E]) const {
-#pragma unroll
-    for (int j = 0; j < E; ++j) f[j] = 1.f + exp2_fast(min_nan(f[j] * k, 30.f));
-#pragma unroll
-    for (int j = 0; j + 1 < E; j += 2) {
-      const float both = rcp_fast(f[j] * f[j + 1]), r = both * f[j + 1];
-      f[j + 1] = both * f[j];
-      f[j] = r;
+    if (E == 1) {
+      f[0] = rcp_fast(1.f + exp2_fast(min_nan(f[0] * k, 30.f)));
+      return;
     }
-    if (E % 2) f[E - 1] = rcp_fast(f[E - 1]);
+#pragma unroll
+    for (int j = 0; j + 3 < E; j += 4) {
+      const float2 a = denominators(f[j], f[j + 1]), b = denominators(f[j + 2], f[j + 3]);
+      const float2 p = mul2(make_float2(a.x, b.x), make_float2(a.y, b.y));
+      const float all = rcp_fast(p.x * p.y);
+      const float2 q = mul2(make_float2(all, all), make_float2(p.y, p.x));   // 1 / (a.x a.y), 1 / (b.x b.y)
+      const float2 ra = mul2(make_float2(q.x, q.x), make_float2(a.y, a.x)), rb = mul2(make_float2(q.y, q.y), make_float2(b.y, b.x));
+      f[j] = ra.x;
+      f[j + 1] = ra.y;
+      f[j + 2] = rb.x;
+      f[j + 3] = rb.y;
+    }
   }
   __device__ __forceinline__ float of_r(float r) const { return fmaf(-2.f * cap, r, cap); }
   // one class, whether there is a cap or not: its capped logit, and dy / dz
@@ -109,27 +120,44 @@ __device__ __forceinline__ Stats combine(Stats a, Stats b, float c) {
 }
 __device__ __forceinline__ bool no_class(Stats a) { return a.m == -INFINITY && a.s == 0.f; }   // (a NaN makes the sum NaN)
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 template <int E>
 __device__ __forceinline__ float largest(const float (&f)[E]) {
   float mx = f[0];
 #pragma unroll
-  for (int j = 1; j < E; ++j) mx = fmaxf(mx, f[j]);
-  return mx;
+  for (int j = 1; j + 1 < E; j += 2) mx = max3(mx, f[j], f[j + 1]);
+  return E % 2 ? mx : fmaxf(mx, f[E - 1]);
 }
+constexpr float ABSENT = 1e30f;   // the r of a class that is not there: its exponent is far below any, and finite
 // Adds E classes of logits f with the largest (capped) logit mx, known first so that the exponentials do not wait for one another.  A masked class
-// (-inf) adds nothing: its exponent is kept finite where 0 * infinity would come up.  With CAP f are the classes' r (infinite for one that is
-// not there).
+// (-inf) adds nothing: its exponent is kept finite where 0 * infinity would come up.  With CAP f are the classes' r (ABSENT for one that is not there).  Two-wide arithmetic
+// halves the instructions beside the exponentials, which the issue slots are short of at two bytes a class.
 template <bool CAP, bool W, int E>
 __device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], float mx, const Scaling& sc) {
   if (mx > a.m) a = shifted(a, mx, sc.c);
   const float ref = a.m == -INFINITY ? 0.f : a.m;
   const float t0 = (sc.cap - ref) * sc.c, t1 = -2.f * sc.cap * sc.c;
+  float2 s = make_float2(0.f, 0.f), w = s;
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const float t = CAP ? fmaf(f[j], t1, t0) : (f[j] - ref) * sc.c, e = exp2_fast(t);
-    a.s += e;
-    if (W) a.w = fmaf(e, fmaxf(t, -FLT_MAX), a.w);
+  for (int j = 0; j + 1 < E; j += 2) {
+    const float2 x = make_float2(f[j], f[j + 1]);
+    const float2 t = CAP ? fma2(x, make_float2(t1, t1), make_float2(t0, t0))
+                         : mul2(add2(x, make_float2(-ref, -ref)), make_float2(sc.c, sc.c));
+    const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+    s = add2(s, e);
+    if (W) w = fma2(e, CAP ? t : make_float2(fmaxf(t.x, -FLT_MAX), fmaxf(t.y, -FLT_MAX)), w);
   }
+  if (E % 2) {
+    const float t = CAP ? fmaf(f[E - 1], t1, t0) : (f[E - 1] - ref) * sc.c, e = exp2_fast(t);
+    s.x += e;
+    if (W) w.x = fmaf(e, fmaxf(t, -FLT_MAX), w.x);
+  }
+  a.s += s.x + s.y;
+  if (W) a.w += w.x + w.y;
 }
 // one class of capped logit y
 __device__ __forceinline__ void add_class(Stats& a, float y, const Scaling& sc) {
@@ -443,7 +471,7 @@ __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 4 : 6)
       if (b + TP_THREADS * U > v1) {
 #pragma unroll
         for (int j = 0; j < E; ++j)
-          if (b + j / N * TP_THREADS + (int)threadIdx.x >= v1) y[j] = INFINITY;
+          if (b + j / N * TP_THREADS + (int)threadIdx.x >= v1) y[j] = ABSENT;
       }
       add_classes<true, true, E>(a, y, b + (int)threadIdx.x < v1 ? p.sc.capped(mx) : -INFINITY, p.sc);
     } else {
@@ -629,7 +657,7 @@ struct ScoreGradArgs {
 
 // dz = dy/dz (g_lp (onehot - p) - g_H p (log p + H)) = dy/dz (g_lp onehot - p (k0 + k1 t)) with t = log2 p.
 template <class T, class D, bool CAP>
-__global__ void __launch_bounds__(GRAD_THREADS, 6)
+__global__ void __launch_bounds__(GRAD_THREADS, CAP ? 4 : 6)
     token_log_probs_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts,
                                int per_block, ScoreGradArgs p) {
   const long long row = blockIdx.x / (unsigned)parts;
@@ -652,18 +680,32 @@ __global__ void __launch_bounds__(GRAD_THREADS, 6)
     k0 = k1 = gl = 0.f;
   }
   if (CAP) k0 *= 4.f, k1 *= 4.f, gl *= 4.f;   // of the slope 4 r (1 - r)
+  k0 = -k0, k1 = -k1;
   const float t0 = (p.sc.cap - norm.x) * p.sc.c - norm.y, t1 = -2.f * p.sc.cap * p.sc.c;
   map_span<T, D>(logits + row * ld, dlogits + row * ld_d, p.V, part, parts, per_block, [&](auto& f, int i) {
     constexpr int M = sizeof(f) / sizeof(float);
     if (CAP) p.sc.reciprocals(f);
-#pragma unroll
-    for (int j = 0; j < M; ++j) {
-      const float t = CAP ? fmaf(f[j], t1, t0) : fmaf(f[j] - norm.x, p.sc.c, -norm.y), e = exp2_fast(t);
+    auto pair = [&](float2 x) {
+      const float2 t = CAP ? fma2(x, make_float2(t1, t1), make_float2(t0, t0))
+                           : fma2(add2(x, make_float2(-norm.x, -norm.x)), make_float2(p.sc.c, p.sc.c), make_float2(-norm.y, -norm.y));
       // (2^t is 0 from -150 on; what it is multiplied by stays finite)
-      float g = -e * fmaf(k1, fmaxf(t, -1024.f), k0);
-      if (i + j == id) g += gl;
-      f[j] = CAP ? g * fmaf(-f[j], f[j], f[j]) : g;
+      const float2 u = CAP ? t : make_float2(fmaxf(t.x, -1024.f), fmaxf(t.y, -1024.f));
+      return mul2(make_float2(exp2_fast(t.x), exp2_fast(t.y)), fma2(u, make_float2(k1, k1), make_float2(k0, k0)));
+    };
+    float g[M + 1];
+#pragma unroll
+    for (int j = 0; j < M; j += 2) {
+      const float2 o = pair(make_float2(f[j], j + 1 < M ? f[j + 1] : f[j]));
+      g[j] = o.x;
+      g[j + 1] = o.y;
     }
+    if ((unsigned)(id - i) < (unsigned)M) {
+#pragma unroll
+      for (int j = 0; j < M; ++j)
+        if (i + j == id) g[j] += gl;
+    }
+#pragma unroll
+    for (int j = 0; j < M; ++j) f[j] = CAP ? g[j] * fmaf(-f[j], f[j], f[j]) : g[j];
   });
 }
 
@@ -838,14 +880,14 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 4 : 6)
       if (out[k]) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          if ((out[k] >> j) & 1) f[k * N + j] = CAP ? INFINITY : -INFINITY;
+          if ((out[k] >> j) & 1) f[k * N + j] = CAP ? ABSENT : -INFINITY;
       }
     }
     if (CAP) {
       float least = f[0];
 #pragma unroll
       for (int j = 1; j < E; ++j) least = fminf(least, f[j]);
-      add_classes<true, false, E>(a, f, p.sc.of_r(least), p.sc);
+      add_classes<true, false, E>(a, f, least == ABSENT ? -INFINITY : p.sc.of_r(least), p.sc);
     } else {
       add_classes<false, false, E>(a, f, largest(f), p.sc);
     }
@@ -880,7 +922,7 @@ struct DistillGradArgs {
 };
 
 template <class T, class D, bool CAP>
-__global__ void __launch_bounds__(GRAD_THREADS, 6)
+__global__ void __launch_bounds__(GRAD_THREADS, CAP ? 4 : 6)
     distill_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts, int per_block,
                        DistillGradArgs p) {
   const long long row = blockIdx.x / (unsigned)parts;
@@ -902,12 +944,24 @@ __global__ void __launch_bounds__(GRAD_THREADS, 6)
   const float t0 = (p.sc.cap - norm.z) * p.sc.c - norm.w, t1 = -2.f * p.sc.cap * p.sc.c;
   const int2 span = map_span<T, D>(z, d, p.V, part, parts, per_block, [&](auto& f, int) {
     constexpr int M = sizeof(f) / sizeof(float);
-    if (CAP) p.sc.reciprocals(f);
+    if (zero) {
 #pragma unroll
-    for (int j = 0; j < M; ++j) {
-      const float g = exp2_fast(CAP ? fmaf(f[j], t1, t0) : fmaf(f[j] - norm.z, p.sc.c, -norm.w)) * coef;
-      f[j] = zero ? 0.f : CAP ? g * fmaf(-f[j], f[j], f[j]) : g;
+      for (int j = 0; j < M; ++j) f[j] = 0.f;
+      return;
     }
+    if (CAP) p.sc.reciprocals(f);
+    float g[M + 1];
+#pragma unroll
+    for (int j = 0; j < M; j += 2) {
+      const float2 x = make_float2(f[j], j + 1 < M ? f[j + 1] : f[j]);
+      const float2 t = CAP ? fma2(x, make_float2(t1, t1), make_float2(t0, t0))
+                           : fma2(add2(x, make_float2(-norm.z, -norm.z)), make_float2(p.sc.c, p.sc.c), make_float2(-norm.w, -norm.w));
+      const float2 o = mul2(make_float2(exp2_fast(t.x), exp2_fast(t.y)), make_float2(coef, coef));
+      g[j] = o.x;
+      g[j + 1] = o.y;
+    }
+#pragma unroll
+    for (int j = 0; j < M; ++j) f[j] = CAP ? g[j] * fmaf(-f[j], f[j], f[j]) : g[j];
   });
   // the teacher's classes, over what has just been written for them
   __syncthreads();
