@@ -657,7 +657,7 @@ struct ScoreGradArgs {
 
 // dz = dy/dz (g_lp (onehot - p) - g_H p (log p + H)) = dy/dz (g_lp onehot - p (k0 + k1 t)) with t = log2 p.
 template <class T, class D, bool CAP>
-__global__ void __launch_bounds__(GRAD_THREADS, CAP ? 4 : 6)
+__global__ void __launch_bounds__(GRAD_THREADS, CAP && sizeof(T) == 2 ? 5 : 6)
     token_log_probs_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts,
                                int per_block, ScoreGradArgs p) {
   const long long row = blockIdx.x / (unsigned)parts;
@@ -736,152 +736,122 @@ struct DistillArgs {
   Scaling sc;
 };
 
-// The teacher's pairs of a row in shared memory: class (-1: does not count), value, student's capped logit.
-struct Pairs {
-  int cls[OB_TOP_K_MAX], repeated[OB_TOP_K_MAX];
-  float t[OB_TOP_K_MAX], y[OB_TOP_K_MAX];
-};
-
-// The row's loss and what its gradient needs, by one warp: `others` = statistics of the classes outside the teacher's.
-__device__ __forceinline__ void distill_row(const Pairs& pairs, Stats others_stats, long long row, const DistillArgs& p) {
-  const int lane = threadIdx.x & 31;
-  constexpr int N = OB_TOP_K_MAX / 32;
-  const double ln2 = 0.69314718055994530942;
-  float t[N], y[N];
-  bool in[N];
-  Stats st = empty_stats();
-  float t_max = -INFINITY;
-  bool any = false;
+// f <- gradients of classes outside the teacher's with logits f: coef * 2^((cap(f) - m) c - log_s) [* slope]; zeros whatever f is if `zero`.
+template <bool CAP, int M>
+__device__ __forceinline__ void rest_gradient(float (&f)[M], bool zero, float m, float log_s, float coef, const Scaling& sc) {
+  if (zero) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int i = n * 32 + lane;
-    in[n] = i < p.k && pairs.cls[i] >= 0;
-    t[n] = in[n] ? pairs.t[i] : -INFINITY;
-    y[n] = in[n] ? pairs.y[i] : -INFINITY;
-    if (in[n]) add_class(st, y[n], p.sc);
-    t_max = fmaxf(t_max, t[n]);
-    any |= in[n] && !(p.renormalize && t[n] == -INFINITY);
+    for (int j = 0; j < M; ++j) f[j] = 0.f;
+    return;
+  }
+  if (CAP) sc.reciprocals(f);
+  const float t0 = (sc.cap - m) * sc.c - log_s, t1 = -2.f * sc.cap * sc.c;
+  float g[M + 1];
+#pragma unroll
+  for (int j = 0; j < M; j += 2) {
+    const float2 x = make_float2(f[j], j + 1 < M ? f[j + 1] : f[j]);
+    const float2 t = CAP ? fma2(x, make_float2(t1, t1), make_float2(t0, t0))
+                         : fma2(add2(x, make_float2(-m, -m)), make_float2(sc.c, sc.c), make_float2(-log_s, -log_s));
+    const float2 o = mul2(make_float2(exp2_fast(t.x), exp2_fast(t.y)), make_float2(coef, coef));
+    g[j] = o.x;
+    g[j + 1] = o.y;
   }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) t_max = fmaxf(t_max, __shfl_xor_sync(0xffffffffu, t_max, off));
-  any = __any_sync(0xffffffffu, any);
-  const Stats a = others_stats, all = combine(shuffle_combine(st, 16, p.sc.c), a, p.sc.c);
-  const bool others = !no_class(a);
-  const float log_s = log2f(all.s), rest_log_s = log2f(a.s);
-  const double shift = p.renormalize && t_max > -INFINITY ? (double)t_max : 0.0;
-  double q[N], sum = 0.0;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    q[n] = in[n] ? exp((double)t[n] - shift) : 0.0;
-    sum += q[n];
-  }
-  sum = warp_sum(sum);
-  double log_norm = shift, mass = sum, rest = 0.0;
-  if (p.renormalize) {
-    log_norm += log(sum);
-    mass = 1.0;
-  } else if (others) {
-    rest = fmax(0.0, 1.0 - sum);
-  }
-  double loss = 0.0;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    if (p.renormalize) q[n] /= sum;
-    const double lp = y[n] == -INFINITY ? -INFINITY : (((double)y[n] - all.m) * p.sc.c - log_s) * ln2;
-    if (in[n] && q[n] != 0.0) loss += q[n] * ((double)t[n] - log_norm - lp);
-    const int i = n * 32 + lane;
-    if (i < p.k) p.q[row * p.k + i] = in[n] && any ? (float)q[n] : -1.f;
-  }
-  loss = warp_sum(loss);
-  if (lane == 0) {
-    const double rest_lp = (((double)a.m - all.m) * p.sc.c + rest_log_s - log_s) * ln2;
-    if (rest > 0.0) loss += rest * (log(rest) - rest_lp);
-    p.row_loss[row] = any ? (float)loss : 0.f;
-    const double total = mass + rest;
-    float4* o = reinterpret_cast<float4*>(p.row_stats + row * 8);
-    o[0] = make_float4(any ? (float)total : -1.f, others && any ? (float)(total * exp(rest_lp) - rest) : 0.f, 0.f, 0.f);
-    o[1] = make_float4(all.m, log_s, a.m, rest_log_s);
-  }
+  for (int j = 0; j < M; ++j) f[j] = CAP ? g[j] * fmaf(-f[j], f[j], f[j]) : g[j];
 }
 
-// A row belongs to a cluster of C CTAs as in the log probabilities.  A bit of shared memory per class of the slice says which the teacher
-// names; four or eight of them, one vector's, cost one look per 16 bytes.
+// Sums over the block, the same in every thread.
+__device__ __forceinline__ double block_sum(double x, double* red) {
+  x = warp_sum(x);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int i = 0; i < TP_THREADS / 32; ++i) t += red[i];
+  return t;
+}
+
+// A row belongs to a cluster of C CTAs as in the log probabilities.  Thread t holds the teacher's pair t.  One bit of shared memory per vector, the
+// bits of a thread's batch side by side, says whether the teacher names one of its classes, one bit per class which: a batch without one, and
+// that is most of them, costs one look.
 template <class T, int U, bool CAP>
-__global__ void __launch_bounds__(TP_THREADS, CAP ? 4 : 6)
-    distill_fwd_kernel(const T* __restrict__ logits, long long ld, int C, DistillArgs p) {
+__global__ void __launch_bounds__(TP_THREADS, 6)
+    distill_fwd_kernel(const T* __restrict__ logits, long long ld, int C, int slice_vectors, DistillArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
   extern __shared__ __align__(16) char shared_bytes[];
-  unsigned* named = reinterpret_cast<unsigned*>(shared_bytes);
-  __shared__ Stats red[TP_THREADS / 32], slices[8];
-  __shared__ Pairs pairs;
+  unsigned* flags = reinterpret_cast<unsigned*>(shared_bytes);   // a bit per vector, whole batches
+  const int flag_words = (slice_vectors + TP_THREADS * U - 1) / (TP_THREADS * U) * (TP_THREADS * U / 32);
+  unsigned* named = flags + flag_words;                          // a bit per class
+  __shared__ Stats red[TP_THREADS / 32], parts[8];
+  __shared__ double red_d[TP_THREADS / 32];
+  __shared__ int cls_s[OB_TOP_K_MAX];
   if (C > 1) cluster_arrive();
   const long long row = blockIdx.x / (unsigned)C;
   const int part = (int)(blockIdx.x - row * C);
   const Row<T> r(logits + row * ld, p.V);
   const int v0 = (int)((long long)r.nvec * part / C), v1 = (int)((long long)r.nvec * (part + 1) / C);
-  const int lo = part == 0 ? 0 : r.class_of(v0), hi = part == C - 1 ? p.V : r.class_of(v1);
-  // the bit of class i: vectors begin at multiples of N, the row's head lies in front of the first
-  const int shift = N - r.class_of(v0);
-  long long id = -1;
+  const int c0 = r.class_of(v0), c1 = r.class_of(v1);
+  const int lo = part == 0 ? 0 : c0, hi = part == C - 1 ? p.V : c1;
+  const int shift = N - c0;   // the bit of class i is i + shift: vectors begin at multiples of N, the row's head lies in front of the first
+
+  // ---- the classes that the teacher names
+  int id = -1;
+  float t = -INFINITY, y = -INFINITY;
   if ((int)threadIdx.x < p.k) {
-    id = teacher_id(p.teacher_ids, p.ids_64, row * p.ld_t + threadIdx.x);
-    if (id < 0 || id >= p.V) id = -1;
-    if (part == 0) {
-      pairs.t[threadIdx.x] = p.teacher_log_probs[row * p.ld_t + threadIdx.x];
-      if (id >= 0) pairs.y[threadIdx.x] = p.sc.capped(to_f(r.z[id]));
+    const long long i = teacher_id(p.teacher_ids, p.ids_64, row * p.ld_t + threadIdx.x);
+    if (i >= 0 && i < p.V) {
+      id = (int)i;
+      t = p.teacher_log_probs[row * p.ld_t + threadIdx.x];
+      y = to_f(r.z[i]);   // (waited for at the end)
     }
   }
-  if (threadIdx.x < OB_TOP_K_MAX) {
-    pairs.cls[threadIdx.x] = (int)id;
-    pairs.repeated[threadIdx.x] = 0;
-  }
+  if (threadIdx.x < OB_TOP_K_MAX) cls_s[threadIdx.x] = id;
+  for (int i = threadIdx.x; i < flag_words; i += TP_THREADS) flags[i] = 0;
   for (int i = threadIdx.x; i < (hi + shift + 31) / 32; i += TP_THREADS) named[i] = 0;
   __syncthreads();
-  {
-    // some threads look for an earlier pair with the class of one, each among a share of them
-    constexpr int SHARE = OB_TOP_K_MAX * OB_TOP_K_MAX / TP_THREADS;
-    const int i = threadIdx.x % OB_TOP_K_MAX, j0 = threadIdx.x / OB_TOP_K_MAX * SHARE;
-    const int mine = pairs.cls[i];
-    bool before = false;
-    if (mine >= 0 && j0 < i) {
-#pragma unroll
-      for (int j = 0; j < SHARE; ++j) before |= pairs.cls[j0 + j] == mine && j0 + j < i;
+  bool again = C > 1 && id >= 0;   // (another slice's bits are not here to tell)
+  if (id >= lo && id < hi) {
+    const unsigned bit = 1u << ((id + shift) & 31);
+    again |= (atomicOr(&named[(id + shift) >> 5], bit) & bit) != 0;
+    if (id >= c0 && id < c1) {
+      const int vec = (id - c0) / N, at = (vec / (TP_THREADS * U) * TP_THREADS + vec % TP_THREADS) * U + vec / TP_THREADS % U;
+      atomicOr(&flags[at >> 5], 1u << (at & 31));
     }
-    if (before) pairs.repeated[i] = 1;
   }
-  __syncthreads();
-  if (threadIdx.x < OB_TOP_K_MAX) {
-    if (pairs.repeated[threadIdx.x]) pairs.cls[threadIdx.x] = -1;
-    else if (id >= lo && id < hi) atomicOr(&named[((int)id + shift) >> 5], 1u << (((int)id + shift) & 31));
+  bool in = id >= 0;
+  if (__syncthreads_or(again) && in) {   // of several pairs with one class the first counts
+    for (int j = 0; j < (int)threadIdx.x; ++j) in &= cls_s[j] != id;
   }
-  __syncthreads();
+
+  // ---- the statistics of the others
   Stats a = empty_stats();
+  auto is_named = [&](int i) { return (named[(i + shift) >> 5] >> ((i + shift) & 31)) & 1; };
   const int single = r.single(threadIdx.x, part == 0, part == C - 1);
-  if (single >= 0 && !((named[(single + shift) >> 5] >> ((single + shift) & 31)) & 1)) {
-    add_class(a, p.sc.capped(to_f(r.z[single])), p.sc);
-  }
-  for (int b = v0; b < v1; b += TP_THREADS * U) {
+  if (single >= 0 && !is_named(single)) add_class(a, p.sc.capped(to_f(r.z[single])), p.sc);
+  for (int b = v0, batch = 0; b < v1; b += TP_THREADS * U, ++batch) {
     uint4 v[U];
-    unsigned out[U];
     load_batch<T, U>(r, b + threadIdx.x, b + TP_THREADS * U <= v1, v1, v);
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int i = b + k * TP_THREADS + threadIdx.x, bit = (i - v0 + 1) * N;
-      out[k] = i < v1 ? (named[bit >> 5] >> (bit & 31)) & ((1u << N) - 1) : (1u << N) - 1;
-    }
     float f[E];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      unpack<T>(v[k], f + k * N);
-    }
+    for (int k = 0; k < U; ++k) unpack<T>(v[k], f + k * N);
     if (CAP) p.sc.reciprocals(f);
+    const int bit = (batch * TP_THREADS + threadIdx.x) * U;
+    const unsigned some = (flags[bit >> 5] >> (bit & 31)) & ((1u << U) - 1);
+    if (some) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (out[k]) {
+      for (int k = 0; k < U; ++k) {
+        const int at = (b - v0 + k * TP_THREADS + threadIdx.x + 1) * N;
+        const unsigned out = (some >> k) & 1 ? named[at >> 5] >> (at & 31) : 0u;
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          if ((out[k] >> j) & 1) f[k * N + j] = CAP ? ABSENT : -INFINITY;
+          if ((out >> j) & 1) f[k * N + j] = CAP ? ABSENT : -INFINITY;
       }
+    }
+    if (CAP && b + TP_THREADS * U > v1) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (b + j / N * TP_THREADS + (int)threadIdx.x >= v1) f[j] = ABSENT;
     }
     if (CAP) {
       float least = f[0];
@@ -896,18 +866,60 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 4 : 6)
   if (C > 1) {
     cluster_wait();   // the first CTA runs
     if (threadIdx.x == 0) {
-      const uint32_t at = mapa_shared(smem_u32(&slices[part]), 0);
+      const uint32_t at = mapa_shared(smem_u32(&parts[part]), 0);
       store_cluster(at, a.m);
       store_cluster(at + 4, a.s);
     }
     cluster_arrive();
     cluster_wait();
     if (part != 0) return;
-    a = Stats{slices[0].m, slices[0].s, 0.f};
-    for (int i = 1; i < C; ++i) a = combine(a, Stats{slices[i].m, slices[i].s, 0.f}, p.sc.c);
+    a = Stats{parts[0].m, parts[0].s, 0.f};
+    for (int i = 1; i < C; ++i) a = combine(a, Stats{parts[i].m, parts[i].s, 0.f}, p.sc.c);
   }
-  if (threadIdx.x < 32) distill_row(pairs, a, row, p);
+
+  // ---- the teacher and the row
+  const double ln2 = 0.69314718055994530942;
+  if (!in) t = -INFINITY;
+  y = in ? p.sc.capped(y) : -INFINITY;
+  Stats st = empty_stats();
+  if (in) add_class(st, y, p.sc);
+  const Stats all = combine(block_combine(st, red, p.sc.c), a, p.sc.c);
+  double t_shift = 0.0;
+  if (p.renormalize) {
+    float t_max = t;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) t_max = fmaxf(t_max, __shfl_xor_sync(0xffffffffu, t_max, off));
+    if ((threadIdx.x & 31) == 0) red_d[threadIdx.x >> 5] = (double)t_max;
+    __syncthreads();
+    for (int i = 0; i < OB_TOP_K_MAX / 32; ++i) t_max = fmaxf(t_max, (float)red_d[i]);
+    if (t_max > -INFINITY) t_shift = (double)t_max;
+  }
+  const bool any = __syncthreads_or(in && !(p.renormalize && t == -INFINITY));
+  double q = in ? exp((double)t - t_shift) : 0.0;
+  const double sum = block_sum(q, red_d);
+  const bool others = !no_class(a);
+  const float log_s = log2f(all.s), rest_log_s = log2f(a.s);
+  double mass = sum, rest = 0.0, log_norm = t_shift;
+  if (p.renormalize) {
+    log_norm += log(sum);
+    mass = 1.0;
+    q /= sum;
+  } else if (others) {
+    rest = fmax(0.0, 1.0 - sum);
+  }
+  const double lp = y == -INFINITY ? -INFINITY : (((double)y - all.m) * p.sc.c - log_s) * ln2;
+  double loss = block_sum(in && q != 0.0 ? q * ((double)t - log_norm - lp) : 0.0, red_d);
+  if ((int)threadIdx.x < p.k) p.q[row * p.k + threadIdx.x] = in && any ? (float)q : -1.f;
+  if (threadIdx.x == 0) {
+    const double total = mass + rest, rest_lp = (((double)a.m - all.m) * p.sc.c + rest_log_s - log_s) * ln2;
+    if (rest > 0.0) loss += rest * (log(rest) - rest_lp);
+    p.row_loss[row] = any ? (float)loss : 0.f;
+    float4* o = reinterpret_cast<float4*>(p.row_stats + row * 8);
+    o[0] = make_float4(any ? (float)total : -1.f, others && any ? (float)(total * exp(rest_lp) - rest) : 0.f, 0.f, 0.f);
+    o[1] = make_float4(all.m, log_s, a.m, rest_log_s);
+  }
 }
+static_assert(OB_TOP_K_MAX <= TP_THREADS, "one thread per class of the teacher");
 
 struct DistillGradArgs {
   const void* teacher_ids;
@@ -922,7 +934,7 @@ struct DistillGradArgs {
 };
 
 template <class T, class D, bool CAP>
-__global__ void __launch_bounds__(GRAD_THREADS, CAP ? 4 : 6)
+__global__ void __launch_bounds__(GRAD_THREADS, 6)
     distill_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts, int per_block,
                        DistillGradArgs p) {
   const long long row = blockIdx.x / (unsigned)parts;
@@ -941,27 +953,8 @@ __global__ void __launch_bounds__(GRAD_THREADS, CAP ? 4 : 6)
   const bool nothing = st.x < 0.f || (norm.x == -INFINITY && norm.y == -INFINITY);
   const bool zero = nothing || (norm.z == -INFINITY && norm.w == -INFINITY);   // no class outside the teacher's
   const float coef = st.y * gs * p.sc.inv_temp * (CAP ? 4.f : 1.f);
-  const float t0 = (p.sc.cap - norm.z) * p.sc.c - norm.w, t1 = -2.f * p.sc.cap * p.sc.c;
   const int2 span = map_span<T, D>(z, d, p.V, part, parts, per_block, [&](auto& f, int) {
-    constexpr int M = sizeof(f) / sizeof(float);
-    if (zero) {
-#pragma unroll
-      for (int j = 0; j < M; ++j) f[j] = 0.f;
-      return;
-    }
-    if (CAP) p.sc.reciprocals(f);
-    float g[M + 1];
-#pragma unroll
-    for (int j = 0; j < M; j += 2) {
-      const float2 x = make_float2(f[j], j + 1 < M ? f[j + 1] : f[j]);
-      const float2 t = CAP ? fma2(x, make_float2(t1, t1), make_float2(t0, t0))
-                           : fma2(add2(x, make_float2(-norm.z, -norm.z)), make_float2(p.sc.c, p.sc.c), make_float2(-norm.w, -norm.w));
-      const float2 o = mul2(make_float2(exp2_fast(t.x), exp2_fast(t.y)), make_float2(coef, coef));
-      g[j] = o.x;
-      g[j + 1] = o.y;
-    }
-#pragma unroll
-    for (int j = 0; j < M; ++j) f[j] = CAP ? g[j] * fmaf(-f[j], f[j], f[j]) : g[j];
+    rest_gradient<CAP>(f, zero, norm.z, norm.w, coef, p.sc);
   });
   // the teacher's classes, over what has just been written for them
   __syncthreads();
@@ -1088,13 +1081,13 @@ template <class T, int U, bool CAP>
 static int launch_distill(const T* logits, long long ld, long long rows, const DistillArgs& args, cudaStream_t stream) {
   constexpr int N = Row<T>::N, LIMIT = 160 * 1024;
   auto kernel = distill_fwd_kernel<T, U, CAP>;
-  const int C = ctas_per_row(rows, args.V, TP_THREADS * U * N);
-  // a bit for each class of a slice, with the row's head, tail and the rounding of its vectors
-  const int bytes = (args.V / C + 4 * N + 31) / 32 * 4;
-  if (bytes > LIMIT) OB_FAIL(-6, "distillation: %d classes are more than %d", args.V, LIMIT * 8);
+  const int C = ctas_per_row(rows, args.V, TP_THREADS * U * N), vectors = args.V / N / C + 1;
+  // a bit for each vector of whole batches and a bit for each class, with the row's head and tail
+  const int bytes = (vectors + TP_THREADS * U - 1) / (TP_THREADS * U) * (TP_THREADS * U / 8) + (vectors * N + 4 * N + 31) / 32 * 4;
+  if (bytes > LIMIT) OB_FAIL(-6, "distillation: no room in shared memory for the bits of %d classes", args.V);
   static bool done[64] = {};
   if (int rc = allow_shared(kernel, LIMIT, done)) return rc;
-  return launch_clusters(kernel, rows * C, C, bytes, stream, logits, ld, C, args);
+  return launch_clusters(kernel, rows * C, C, bytes, stream, logits, ld, C, vectors, args);
 }
 
 // Calls launch(z, d, parts, per_block) with the types of the logits and of their gradient and the spans of a row.
