@@ -426,10 +426,10 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, unsigned long long 
 // threads by chance; it is looked for at the first batch, whenever STEP more groups have come together, and at the end if there are many.  Then the
 // classes of the groups above it are read again and put in order.
 template <class T, int U, bool CAP, bool TOP>
-__global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 4 : 6)
+__global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 4 : sizeof(T) == 2 ? 5 : 6)
     token_log_probs_fwd_kernel(const T* __restrict__ logits, long long ld, int C, ScoreArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
-  constexpr bool AHEAD = TOP || CAP;
+  constexpr bool AHEAD = TOP || CAP || sizeof(T) == 2;
   extern __shared__ __align__(16) char shared_bytes[];
   TopWork& work = *reinterpret_cast<TopWork*>(shared_bytes);                     // TOP
   Slice* slices = reinterpret_cast<Slice*>(shared_bytes + sizeof(TopWork));      // TOP, one per CTA of the cluster
