@@ -43,6 +43,8 @@
 
 #include "host_common.h"
 #include "sm100.cuh"
+#include "token_probs.h"
+#include "token_stats.cuh"
 
 namespace ob {
 
@@ -115,7 +117,34 @@ struct KernelParams {
   uint8_t* pf_dst;             // staging slot of shard 0 (shard s at + s * pf_dst_stride)
   long long pf_dst_stride;
   long long pf_off, pf_bytes;  // multiples of 16
+  // Scores of tokens in place of an output (kernels of their own)
+  const long long* score_ids;
+  float4* score_parts;         // [column tile][M]
+  float* score_target;
+  int score_rows;
+  Scaling score_sc;
 };
+
+// Statistics of 32 logits of a row from a tile's columns [col, col + 32), of which the first n are there.
+template <bool CAP>
+__device__ __forceinline__ void score_columns(Stats& a, float (&f)[32], int n, const Scaling& sc) {
+  if (CAP) sc.reciprocals(f);
+  if (n < 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j >= n) f[j] = CAP ? ABSENT : -INFINITY;
+  }
+  float mx;
+  if (CAP) {
+    float least = f[0];
+#pragma unroll
+    for (int j = 1; j < 32; ++j) least = fminf(least, f[j]);
+    mx = sc.of_r(least);
+  } else {
+    mx = largest(f);
+  }
+  add_classes<CAP, true, 32>(a, f, mx, sc);
+}
 
 // One warp-interleaved copy of n16 16-byte words; cw = this copy warp's index among n_cw.
 __device__ __forceinline__ void warp_copy16(const uint4* __restrict__ src, uint4* __restrict__ dst, long long n16, int cw,
@@ -218,7 +247,9 @@ __device__ __forceinline__ const CUtensorMap* pick_segment(const CUtensorMap* s0
 // issue that comes later after its stage is freed is a load that arrives later.  With the choice of the map in that loop of
 // every kernel, GEMMs without segments took 2-3 % longer (65536 x 3072 x 1024 297 us, now 287; 8192 x 12288 x 4096 541, now
 // 528) and contractions over segments 6 % (8192 x 4096 x 22016 1030, now 969; 966 of one tensor); one branch per map took 10 %.
-template <bool A_MN, bool B_MN, int CG, int BN, bool SEG>
+// SCORE: in place of C the epilogue gives the statistics of its columns' softmax (token_stats.cuh): 256 exponentials a row and tile, of which the
+// special-function unit does 16 a clock, run under the next tile's main loop, and the logits never leave the SM.
+template <bool A_MN, bool B_MN, int CG, int BN, bool SEG, bool SCORE = false>
 __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
                                           const CUtensorMap& tmC, const CUtensorMap& tmS1, const CUtensorMap& tmS2,
                                           const KernelParams& p) {
@@ -565,7 +596,31 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         cbase = reinterpret_cast<uint8_t*>(p.c);
         row_off = (long long)(m_shard * p.M_s + m_local0 + row_in_tile) * p.ldc + n_glob0;
       }
-      if (BN == BN_WIDE && glu && p.tma_epi) {
+      if constexpr (SCORE) {
+        const int row = m_local0 + row_in_tile;   // (one M shard)
+        const bool scored = row < p.score_rows;
+        long long want = -1;   // the token's column in this tile
+        if (scored && p.score_ids != nullptr) want = p.score_ids[row] - n_glob0;
+        if (want >= n_valid) want = -1;
+        Stats a = empty_stats();
+        for (int c0 = 0; c0 < BN; c0 += 32) {
+          if (c0 >= n_valid) break;  // warp-uniform
+          uint32_t x[32];
+          tmem_ld32(t_row + (uint32_t)c0, x);
+          tmem_ld_wait();
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(x[j]);
+          if (want >= c0 && want < c0 + 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (want == c0 + j) p.score_target[row] = f[j];
+          }
+          if (p.score_sc.cap > 0.f) score_columns<true>(a, f, n_valid - c0, p.score_sc);
+          else score_columns<false>(a, f, n_valid - c0, p.score_sc);
+        }
+        if (scored) p.score_parts[(long long)nt * p.M + row] = make_float4(a.m, a.s, a.w, 0.f);
+      } else if (BN == BN_WIDE && glu && p.tma_epi) {
         // Gated epilogue, columns [0, 128) = gate, [128, 256) = up: 64 output columns at a time, the activation and (when
         // kept for the backward pass) the two pre-activations staged one after the other and stored by TMA.  With a k loop
         // of 16 iterations this epilogue is longer than the main loop: 65536 x 2816 x 1024 (three outputs) took 898 us with
@@ -890,6 +945,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
   gemm_body<A_MN, B_MN, 2, BN_WIDE, SEG>(tmA, tmB, tmB2, tmC, tmS1, tmS2, p);
 }
 
+// The scores of tokens: K-major operands, no output.
+template <int BN>
+__global__ void __launch_bounds__(GEMM_THREADS, 1)
+    gemm_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const KernelParams p) {
+  gemm_body<false, false, 1, BN, false, true>(tmA, tmB, tmB, tmB, tmB, tmB, p);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
+    gemm_scores_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const KernelParams p) {
+  gemm_body<false, false, 2, BN_WIDE, false, true>(tmA, tmB, tmB, tmB, tmB, tmB, p);
+}
+
 constexpr int MAX_DEVICES = 64;
 
 // The tensor maps of a launch; S1 / S2 are the second and third output of the gated epilogue, or the segments after the
@@ -919,6 +985,26 @@ static int launch(const Maps& m, const KernelParams& kp, int grid, cudaStream_t 
     }
     gemm_bf16_kernel<A_MN, B_MN, BN, SEG><<<grid, GEMM_THREADS, smem, stream>>>(m.A, m.B, m.B2, m.C, m.S1, m.S2, kp);
   }
+  OB_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+template <int CG, int BN>
+static int launch_scores_gemm(const Maps& m, const KernelParams& kp, int grid, cudaStream_t stream) {
+  static bool attr_set[MAX_DEVICES] = {};
+  int dev = 0;
+  OB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= MAX_DEVICES) OB_FAIL(-20, "device index %d out of range", dev);
+  constexpr int smem = Geo<CG, BN>::SMEM_BYTES;
+  auto kernel = [] {
+    if constexpr (CG == 2) return gemm_scores_pair_kernel;
+    else return gemm_scores_kernel<BN>;
+  }();
+  if (!attr_set[dev]) {
+    OB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attr_set[dev] = true;
+  }
+  kernel<<<grid, GEMM_THREADS, smem, stream>>>(m.A, m.B, kp);
   OB_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -970,11 +1056,11 @@ static bool split_k_enabled() {
   return v != 0;
 }
 
-}  // namespace ob
+// Column tiles of at most this many columns in more than one wave (narrower ones come in one wave, at most one tile per SM).
+static long long score_tiles(int N, int N_s) { return (long long)(N / N_s) * ((N_s + BN_WIDE - 1) / BN_WIDE); }
 
-using namespace ob;
-
-extern "C" int ob_gemm_bf16(const ObGemmArgs* a, cudaStream_t stream) {
+// ob_gemm_bf16; with `scores` the kernels that give them, and in *n_tiles their column tiles.
+static int run_gemm(const ObGemmArgs* a, const ObScoreArgs* scores, int* n_tiles, cudaStream_t stream) {
   if (a == nullptr) OB_FAIL(-1, "null args");
   if (a->M <= 0 || a->N <= 0 || a->Kc <= 0) OB_FAIL(-2, "empty problem M=%d N=%d K=%d", a->M, a->N, a->Kc);
   const bool glu = (a->epi == EPI_SWIGLU || a->epi == EPI_GEGLU);
@@ -1202,7 +1288,7 @@ extern "C" int ob_gemm_bf16(const ObGemmArgs* a, cudaStream_t stream) {
   }
   // Output map for the TMA epilogue (local destinations only; peer destinations keep the direct red.add path).
   kp.tma_epi = 0;
-  const bool tma_ok = (a->epi == EPI_BF16 || a->epi == EPI_F32 || a->epi == EPI_F32_ACC ||
+  const bool tma_ok = scores == nullptr && (a->epi == EPI_BF16 || a->epi == EPI_F32 || a->epi == EPI_F32_ACC ||
                        (glu && a->c_shard_stride <= 0 && (a->c2 == nullptr) == (a->c3 == nullptr))) && a->c_shards == nullptr &&
                       !a->no_tma_epilogue && (kp.m_shards == 1 || a->c_shard_stride > 0 || M_s % BM == 0) &&
                       // the store clips at the end of the matrix, not at a column shard's end: a shard's last tile may
@@ -1247,9 +1333,46 @@ extern "C" int ob_gemm_bf16(const ObGemmArgs* a, cudaStream_t stream) {
     kp.tma_epi = 2;
   if (a->c_shards != nullptr && a->epi == EPI_BF16_ACC && kp.tma_epi != 2)
     OB_FAIL(-18, "EPI_BF16_ACC towards c_shards needs the staged epilogue (16-byte aligned rows, local partial in c)");
+  if (scores != nullptr) {
+    *n_tiles = kp.n_shards * kp.n_tiles_per_shard;
+    if (4ll * a->M * *n_tiles > scores->parts_size) OB_FAIL(-21, "scores: scratch of %lld floats for %d x %d tiles", scores->parts_size, a->M, *n_tiles);
+    kp.score_ids = scores->ids;
+    kp.score_parts = reinterpret_cast<float4*>(scores->parts);
+    kp.score_target = scores->target;
+    kp.score_rows = (int)scores->rows;
+    kp.score_sc = scaling(scores->softcap, scores->inv_temp);
+    if (CG == 2) return launch_scores_gemm<2, BN_WIDE>(maps, kp, grid, stream);
+    if (BN == BN_NARROW) return launch_scores_gemm<1, BN_NARROW>(maps, kp, grid, stream);
+    return launch_scores_gemm<1, BN_WIDE>(maps, kp, grid, stream);
+  }
   if (CG == 2) return launch_tiles<2, BN_WIDE>(a->a_mn != 0, a->b_mn != 0, maps, kp, grid, stream);
   if (BN == BN_NARROW) return launch_tiles<1, BN_NARROW>(a->a_mn != 0, a->b_mn != 0, maps, kp, grid, stream);
   return launch_tiles<1, BN_WIDE>(a->a_mn != 0, a->b_mn != 0, maps, kp, grid, stream);
+}
+
+}  // namespace ob
+
+using namespace ob;
+
+extern "C" int ob_gemm_bf16(const ObGemmArgs* args, cudaStream_t stream) { return run_gemm(args, nullptr, nullptr, stream); }
+
+extern "C" long long ob_gemm_scores_parts(int M, int N, int N_s) {
+  if (M <= 0 || N <= 0 || N_s <= 0 || N % N_s) return 0;
+  const long long wide = score_tiles(N, N_s), one_wave = sm_count();
+  return 4ll * M * (wide > one_wave ? wide : one_wave);
+}
+
+extern "C" int ob_gemm_scores(const ObGemmArgs* a, const ObScoreArgs* s, cudaStream_t stream) {
+  if (a == nullptr || s == nullptr) OB_FAIL(-1, "null args");
+  if (a->a_mn || a->b_mn || a->seg != SEG_NONE || a->c_shards != nullptr || a->epi != EPI_F32 || a->c != nullptr || (a->M_s > 0 && a->M_s != a->M))
+    OB_FAIL(-22, "scores: K-major operands, one row shard and no output");
+  if (s->rows < 0 || s->rows > a->M || s->parts == nullptr || s->entropy == nullptr || (reinterpret_cast<uintptr_t>(s->parts) & 15) != 0 ||
+      (s->log_probs != nullptr && (s->ids == nullptr || s->target == nullptr)) || (s->ids != nullptr && s->target == nullptr))
+    OB_FAIL(-5, "scores: missing tensor");
+  int n_tiles = 0;
+  if (int rc = run_gemm(a, s, &n_tiles, stream)) return rc;
+  return ob_join_scores(s->parts, s->target, a->M, n_tiles, s->ids, s->log_probs, s->entropy, s->norm, s->rows, a->N, s->ignore_index,
+                        s->softcap, s->inv_temp, stream);
 }
 
 extern "C" const char* ob_last_error() { return ob::last_error_buf(); }

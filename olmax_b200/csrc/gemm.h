@@ -82,6 +82,25 @@ typedef struct ObGemmArgs {
 } ObGemmArgs;
 
 int ob_gemm_bf16(const ObGemmArgs* args, cudaStream_t stream);
+
+// Scores of tokens under the softmax of A . B^T (a language model's head), without C: the epilogue leaves every row's statistics of a tile's
+// columns and the column of its token in `parts` / `target`, and a second kernel joins them (ob_join_scores).
+typedef struct ObScoreArgs {
+  const long long* ids;    // [rows] or null
+  float* parts;            // scratch of parts_size floats, 16-byte aligned: 4 * M for every column tile (ob_gemm_scores_parts)
+  long long parts_size;
+  float* target;           // scratch [rows]
+  float* log_probs;        // [rows] or null
+  float* entropy;          // [rows]
+  float* norm;             // [rows, 2] or null
+  long long rows;          // rows of A that are there: the rest up to M is padding
+  int ignore_index;
+  float softcap, inv_temp;
+} ObScoreArgs;
+// floats of scratch that ob_gemm_scores needs at most for M rows and N columns in shards of N_s
+long long ob_gemm_scores_parts(int M, int N, int N_s);
+// A and B K-major, epi = EPI_F32, c null; shards of B, all-gather and prefetch as in ob_gemm_bf16.
+int ob_gemm_scores(const ObGemmArgs* args, const ObScoreArgs* scores, cudaStream_t stream);
 const char* ob_last_error();
 
 #ifdef __cplusplus

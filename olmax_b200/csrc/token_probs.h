@@ -21,6 +21,11 @@ extern "C" {
 int ob_token_log_probs_fwd(const void* logits, int dtype, long long ld, const long long* ids, float* log_probs, float* entropy,
                            float* norm, int top_k, float* top_log_probs, long long* top_ids, long long rows, int V,
                            int ignore_index, float softcap, float inv_temp, cudaStream_t stream);
+// The same of logits that exist as statistics of `n` groups of classes only: parts[i * stride + r] = four floats (largest capped logit m, sum 2^t, sum
+// 2^t t, unused) with t = (cap(z) - m) log2(e) inv_temp over group i, target[r] = the logit of class ids[r] (undefined where it is not scored).
+int ob_join_scores(const float* parts, const float* target, long long stride, int n, const long long* ids, float* log_probs,
+                   float* entropy, float* norm, long long rows, int V, int ignore_index, float softcap, float inv_temp,
+                   cudaStream_t stream);
 // dlogits (of dtype_d, row stride ld_d) = g_log_probs[r * stride_lp] * d log_probs[r] + g_entropy[r * stride_ent] * d entropy[r]
 // over d logits; either upstream gradient may be null.
 int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const long long* ids, const float* norm,

@@ -78,10 +78,31 @@ class ObGemmArgs(ctypes.Structure):
     ]
 
 
+class ObScoreArgs(ctypes.Structure):
+    _fields_ = [
+        ("ids", ctypes.c_void_p),
+        ("parts", ctypes.c_void_p),
+        ("parts_size", ctypes.c_longlong),
+        ("target", ctypes.c_void_p),
+        ("log_probs", ctypes.c_void_p),
+        ("entropy", ctypes.c_void_p),
+        ("norm", ctypes.c_void_p),
+        ("rows", ctypes.c_longlong),
+        ("ignore_index", ctypes.c_int),
+        ("softcap", ctypes.c_float),
+        ("inv_temp", ctypes.c_float),
+    ]
+
+
 def _declare(lib: ctypes.CDLL) -> None:
     lib.ob_last_error.restype = ctypes.c_char_p
     lib.ob_gemm_bf16.restype = ctypes.c_int
     lib.ob_gemm_bf16.argtypes = [ctypes.POINTER(ObGemmArgs), ctypes.c_void_p]
+    if hasattr(lib, "ob_gemm_scores"):
+        lib.ob_gemm_scores.restype = ctypes.c_int
+        lib.ob_gemm_scores.argtypes = [ctypes.POINTER(ObGemmArgs), ctypes.POINTER(ObScoreArgs), ctypes.c_void_p]
+        lib.ob_gemm_scores_parts.restype = ctypes.c_longlong
+        lib.ob_gemm_scores_parts.argtypes = [ctypes.c_int] * 3
     for name in ("ob_flash_attn_fwd", "ob_flash_attn_bwd"):
         if hasattr(lib, name):
             getattr(lib, name).restype = ctypes.c_int

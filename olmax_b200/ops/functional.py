@@ -1381,8 +1381,7 @@ class _HeadChunks:
             raise ValueError(f"chunk_rows must be positive, got {chunk_rows}")
         self.x2, self.handle = x2, handle
         self.M, self.V = x2.shape[0], handle.tp_shape[0]
-        if handle.tp_shape[1] != x2.shape[1]:
-            raise ValueError(f"hidden states of width {x2.shape[1]} do not fit a head of width {handle.tp_shape[1]}")
+        _check_width(x2, handle)
         self.step = max(8, min((chunk_rows + 7) // 8 * 8, (self.M + 7) // 8 * 8))
         self.padded = (self.M + 7) // 8 * 8
         self.logits = torch.empty((self.step, self.V), dtype=torch.float32, device=x2.device)
@@ -1391,9 +1390,7 @@ class _HeadChunks:
         """(first row, last row + 1, padded rows of x, logits of the real rows)."""
         for r0 in range(0, self.M, self.step):
             r1 = min(self.M, r0 + self.step)
-            xc = self.x2[r0:r1]
-            if (r1 - r0) % 8:
-                xc = torch.cat([xc, xc.new_zeros((-(r1 - r0) % 8, xc.shape[1]))])
+            xc = _whole_rows(self.x2[r0:r1])
             _gemm_fwd(xc, self.handle, out=self.logits[: xc.shape[0]], epi=K.EPI_F32)
             yield r0, r1, xc, self.logits[: r1 - r0]
 
@@ -1406,10 +1403,7 @@ class _HeadChunks:
 
     def finish(self, dlogits, single):
         if single:
-            x2 = self.x2
-            if self.padded > self.M:
-                x2 = torch.cat([x2, x2.new_zeros((self.padded - self.M, x2.shape[1]))])
-            _gemm_wgrad(dlogits, x2, self.handle)
+            _gemm_wgrad(dlogits, _whole_rows(self.x2), self.handle)
             self.handle.store.reduce_unit_now(self.handle.unit)
 
     def chunk_gradient(self, dlogits, single, r0, r1, xc, dx):
@@ -1433,9 +1427,39 @@ class _HeadChunks:
         return dlogits[at : at + r1 - r0]
 
 
+# Rows of one GEMM that gives scores: its scratch holds 16 bytes per row and 256 classes
+_SCORE_ROWS = 16384
+
+
+def _gemm_scores(x2: torch.Tensor, handle, ids, log_probs, entropy, norm, **options) -> None:
+    """Scores of ``x2 @ W^T`` out of the GEMM's epilogue, W read from the gathered unit buffer as in :func:`_gemm_fwd`."""
+    M, Kd = x2.shape
+    N = handle.tp_shape[0]
+    _check_width(x2, handle)
+    for r0 in range(0, M, _SCORE_ROWS):
+        r1 = min(M, r0 + _SCORE_ROWS)
+        xc = _whole_rows(x2[r0:r1])
+        first, kw = _b_operand(handle)
+        kw.update(_ag_kwargs(handle))
+        kw["prefetch"] = handle.store.prefetch_slice(N * Kd)
+        cut = [t[r0:r1] if t is not None else None for t in (ids, log_probs, entropy, norm)]
+        K.gemm_scores(xc, first, *cut, xc.shape[0], N, Kd, rows=r1 - r0, **kw, **options)
+
+
+def _check_width(x2: torch.Tensor, handle) -> None:
+    if handle.tp_shape[1] != x2.shape[1]:
+        raise ValueError(f"hidden states of width {x2.shape[1]} do not fit a head of width {handle.tp_shape[1]}")
+
+
+def _whole_rows(x: torch.Tensor) -> torch.Tensor:
+    """x with zero rows behind it up to a multiple of 8, which the GEMMs take."""
+    pad = -x.shape[0] % 8
+    return torch.cat([x, x.new_zeros((pad, x.shape[1]))]) if pad else x
+
+
 class _LinearTokenLogProbsFn(torch.autograd.Function):
-    """:class:`_TokenLogProbsFn` of ``x @ W^T`` without the logits of more than ``chunk_rows`` rows: they are computed again in the
-    backward pass, which then forms the gradients of x and of the weight chunk by chunk."""
+    """:class:`_TokenLogProbsFn` of ``x @ W^T`` without the logits (with ``top_k`` without those of more than ``chunk_rows`` rows): they are
+    computed in the backward pass, which then forms the gradients of x and of the weight chunk by chunk."""
 
     @staticmethod
     def forward(ctx, x2, handle, ids, top_k, ignore_index, cap, temperature, chunk_rows):
@@ -1452,9 +1476,12 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
             norm = torch.empty((M, 2), dtype=torch.float32, device=dev) if keep else None
             top = torch.empty((M, top_k), dtype=torch.float32, device=dev) if top_k else None
             top_ids = torch.empty((M, top_k), dtype=torch.int64, device=dev) if top_k else None
-            for r0, r1, _, z in _HeadChunks(x2, handle, chunk_rows):
-                cut = [t[r0:r1] if t is not None else None for t in (ids, log_probs, entropy, norm, top, top_ids)]
-                K.token_log_probs_fwd(z, *cut, softcap=cap, **ctx.options)
+            if top_k:   # (the classes themselves need the logits)
+                for r0, r1, _, z in _HeadChunks(x2, handle, chunk_rows):
+                    cut = [t[r0:r1] if t is not None else None for t in (ids, log_probs, entropy, norm, top, top_ids)]
+                    K.token_log_probs_fwd(z, *cut, softcap=cap, **ctx.options)
+            else:
+                _gemm_scores(x2, handle, ids, log_probs, entropy, norm, softcap=cap, **ctx.options)
         else:
             z = (x2 @ handle.full().t()).float()
             log_probs, entropy, norm, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
@@ -1490,8 +1517,9 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
 def linear_token_log_probs(x: torch.Tensor, handle, ids: Optional[torch.Tensor] = None, *, top_k: int = 0,
                            temperature: float = 1.0, logit_softcap: Optional[float] = None, ignore_index: int = -100,
                            chunk_rows: int = 2048) -> TokenLogProbs:
-    """:func:`token_log_probs` of the LM head ``x @ W^T`` (``handle``: the ``(vocab, d)`` weight, x ``[..., d]``), whose logits exist
-    ``chunk_rows`` rows at a time.  Differentiable with respect to x and the weight (the logits are computed again)."""
+    """:func:`token_log_probs` of the LM head ``x @ W^T`` (``handle``: the ``(vocab, d)`` weight, x ``[..., d]``), whose logits are
+    never formed: their statistics come out of the GEMM's epilogue.  With ``top_k``, and in the backward pass (it is differentiable
+    with respect to x and the weight), they exist ``chunk_rows`` rows at a time."""
     cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap, top_k)
     shape = x.shape[:-1]
     lab = _token_rows(ids, shape, x.device) if ids is not None else None

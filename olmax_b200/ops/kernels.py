@@ -19,7 +19,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import KernelError, ObAttnArgs, ObGemmArgs, check, lib, register_signature, status_buffer, stream_ptr
+from ._lib import KernelError, ObAttnArgs, ObGemmArgs, ObScoreArgs, check, lib, register_signature, status_buffer, stream_ptr
 
 __all__ = [
     "EPI_BF16", "EPI_F32", "EPI_F32_ACC", "EPI_F32_RED", "EPI_SWIGLU", "EPI_GEGLU", "EPI_BF16_ACC",
@@ -28,7 +28,7 @@ __all__ = [
     "embed_gather", "embed_scatter", "ce_fwd_bwd", "ce_vp_stats", "ce_vp_grad", "count_valid", "adamw", "sumsq", "clip_coef", "cast_f32_bf16",
     "layernorm_fwd", "layernorm_bwd", "gather_shards", "scatter_add_shards", "allreduce_p2p", "allreduce_multimem",
     "peer_barrier", "peer_signal", "peer_wait", "copy_bytes", "push_copy", "fold_slots_bf16", "reduce_slots",
-    "token_log_probs_fwd", "token_log_probs_bwd", "distill_work", "distill_fwd", "distill_bwd", "distill_reduce", "distill_count", "TOP_K_MAX",
+    "gemm_scores", "token_log_probs_fwd", "token_log_probs_bwd", "distill_work", "distill_fwd", "distill_bwd", "distill_reduce", "distill_count", "TOP_K_MAX",
     "launch_count", "reset_launch_count", "pointer_table",
     "timing_enabled", "set_timing", "timed_region", "timing_report", "format_timing",
 ]
@@ -112,6 +112,13 @@ def _req_bf16(*ts: Optional[torch.Tensor]) -> None:
 def pointer_table(ptrs: Sequence[int], device: torch.device) -> torch.Tensor:
     """int64 CUDA tensor holding raw pointers (what the kernels take as ``T* const*``)."""
     return torch.tensor(list(ptrs), dtype=torch.int64, device=device)
+
+
+def _set_prefetch(args: ObGemmArgs, prefetch: Optional[tuple]) -> None:
+    if prefetch is not None:
+        table, dst_ptr, dst_stride, off, nbytes, shards, rank = prefetch
+        args.pf_src, args.pf_dst, args.pf_dst_stride = table.data_ptr(), dst_ptr, dst_stride
+        args.pf_off, args.pf_bytes, args.pf_shards, args.pf_rank = off, nbytes, shards, rank
 
 
 def gemm(
@@ -201,12 +208,32 @@ def gemm(
             args.seg_len[i] = t.shape[-1]
             if i > 0:
                 args.seg_ptr[i - 1], args.seg_ld[i - 1] = t.data_ptr(), t.stride(0)
-    if prefetch is not None:
-        table, dst_ptr, dst_stride, off, nbytes, shards, rank = prefetch
-        args.pf_src, args.pf_dst, args.pf_dst_stride = table.data_ptr(), dst_ptr, dst_stride
-        args.pf_off, args.pf_bytes, args.pf_shards, args.pf_rank = off, nbytes, shards, rank
+    _set_prefetch(args, prefetch)
     check(lib().ob_gemm_bf16(ctypes.byref(args), stream_ptr(a.device)), "gemm")
     _count()
+
+
+def gemm_scores(a, b, ids, log_probs, entropy, norm, M: int, N: int, K: int, *, rows: int, N_s: int = 0, b_shard_stride: int = 0,
+                ag_src=None, ag_flags=None, ag_rank: int = 0, prefetch: Optional[tuple] = None, ignore_index: int = -100,
+                softcap: float = 0.0, temperature: float = 1.0) -> None:
+    """:func:`token_log_probs_fwd` of the logits ``A[M, K] . B[N, K]^T`` without the logits: their statistics come out of the GEMM's
+    epilogue.  The first ``rows`` rows are there; B's shards, all-gather and prefetch as in :func:`gemm`."""
+    _req_bf16(a, b)
+    with _on(a.device):
+        size = lib().ob_gemm_scores_parts(M, N, N_s or N)
+        scratch = torch.empty(size + M, dtype=torch.float32, device=a.device)
+        args, sc = ObGemmArgs(), ObScoreArgs()
+        args.a, args.lda, args.b, args.ldb = a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0)
+        args.M, args.N, args.Kc, args.N_s, args.b_shard_stride = M, N, K, N_s, b_shard_stride
+        args.epi, args.alpha, args.status = EPI_F32, 1.0, status_buffer(a.device).data_ptr()
+        if ag_src is not None:
+            args.ag_src, args.ag_flags, args.ag_rank = ag_src.data_ptr(), _ptr(ag_flags), ag_rank
+        _set_prefetch(args, prefetch)
+        sc.ids, sc.log_probs, sc.entropy, sc.norm = _ptr(ids), _ptr(log_probs), entropy.data_ptr(), _ptr(norm)
+        sc.parts, sc.parts_size, sc.target = scratch.data_ptr(), size, scratch.data_ptr() + 4 * size
+        sc.rows, sc.ignore_index, sc.softcap, sc.inv_temp = rows, ignore_index, softcap, 1.0 / temperature
+        check(lib().ob_gemm_scores(ctypes.byref(args), ctypes.byref(sc), stream_ptr(a.device)), "gemm_scores")
+    _count(2)
 
 
 _BSHD = {f: (f, *((f if f != "d_o" else "do") + s for s in ("_sb", "_ss", "_sh")))
@@ -717,7 +744,7 @@ def format_timing(report: dict, top: int = 40) -> str:
 
 for _name in ("gemm", "flash_attn_fwd", "flash_attn_bwd", "rmsnorm_fwd", "rmsnorm_bwd", "rmsnorm_rope_fwd",
               "rmsnorm_rope_bwd", "layernorm_fwd", "layernorm_bwd",
-              "rope", "rope_pair", "glu_fwd", "glu_bwd", "embed_gather", "embed_scatter", "ce_fwd_bwd", "ce_vp_stats", "ce_vp_grad", "token_log_probs_fwd", "token_log_probs_bwd",
+              "rope", "rope_pair", "glu_fwd", "glu_bwd", "embed_gather", "embed_scatter", "ce_fwd_bwd", "ce_vp_stats", "ce_vp_grad", "gemm_scores", "token_log_probs_fwd", "token_log_probs_bwd",
               "distill_fwd", "distill_bwd", "distill_reduce", "distill_count", "count_valid",
               "adamw", "sumsq",
               "clip_coef", "cast_f32_bf16", "gather_shards", "scatter_add_shards", "allreduce_p2p", "allreduce_multimem",

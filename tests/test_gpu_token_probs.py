@@ -484,3 +484,57 @@ def test_top_classes_of_long_rows_in_bad_orders(dtype):
             out = F.token_log_probs(part, top_k=k)
             want = part.sort(dim=-1, descending=True, stable=True).indices[:, :k]
             assert torch.equal(out.top_ids, want)
+
+
+@pytest.mark.parametrize("rows,V,d,cap,temperature", [(1, 8, 64, None, 1.0), (7, 264, 128, None, 1.0), (300, 1000, 256, 30.0, 0.7), (2048, 5000, 512, None, 1.0),
+                                                      (1100, 20008, 72, None, 2.0), (328, 50304, 128, 30.0, 1.0)])
+def test_head_scores_out_of_the_epilogue(rows, V, d, cap, temperature):
+    """Tiles of both geometries, ragged in rows, classes and contraction, against the same head's fp32 logits."""
+    head = _bf16_head(V, d, cap)
+    w = head.weight.full()
+    x = torch.randn(rows, d, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(torch.bfloat16)
+    ids = _ids(rows, V)
+    z = x.double() @ w.double().t()
+    gemm = d * 2.0 ** -24 * float((x.double().abs() @ w.double().abs().t()).max())
+    y_max = min(float(z.abs().max()), cap or math.inf) / temperature
+    lp, ent, _, _ = scores_64(z, ids, 1, temperature, cap or 0.0)
+    e = _eps(V, y_max, cap or 0.0, temperature) + 2 * gemm / temperature
+    with torch.no_grad():
+        out = head.token_log_probs(x, ids, temperature=temperature)
+        none = head.token_log_probs(x, temperature=temperature)
+        three = head.token_log_probs(x.view(1, rows, d), ids.view(1, rows), temperature=temperature)
+    _close(out.log_probs, lp, 2 * e)
+    _close(out.entropy, ent, (2 + ent) * e)
+    assert none.log_probs is None and torch.equal(none.entropy, out.entropy) and torch.equal(three.log_probs[0], out.log_probs)
+    from olmax_b200.ops import _lib
+
+    _lib.check_status()
+
+
+def test_head_scores_of_weight_shards():
+    """B in row blocks a stride apart, as a gathered unit is laid out."""
+    from olmax_b200.ops import kernels as K
+
+    M, N, Kd, R, rows = 512, 2400, 256, 4, 509
+    g = torch.Generator(device=DEV).manual_seed(5)
+    a = torch.randn(M, Kd, generator=g, device=DEV).to(torch.bfloat16)
+    stride = (N // R) * Kd + 1024
+    buf = torch.randn(R * stride, generator=g, device=DEV).to(torch.bfloat16)
+    b = torch.cat([buf[r * stride : r * stride + (N // R) * Kd].view(N // R, Kd) for r in range(R)])
+    ids = _ids(rows, N)
+    out = [[torch.full((rows + 1,), 7.0, device=DEV) for _ in range(2)] for _ in range(2)]
+    K.gemm_scores(a, b, ids, out[0][0][:rows], out[0][1][:rows], None, M, N, Kd, rows=rows)
+    K.gemm_scores(a, buf[: (N // R) * Kd].view(N // R, Kd), ids, out[1][0][:rows], out[1][1][:rows], None, M, N, Kd, rows=rows, N_s=N // R,
+                  b_shard_stride=stride)
+    z = a.double() @ b.double().t()
+    lp, ent, _, _ = scores_64(z[:rows], ids, 1)
+    gemm = Kd * 2.0 ** -24 * float((a.double().abs() @ b.double().abs().t()).max())
+    e = _eps(N, float(z.abs().max())) + 2 * gemm
+    for lp_got, ent_got in out:
+        _close(lp_got[:rows], lp, 2 * e)
+        _close(ent_got[:rows], ent, (2 + ent) * e)
+        assert lp_got[rows] == 7.0 and ent_got[rows] == 7.0       # rows behind the last one are left as they were
+    with pytest.raises(K.KernelError):
+        K.gemm_scores(a, b, ids, out[0][0], out[0][1], None, M, N, Kd, rows=M + 1)
+    with pytest.raises(K.KernelError):
+        K.gemm_scores(a, b, ids, out[0][0], out[0][1], None, M, N, Kd - 4, rows=rows)
