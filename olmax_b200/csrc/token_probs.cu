@@ -438,24 +438,30 @@ __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 4 : sizeof(T) == 2 ? 
   }
 }
 
-// The scores of rows whose statistics lie in `n` parts, parts[i * stride + row] = (m, s, w, -): eight threads per row, parts in order.
-__global__ void __launch_bounds__(256)
+// The scores of rows whose statistics lie in `n` parts, parts[i * stride + row] = (m, s, w, -).  A block has 32 rows: a warp reads every 32nd part of
+// them, row by lane, and joins one row, part by lane.
+__global__ void __launch_bounds__(1024)
     join_scores_kernel(const float4* __restrict__ parts, const float* __restrict__ target, long long stride, int n, long long rows,
                        ScoreArgs p) {
-  __shared__ Stats red[8][32];
-  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
-  const long long row = (long long)blockIdx.x * 32 + lane;
+  __shared__ Stats red[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row0 = (long long)blockIdx.x * 32, row = row0 + warp;
+  constexpr int U = 4;
   Stats a = empty_stats();
-  if (row < rows) {
-    for (int i = group; i < n; i += 8) {
-      const float4 x = parts[i * stride + row];
-      a = combine(a, Stats{x.x, x.y, x.z}, p.sc.c);
+  if (row0 + lane < rows) {
+    for (int i0 = warp; i0 < n; i0 += 32 * U) {
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        x[u] = i0 + u * 32 < n ? parts[(i0 + u * 32) * stride + row0 + lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) a = combine(a, Stats{x[u].x, x[u].y, x[u].z}, p.sc.c);
     }
   }
-  red[group][lane] = a;
+  red[warp][lane] = a;
   __syncthreads();
-  if (group != 0 || row >= rows) return;
-  for (int i = 1; i < 8; ++i) a = combine(a, red[i][lane], p.sc.c);
+  a = shuffle_combine(red[lane][warp], 16, p.sc.c);
+  if (lane != 0 || row >= rows) return;
   const float log_s = log2f(a.s);
   if (p.log_probs != nullptr) {
     const long long id = p.ids[row];
@@ -1033,7 +1039,7 @@ extern "C" int ob_join_scores(const float* parts, const float* target, long long
     OB_FAIL(-5, "scores of parts: missing tensor");
   if (n < 1 || stride < rows || rows > 32ll * INT_MAX) OB_FAIL(-3, "scores of parts: %lld rows in %d parts %lld apart", rows, n, stride);
   const ScoreArgs args{ids, log_probs, entropy, norm, 0, nullptr, nullptr, V, ignore_index, scaling(softcap, inv_temp)};
-  join_scores_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>((const float4*)parts, target, stride, n, rows, args);
+  join_scores_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>((const float4*)parts, target, stride, n, rows, args);
   OB_CUDA_OK(cudaGetLastError());
   return 0;
 }

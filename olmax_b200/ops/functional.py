@@ -1457,6 +1457,28 @@ def _whole_rows(x: torch.Tensor) -> torch.Tensor:
     return torch.cat([x, x.new_zeros((pad, x.shape[1]))]) if pad else x
 
 
+def _linear_scores(x2: torch.Tensor, handle, ids, top_k: int, ignore_index: int, cap: float, temperature: float, chunk_rows: int,
+                   keep: bool):
+    """:func:`_scores` of ``x2 @ W^T``."""
+    if not _on_gpu(x2):
+        return _scores((x2 @ handle.full().t()).float(), ids, top_k, ignore_index, cap, temperature, keep)
+    M, dev = x2.shape[0], x2.device
+    options = dict(ignore_index=ignore_index, softcap=cap, temperature=temperature)
+    log_probs = torch.empty(M, dtype=torch.float32, device=dev) if ids is not None else None
+    entropy = torch.empty(M, dtype=torch.float32, device=dev)
+    norm = torch.empty((M, 2), dtype=torch.float32, device=dev) if keep else None
+    if not top_k:
+        _gemm_scores(x2, handle, ids, log_probs, entropy, norm, **options)
+        return log_probs, entropy, None, None, norm
+    # the classes themselves need the logits
+    top = torch.empty((M, top_k), dtype=torch.float32, device=dev)
+    top_ids = torch.empty((M, top_k), dtype=torch.int64, device=dev)
+    for r0, r1, _, z in _HeadChunks(x2, handle, chunk_rows):
+        cut = [t[r0:r1] if t is not None else None for t in (ids, log_probs, entropy, norm, top, top_ids)]
+        K.token_log_probs_fwd(z, *cut, **options)
+    return log_probs, entropy, top, top_ids, norm
+
+
 class _LinearTokenLogProbsFn(torch.autograd.Function):
     """:class:`_TokenLogProbsFn` of ``x @ W^T`` without the logits (with ``top_k`` without those of more than ``chunk_rows`` rows): they are
     computed in the backward pass, which then forms the gradients of x and of the weight chunk by chunk."""
@@ -1467,26 +1489,8 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
         ctx.handle, ctx.chunk_rows = handle, chunk_rows
         ctx.options = dict(ignore_index=ignore_index, temperature=temperature)
         ctx.cap = cap
-        keep = bool(ctx.needs_input_grad[0])
-        M = x2.shape[0]
-        if _on_gpu(x2):
-            dev = x2.device
-            log_probs = torch.empty(M, dtype=torch.float32, device=dev) if ids is not None else None
-            entropy = torch.empty(M, dtype=torch.float32, device=dev)
-            norm = torch.empty((M, 2), dtype=torch.float32, device=dev) if keep else None
-            top = torch.empty((M, top_k), dtype=torch.float32, device=dev) if top_k else None
-            top_ids = torch.empty((M, top_k), dtype=torch.int64, device=dev) if top_k else None
-            if top_k:   # (the classes themselves need the logits)
-                for r0, r1, _, z in _HeadChunks(x2, handle, chunk_rows):
-                    cut = [t[r0:r1] if t is not None else None for t in (ids, log_probs, entropy, norm, top, top_ids)]
-                    K.token_log_probs_fwd(z, *cut, softcap=cap, **ctx.options)
-            else:
-                _gemm_scores(x2, handle, ids, log_probs, entropy, norm, softcap=cap, **ctx.options)
-        else:
-            z = (x2 @ handle.full().t()).float()
-            log_probs, entropy, norm, top, top_ids = ref.token_log_probs(z, ids, top_k, cap=cap, **ctx.options)
-        if keep:
-            ctx.save_for_backward(x2, ids, norm, entropy)
+        log_probs, entropy, top, top_ids, norm = _linear_scores(x2, handle, ids, top_k, ignore_index, cap, temperature, chunk_rows, True)
+        ctx.save_for_backward(x2, ids, norm, entropy)
         ctx.mark_non_differentiable(*(t for t in (top, top_ids) if t is not None))
         return log_probs, entropy, top, top_ids
 
@@ -1523,9 +1527,11 @@ def linear_token_log_probs(x: torch.Tensor, handle, ids: Optional[torch.Tensor] 
     cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap, top_k)
     shape = x.shape[:-1]
     lab = _token_rows(ids, shape, x.device) if ids is not None else None
-    x2 = x.reshape(math.prod(shape), x.shape[-1]).contiguous()
-    return _shaped(_LinearTokenLogProbsFn.apply(x2, handle, lab, int(top_k), int(ignore_index), cap, float(temperature),
-                                                int(chunk_rows)), shape, top_k)
+    x2 = (x if x.dim() == 2 else x.reshape(math.prod(shape), x.shape[-1])).contiguous()
+    args = (x2, handle, lab, int(top_k), int(ignore_index), cap, float(temperature), int(chunk_rows))
+    if x.requires_grad and torch.is_grad_enabled():
+        return _shaped(_LinearTokenLogProbsFn.apply(*args), shape, top_k)
+    return _shaped(_linear_scores(*args, False)[:4], shape, top_k)
 
 
 class _LinearDistillationFn(torch.autograd.Function):
