@@ -95,7 +95,8 @@ typedef struct ObScoreArgs {
   float* norm;             // [rows, 2] or null
   long long rows;          // rows of A that are there: the rest up to M is padding
   int ignore_index;
-  float softcap, inv_temp;
+  float softcap;
+  double inv_temp;
 } ObScoreArgs;
 // floats of scratch that ob_gemm_scores needs at most for M rows and N columns in shards of N_s
 long long ob_gemm_scores_parts(int M, int N, int N_s);

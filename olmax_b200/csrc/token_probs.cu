@@ -117,7 +117,7 @@ struct TopWork {
   static constexpr int EVERY = 4;                          // batches between two looks at the number of groups, but for the first ones
   static constexpr int LIMIT = 1536;                       // groups kept from one look to the next
   static constexpr int GROUPS = LIMIT + EVERY * TP_THREADS;   // ... and those that come until then
-  static constexpr int STEP = 192;
+  static constexpr int STEP = 128;
   static constexpr int CLASSES = 512;
   unsigned group_key[GROUPS];
   int group[GROUPS];
@@ -633,6 +633,7 @@ struct DistillArgs {
   long long ld_t;
   float *row_loss, *row_stats, *q;
   int V;
+  double inv_temp;
   Scaling sc;
 };
 
@@ -778,7 +779,6 @@ __global__ void __launch_bounds__(TP_THREADS, 6)
   }
 
   // ---- the teacher and the row
-  const double ln2 = 0.69314718055994530942;
   if (!in) t = -INFINITY;
   y = in ? p.sc.capped(y) : -INFINITY;
   Stats st = empty_stats();
@@ -798,7 +798,6 @@ __global__ void __launch_bounds__(TP_THREADS, 6)
   double q = in ? exp((double)t - t_shift) : 0.0;
   const double sum = block_sum(q, red_d);
   const bool others = !no_class(a);
-  const float log_s = log2f(all.s), rest_log_s = log2f(a.s);
   double mass = sum, rest = 0.0, log_norm = t_shift;
   if (p.renormalize) {
     log_norm += log(sum);
@@ -807,16 +806,20 @@ __global__ void __launch_bounds__(TP_THREADS, 6)
   } else if (others) {
     rest = fmax(0.0, 1.0 - sum);
   }
-  const double lp = y == -INFINITY ? -INFINITY : (((double)y - all.m) * p.sc.c - log_s) * ln2;
-  double loss = block_sum(in && q != 0.0 ? q * ((double)t - log_norm - lp) : 0.0, red_d);
+  // sum q (log q - log p), but for log p's common part; in 64 bits, the temperature too, for a loss that is a small difference of logarithms
+  const bool none = no_class(all);
+  const double log_p0 = y == -INFINITY ? -INFINITY : ((double)y - all.m) * p.inv_temp;
+  double loss = block_sum(in && q != 0.0 ? q * ((double)t - log_norm - log_p0) : 0.0, red_d);
   if ((int)threadIdx.x < p.k) p.q[row * p.k + threadIdx.x] = in && any ? (float)q : -1.f;
   if (threadIdx.x == 0) {
-    const double total = mass + rest, rest_lp = (((double)a.m - all.m) * p.sc.c + rest_log_s - log_s) * ln2;
+    const double log_s = none ? 0.0 : log((double)all.s), rest_log_s = others ? log((double)a.s) : 0.0;
+    const double total = mass + rest, rest_lp = ((double)a.m - all.m) * p.inv_temp + rest_log_s - log_s;
+    loss += mass * log_s;
     if (rest > 0.0) loss += rest * (log(rest) - rest_lp);
     p.row_loss[row] = any ? (float)loss : 0.f;
     float4* o = reinterpret_cast<float4*>(p.row_stats + row * 8);
     o[0] = make_float4(any ? (float)total : -1.f, others && any ? (float)(total * exp(rest_lp) - rest) : 0.f, 0.f, 0.f);
-    o[1] = make_float4(all.m, log_s, a.m, rest_log_s);
+    o[1] = make_float4(all.m, log2f(all.s), a.m, log2f(a.s));
   }
 }
 static_assert(OB_TOP_K_MAX <= TP_THREADS, "one thread per class of the teacher");
@@ -1012,7 +1015,7 @@ using namespace ob;
 
 extern "C" int ob_token_log_probs_fwd(const void* logits, int dtype, long long ld, const long long* ids, float* log_probs,
                                       float* entropy, float* norm, int top_k, float* top_log_probs, long long* top_ids,
-                                      long long rows, int V, int ignore_index, float softcap, float inv_temp,
+                                      long long rows, int V, int ignore_index, float softcap, double inv_temp,
                                       cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (int rc = check_logits("token_log_probs", logits, dtype, ld, rows, V)) return rc;
@@ -1032,7 +1035,7 @@ extern "C" int ob_token_log_probs_fwd(const void* logits, int dtype, long long l
 }
 
 extern "C" int ob_join_scores(const float* parts, const float* target, long long stride, int n, const long long* ids, float* log_probs,
-                              float* entropy, float* norm, long long rows, int V, int ignore_index, float softcap, float inv_temp,
+                              float* entropy, float* norm, long long rows, int V, int ignore_index, float softcap, double inv_temp,
                               cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (parts == nullptr || entropy == nullptr || (log_probs != nullptr && (ids == nullptr || target == nullptr)))
@@ -1047,7 +1050,7 @@ extern "C" int ob_join_scores(const float* parts, const float* target, long long
 extern "C" int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const long long* ids, const float* norm,
                                       const float* entropy, const float* g_log_probs, long long stride_lp,
                                       const float* g_entropy, long long stride_ent, void* dlogits, int dtype_d, long long ld_d,
-                                      long long rows, int V, int ignore_index, float softcap, float inv_temp,
+                                      long long rows, int V, int ignore_index, float softcap, double inv_temp,
                                       cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (int rc = check_logits("token_log_probs backward", logits, dtype, ld, rows, V)) return rc;
@@ -1067,14 +1070,14 @@ extern "C" int ob_token_log_probs_bwd(const void* logits, int dtype, long long l
 
 extern "C" int ob_distill_fwd(const void* logits, int dtype, long long ld, const void* teacher_ids, int ids_64,
                               const float* teacher_log_probs, long long ld_t, int k, int renormalize, float* row_loss,
-                              float* row_stats, float* q, long long rows, int V, float softcap, float inv_temp,
+                              float* row_stats, float* q, long long rows, int V, float softcap, double inv_temp,
                               cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (int rc = check_logits("distillation", logits, dtype, ld, rows, V)) return rc;
   if (k < 1 || k > OB_TOP_K_MAX) OB_FAIL(-4, "distillation: %d teacher classes outside [1, %d]", k, OB_TOP_K_MAX);
   if (teacher_ids == nullptr || teacher_log_probs == nullptr || row_loss == nullptr || row_stats == nullptr || q == nullptr)
     OB_FAIL(-5, "distillation: missing tensor");
-  const DistillArgs args{teacher_ids, teacher_log_probs, ids_64, k, renormalize, ld_t, row_loss, row_stats, q, V, scaling(softcap, inv_temp)};
+  const DistillArgs args{teacher_ids, teacher_log_probs, ids_64, k, renormalize, ld_t, row_loss, row_stats, q, V, inv_temp, scaling(softcap, inv_temp)};
   if (dtype == OB_F32)
     return softcap > 0.f ? launch_distill<float, 4, true>((const float*)logits, ld, rows, args, stream)
                          : launch_distill<float, 4, false>((const float*)logits, ld, rows, args, stream);
@@ -1085,7 +1088,7 @@ extern "C" int ob_distill_fwd(const void* logits, int dtype, long long ld, const
 extern "C" int ob_distill_bwd(const void* logits, int dtype, long long ld, const void* teacher_ids, int ids_64, long long ld_t,
                               int k, const float* row_stats, const float* q, const float* g, long long stride_g,
                               const float* inv_count, float scale, void* dlogits, int dtype_d, long long ld_d, long long rows,
-                              int V, float softcap, float inv_temp, cudaStream_t stream) {
+                              int V, float softcap, double inv_temp, cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (int rc = check_logits("distillation backward", logits, dtype, ld, rows, V)) return rc;
   if (k < 1 || k > OB_TOP_K_MAX) OB_FAIL(-4, "distillation backward: %d teacher classes outside [1, %d]", k, OB_TOP_K_MAX);

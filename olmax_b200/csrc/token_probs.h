@@ -20,18 +20,18 @@ extern "C" {
 // in order, equal logits by their class (top_k <= min(V, OB_TOP_K_MAX)).
 int ob_token_log_probs_fwd(const void* logits, int dtype, long long ld, const long long* ids, float* log_probs, float* entropy,
                            float* norm, int top_k, float* top_log_probs, long long* top_ids, long long rows, int V,
-                           int ignore_index, float softcap, float inv_temp, cudaStream_t stream);
+                           int ignore_index, float softcap, double inv_temp, cudaStream_t stream);
 // The same of logits that exist as statistics of `n` groups of classes only: parts[i * stride + r] = four floats (largest capped logit m, sum 2^t, sum
 // 2^t t, unused) with t = (cap(z) - m) log2(e) inv_temp over group i, target[r] = the logit of class ids[r] (undefined where it is not scored).
 int ob_join_scores(const float* parts, const float* target, long long stride, int n, const long long* ids, float* log_probs,
-                   float* entropy, float* norm, long long rows, int V, int ignore_index, float softcap, float inv_temp,
+                   float* entropy, float* norm, long long rows, int V, int ignore_index, float softcap, double inv_temp,
                    cudaStream_t stream);
 // dlogits (of dtype_d, row stride ld_d) = g_log_probs[r * stride_lp] * d log_probs[r] + g_entropy[r * stride_ent] * d entropy[r]
 // over d logits; either upstream gradient may be null.
 int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const long long* ids, const float* norm,
                            const float* entropy, const float* g_log_probs, long long stride_lp, const float* g_entropy,
                            long long stride_ent, void* dlogits, int dtype_d, long long ld_d, long long rows, int V,
-                           int ignore_index, float softcap, float inv_temp, cudaStream_t stream);
+                           int ignore_index, float softcap, double inv_temp, cudaStream_t stream);
 
 // Teacher of a row: k <= OB_TOP_K_MAX pairs (teacher_ids, int32 or int64 by ids_64; teacher_log_probs fp32), rows ld_t apart.  A pair whose id
 // lies outside [0, V) is padding; of several pairs with one id the first counts.
@@ -43,11 +43,11 @@ int ob_token_log_probs_bwd(const void* logits, int dtype, long long ld, const lo
 // of the other classes; q [rows, k] = the teacher's masses, -1 for pairs that do not count.
 int ob_distill_fwd(const void* logits, int dtype, long long ld, const void* teacher_ids, int ids_64,
                    const float* teacher_log_probs, long long ld_t, int k, int renormalize, float* row_loss, float* row_stats,
-                   float* q, long long rows, int V, float softcap, float inv_temp, cudaStream_t stream);
+                   float* q, long long rows, int V, float softcap, double inv_temp, cudaStream_t stream);
 // dlogits = scale * (*inv_count, if given) * g[r * stride_g] * d row_loss[r] / d logits
 int ob_distill_bwd(const void* logits, int dtype, long long ld, const void* teacher_ids, int ids_64, long long ld_t, int k,
                    const float* row_stats, const float* q, const float* g, long long stride_g, const float* inv_count, float scale,
-                   void* dlogits, int dtype_d, long long ld_d, long long rows, int V, float softcap, float inv_temp,
+                   void* dlogits, int dtype_d, long long ld_d, long long rows, int V, float softcap, double inv_temp,
                    cudaStream_t stream);
 // *loss = sum of row_loss, divided by the number of rows with a teacher if mean; *inv_count (may be null) = 1 / max(1, that number)
 int ob_distill_reduce(const float* row_loss, const float* row_stats, long long rows, int mean, float* loss, float* inv_count,

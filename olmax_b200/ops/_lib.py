@@ -90,7 +90,7 @@ class ObScoreArgs(ctypes.Structure):
         ("rows", ctypes.c_longlong),
         ("ignore_index", ctypes.c_int),
         ("softcap", ctypes.c_float),
-        ("inv_temp", ctypes.c_float),
+        ("inv_temp", ctypes.c_double),
     ]
 
 

@@ -1294,10 +1294,11 @@ def _teacher_rows(teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, sh
     k = teacher_ids.shape[-1]
     if not 1 <= k <= K.TOP_K_MAX:
         raise ValueError(f"a teacher names between 1 and {K.TOP_K_MAX} classes, got {k}")
-    rows = math.prod(shape)
-    values = teacher_log_probs.detach()
+    values = teacher_log_probs.detach() if teacher_log_probs.requires_grad else teacher_log_probs
     values = values if values.dtype == torch.float64 and not values.is_cuda else values.float()
-    return teacher_ids.reshape(rows, k).contiguous(), values.reshape(rows, k).contiguous()
+    if teacher_ids.dim() != 2:
+        teacher_ids, values = teacher_ids.reshape(math.prod(shape), k), values.reshape(math.prod(shape), k)
+    return teacher_ids.contiguous(), values.contiguous()
 
 
 class _DistillationFn(torch.autograd.Function):
@@ -1427,8 +1428,9 @@ class _HeadChunks:
         return dlogits[at : at + r1 - r0]
 
 
-# Rows of one GEMM that gives scores: its scratch holds 16 bytes per row and 256 classes
-_SCORE_ROWS = 16384
+def _score_rows(N: int) -> int:
+    """Rows of one GEMM that gives scores: its scratch, 16 bytes per row and 256 classes, stays near 64 MB."""
+    return max(1024, min(16384, (1 << 22) // max(1, N // 256) // 256 * 256))
 
 
 def _gemm_scores(x2: torch.Tensor, handle, ids, log_probs, entropy, norm, **options) -> None:
@@ -1436,8 +1438,9 @@ def _gemm_scores(x2: torch.Tensor, handle, ids, log_probs, entropy, norm, **opti
     M, Kd = x2.shape
     N = handle.tp_shape[0]
     _check_width(x2, handle)
-    for r0 in range(0, M, _SCORE_ROWS):
-        r1 = min(M, r0 + _SCORE_ROWS)
+    step = _score_rows(N)
+    for r0 in range(0, M, step):
+        r1 = min(M, r0 + step)
         xc = _whole_rows(x2[r0:r1])
         first, kw = _b_operand(handle)
         kw.update(_ag_kwargs(handle))

@@ -58,6 +58,7 @@ _vp = ctypes.c_void_p
 _ll = ctypes.c_longlong
 _i = ctypes.c_int
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 register_signature("ob_rmsnorm_fwd", [_vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _ll, _ll, _ll, _i, _f, _vp])
 register_signature("ob_rmsnorm_bwd", [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _ll, _ll, _ll, _f, _vp])
@@ -79,10 +80,10 @@ register_signature("ob_adamw", [_vp, _vp, _vp, _vp, _vp, _ll, _f, _f, _f, _f, _f
 register_signature("ob_sumsq", [_vp, _ll, _vp, _vp])
 register_signature("ob_clip_coef", [_vp, _f, _f, _vp, _vp])
 register_signature("ob_cast_f32_bf16", [_vp, _vp, _ll, _vp])
-register_signature("ob_token_log_probs_fwd", [_vp, _i, _ll, _vp, _vp, _vp, _vp, _i, _vp, _vp, _ll, _i, _i, _f, _f, _vp])
-register_signature("ob_token_log_probs_bwd", [_vp, _i, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _i, _ll, _ll, _i, _i, _f, _f, _vp])
-register_signature("ob_distill_fwd", [_vp, _i, _ll, _vp, _i, _vp, _ll, _i, _i, _vp, _vp, _vp, _ll, _i, _f, _f, _vp])
-register_signature("ob_distill_bwd", [_vp, _i, _ll, _vp, _i, _ll, _i, _vp, _vp, _vp, _ll, _vp, _f, _vp, _i, _ll, _ll, _i, _f, _f, _vp])
+register_signature("ob_token_log_probs_fwd", [_vp, _i, _ll, _vp, _vp, _vp, _vp, _i, _vp, _vp, _ll, _i, _i, _f, _d, _vp])
+register_signature("ob_token_log_probs_bwd", [_vp, _i, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _i, _ll, _ll, _i, _i, _f, _d, _vp])
+register_signature("ob_distill_fwd", [_vp, _i, _ll, _vp, _i, _vp, _ll, _i, _i, _vp, _vp, _vp, _ll, _i, _f, _d, _vp])
+register_signature("ob_distill_bwd", [_vp, _i, _ll, _vp, _i, _ll, _i, _vp, _vp, _vp, _ll, _vp, _f, _vp, _i, _ll, _ll, _i, _f, _d, _vp])
 register_signature("ob_distill_reduce", [_vp, _vp, _ll, _i, _vp, _vp, _vp])
 register_signature("ob_distill_count", [_vp, _i, _vp, _ll, _i, _i, _ll, _i, _vp, _vp])
 register_signature("ob_peer_barrier", [_vp, _i, _i, ctypes.c_uint, _ll, _vp, _vp])
