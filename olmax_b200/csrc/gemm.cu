@@ -125,6 +125,10 @@ struct KernelParams {
   Scaling score_sc;
 };
 
+// SCORE of gemm_body.
+enum { NO_SCORES = 0, SCORES_BY_ROW = 1, SCORES_BY_COLUMN = 2 };
+constexpr int FEW_TOKENS = 16;   // columns of SCORES_BY_COLUMN
+
 // Statistics of 32 logits of a row from a tile's columns [col, col + 32), of which the first n are there.
 template <bool CAP>
 __device__ __forceinline__ void score_columns(Stats& a, float (&f)[32], int n, const Scaling& sc) {
@@ -247,9 +251,12 @@ __device__ __forceinline__ const CUtensorMap* pick_segment(const CUtensorMap* s0
 // issue that comes later after its stage is freed is a load that arrives later.  With the choice of the map in that loop of
 // every kernel, GEMMs without segments took 2-3 % longer (65536 x 3072 x 1024 297 us, now 287; 8192 x 12288 x 4096 541, now
 // 528) and contractions over segments 6 % (8192 x 4096 x 22016 1030, now 969; 966 of one tensor); one branch per map took 10 %.
-// SCORE: in place of C the epilogue gives the statistics of its columns' softmax (token_stats.cuh): 256 exponentials a row and tile, of which the
-// special-function unit does 16 a clock, run under the next tile's main loop, and the logits never leave the SM.
-template <bool A_MN, bool B_MN, int CG, int BN, bool SEG, bool SCORE = false>
+// SCORES_BY_ROW: in place of C the epilogue gives the statistics of its columns' softmax (token_stats.cuh): 256 exponentials a row and tile, of which
+// the special-function unit does 16 a clock, run under the next tile's main loop, and the logits never leave the SM.
+// SCORES_BY_COLUMN: the operands change places for a few tokens, whose product is bound by reading the weights: classes are rows, 128 of them to a
+// tile whatever the number of tokens, so that the tensor cores multiply 64 columns instead of 256 rows of mostly nothing.  Every thread keeps the
+// statistics of FEW_TOKENS columns over its classes of all tiles of the CTA, and the CTA leaves one part per token at the end.
+template <bool A_MN, bool B_MN, int CG, int BN, bool SEG, int SCORE = NO_SCORES>
 __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
                                           const CUtensorMap& tmC, const CUtensorMap& tmS1, const CUtensorMap& tmS2,
                                           const KernelParams& p) {
@@ -565,6 +572,11 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     // have an odd number of them), which is what lets one store still be reading its buffer while the next is filled
     uint32_t chunk = 0;
     bool ok = true;
+    Stats column[SCORE == SCORES_BY_COLUMN ? FEW_TOKENS : 1];
+    if constexpr (SCORE == SCORES_BY_COLUMN) {
+#pragma unroll
+      for (int j = 0; j < FEW_TOKENS; ++j) column[j] = empty_stats();
+    }
     for (int w = worker; w < p.total_items && ok; w += n_workers, ++it) {
       const int buf = it & 1;
       const uint32_t tphase = (uint32_t)(it >> 1) & 1u;
@@ -596,7 +608,21 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         cbase = reinterpret_cast<uint8_t*>(p.c);
         row_off = (long long)(m_shard * p.M_s + m_local0 + row_in_tile) * p.ldc + n_glob0;
       }
-      if constexpr (SCORE) {
+      if constexpr (SCORE == SCORES_BY_COLUMN) {
+        static_assert(FEW_TOKENS == 16, "one load of TMEM");
+        const int cls = m_local0 + row_in_tile;
+        uint32_t x[16];
+        tmem_ld16(t_row, x);
+        tmem_ld_wait();
+        if (row_ok) {
+#pragma unroll
+          for (int j = 0; j < FEW_TOKENS; ++j) {
+            const float z = __uint_as_float(x[j]);
+            add_class(column[j], p.score_sc.capped(z), p.score_sc);
+            if (p.score_ids != nullptr && j < p.score_rows && p.score_ids[j] == cls) p.score_target[j] = z;
+          }
+        }
+      } else if constexpr (SCORE == SCORES_BY_ROW) {
         const int row = m_local0 + row_in_tile;   // (one M shard)
         const bool scored = row < p.score_rows;
         long long want = -1;   // the token's column in this tile
@@ -913,6 +939,22 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         else mbar_arrive(&tempty_bar[buf]);
       }
     }
+    if constexpr (SCORE == SCORES_BY_COLUMN) {
+      // (the output staging is free: there is no output)
+      Stats* warps = reinterpret_cast<Stats*>(epi_smem);   // [4][FEW_TOKENS]
+#pragma unroll
+      for (int j = 0; j < FEW_TOKENS; ++j) {
+        const Stats s = shuffle_combine(column[j], 16, p.score_sc.c);
+        if (lane == 0) warps[q * FEW_TOKENS + j] = s;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const int j = (int)threadIdx.x - 64;
+      if (j < FEW_TOKENS && j < p.score_rows) {
+        Stats s = warps[j];
+        for (int i = 1; i < 4; ++i) s = combine(s, warps[i * FEW_TOKENS + j], p.score_sc.c);
+        p.score_parts[worker * FEW_TOKENS + j] = make_float4(s.m, s.s, s.w, 0.f);
+      }
+    }
   }
 
   // teardown: everyone meets here (also after an aborted wait; with CG = 2 both CTAs, so that neither leaves while
@@ -946,14 +988,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
 }
 
 // The scores of tokens: K-major operands, no output.
-template <int BN>
+template <int BN, int SCORE>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
     gemm_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const KernelParams p) {
-  gemm_body<false, false, 1, BN, false, true>(tmA, tmB, tmB, tmB, tmB, tmB, p);
+  gemm_body<false, false, 1, BN, false, SCORE>(tmA, tmB, tmB, tmB, tmB, tmB, p);
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
     gemm_scores_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const KernelParams p) {
-  gemm_body<false, false, 2, BN_WIDE, false, true>(tmA, tmB, tmB, tmB, tmB, tmB, p);
+  gemm_body<false, false, 2, BN_WIDE, false, SCORES_BY_ROW>(tmA, tmB, tmB, tmB, tmB, tmB, p);
 }
 
 constexpr int MAX_DEVICES = 64;
@@ -989,7 +1031,7 @@ static int launch(const Maps& m, const KernelParams& kp, int grid, cudaStream_t 
   return 0;
 }
 
-template <int CG, int BN>
+template <int CG, int BN, int SCORE>
 static int launch_scores_gemm(const Maps& m, const KernelParams& kp, int grid, cudaStream_t stream) {
   static bool attr_set[MAX_DEVICES] = {};
   int dev = 0;
@@ -998,7 +1040,7 @@ static int launch_scores_gemm(const Maps& m, const KernelParams& kp, int grid, c
   constexpr int smem = Geo<CG, BN>::SMEM_BYTES;
   auto kernel = [] {
     if constexpr (CG == 2) return gemm_scores_pair_kernel;
-    else return gemm_scores_kernel<BN>;
+    else return gemm_scores_kernel<BN, SCORE>;
   }();
   if (!attr_set[dev]) {
     OB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -1059,8 +1101,9 @@ static bool split_k_enabled() {
 // Column tiles of at most this many columns in more than one wave (narrower ones come in one wave, at most one tile per SM).
 static long long score_tiles(int N, int N_s) { return (long long)(N / N_s) * ((N_s + BN_WIDE - 1) / BN_WIDE); }
 
-// ob_gemm_bf16; with `scores` the kernels that give them, and in *n_tiles their column tiles.
-static int run_gemm(const ObGemmArgs* a, const ObScoreArgs* scores, int* n_tiles, cudaStream_t stream) {
+// ob_gemm_bf16; with `scores` the kernels that give them, and in *n_parts the parts (column tiles) that they leave, M rows apart.
+// `few`: A are the weights and B the tokens; *n_parts are then the CTAs, FEW_TOKENS apart.
+static int run_gemm(const ObGemmArgs* a, const ObScoreArgs* scores, bool few, int* n_parts, cudaStream_t stream) {
   if (a == nullptr) OB_FAIL(-1, "null args");
   if (a->M <= 0 || a->N <= 0 || a->Kc <= 0) OB_FAIL(-2, "empty problem M=%d N=%d K=%d", a->M, a->N, a->Kc);
   const bool glu = (a->epi == EPI_SWIGLU || a->epi == EPI_GEGLU);
@@ -1111,6 +1154,7 @@ static int run_gemm(const ObGemmArgs* a, const ObScoreArgs* scores, int* n_tiles
       BN = BN_NARROW;
     }
   }
+  if (few) CG = 1, BN = BN_NARROW;
   if (cap < 2) CG = 1;
   kp.bn_out = glu ? BN / 2 : BN;
   const int BMT = BM * CG;            // tile rows
@@ -1334,16 +1378,18 @@ static int run_gemm(const ObGemmArgs* a, const ObScoreArgs* scores, int* n_tiles
   if (a->c_shards != nullptr && a->epi == EPI_BF16_ACC && kp.tma_epi != 2)
     OB_FAIL(-18, "EPI_BF16_ACC towards c_shards needs the staged epilogue (16-byte aligned rows, local partial in c)");
   if (scores != nullptr) {
-    *n_tiles = kp.n_shards * kp.n_tiles_per_shard;
-    if (4ll * a->M * *n_tiles > scores->parts_size) OB_FAIL(-21, "scores: scratch of %lld floats for %d x %d tiles", scores->parts_size, a->M, *n_tiles);
+    *n_parts = few ? workers : kp.n_shards * kp.n_tiles_per_shard;
+    const int rows = few ? FEW_TOKENS : a->M;
+    if (4ll * rows * *n_parts > scores->parts_size) OB_FAIL(-21, "scores: scratch of %lld floats for %d parts of %d rows", scores->parts_size, *n_parts, rows);
     kp.score_ids = scores->ids;
     kp.score_parts = reinterpret_cast<float4*>(scores->parts);
     kp.score_target = scores->target;
     kp.score_rows = (int)scores->rows;
     kp.score_sc = scaling(scores->softcap, scores->inv_temp);
-    if (CG == 2) return launch_scores_gemm<2, BN_WIDE>(maps, kp, grid, stream);
-    if (BN == BN_NARROW) return launch_scores_gemm<1, BN_NARROW>(maps, kp, grid, stream);
-    return launch_scores_gemm<1, BN_WIDE>(maps, kp, grid, stream);
+    if (few) return launch_scores_gemm<1, BN_NARROW, SCORES_BY_COLUMN>(maps, kp, grid, stream);
+    if (CG == 2) return launch_scores_gemm<2, BN_WIDE, SCORES_BY_ROW>(maps, kp, grid, stream);
+    if (BN == BN_NARROW) return launch_scores_gemm<1, BN_NARROW, SCORES_BY_ROW>(maps, kp, grid, stream);
+    return launch_scores_gemm<1, BN_WIDE, SCORES_BY_ROW>(maps, kp, grid, stream);
   }
   if (CG == 2) return launch_tiles<2, BN_WIDE>(a->a_mn != 0, a->b_mn != 0, maps, kp, grid, stream);
   if (BN == BN_NARROW) return launch_tiles<1, BN_NARROW>(a->a_mn != 0, a->b_mn != 0, maps, kp, grid, stream);
@@ -1354,12 +1400,13 @@ static int run_gemm(const ObGemmArgs* a, const ObScoreArgs* scores, int* n_tiles
 
 using namespace ob;
 
-extern "C" int ob_gemm_bf16(const ObGemmArgs* args, cudaStream_t stream) { return run_gemm(args, nullptr, nullptr, stream); }
+extern "C" int ob_gemm_bf16(const ObGemmArgs* args, cudaStream_t stream) { return run_gemm(args, nullptr, false, nullptr, stream); }
 
 extern "C" long long ob_gemm_scores_parts(int M, int N, int N_s) {
   if (M <= 0 || N <= 0 || N_s <= 0 || N % N_s) return 0;
   const long long wide = score_tiles(N, N_s), one_wave = sm_count();
-  return 4ll * M * (wide > one_wave ? wide : one_wave);
+  const long long parts = wide > one_wave ? wide : one_wave;   // (of few tokens: a part per CTA)
+  return 4ll * (M > FEW_TOKENS ? M : FEW_TOKENS) * parts;
 }
 
 extern "C" int ob_gemm_scores(const ObGemmArgs* a, const ObScoreArgs* s, cudaStream_t stream) {
@@ -1369,9 +1416,19 @@ extern "C" int ob_gemm_scores(const ObGemmArgs* a, const ObScoreArgs* s, cudaStr
   if (s->rows < 0 || s->rows > a->M || s->parts == nullptr || s->entropy == nullptr || (reinterpret_cast<uintptr_t>(s->parts) & 15) != 0 ||
       (s->log_probs != nullptr && (s->ids == nullptr || s->target == nullptr)) || (s->ids != nullptr && s->target == nullptr))
     OB_FAIL(-5, "scores: missing tensor");
-  int n_tiles = 0;
-  if (int rc = run_gemm(a, s, &n_tiles, stream)) return rc;
-  return ob_join_scores(s->parts, s->target, a->M, n_tiles, s->ids, s->log_probs, s->entropy, s->norm, s->rows, a->N, s->ignore_index,
+  // Few tokens and unsharded weights, which are read at 5.4-5.6 TB/s with the operands exchanged: 8 x 100352 x 4096 150 us (195 with tokens as rows),
+  // 8 x 256000 x 4608 441 (604), 8 x 50304 x 1024 35 (41).
+  const bool few = s->rows <= FEW_TOKENS && a->M <= FEW_TOKENS && (a->N_s <= 0 || a->N_s == a->N) && a->ag_src == nullptr;
+  ObGemmArgs turned = *a;
+  if (few) {
+    turned.a = a->b; turned.lda = a->ldb; turned.M = a->N;
+    turned.b = a->a; turned.ldb = a->lda; turned.N = a->M;
+    turned.M_s = turned.N_s = 0;
+    turned.b_shard_stride = 0;
+  }
+  int n_parts = 0;
+  if (int rc = run_gemm(few ? &turned : a, s, few, &n_parts, stream)) return rc;
+  return ob_join_scores(s->parts, s->target, few ? FEW_TOKENS : a->M, n_parts, s->ids, s->log_probs, s->entropy, s->norm, s->rows, a->N, s->ignore_index,
                         s->softcap, s->inv_temp, stream);
 }
 

@@ -27,12 +27,6 @@ __device__ __forceinline__ float from_f<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16(x); }
 
-__device__ __forceinline__ Stats shuffle_combine(Stats a, int first, float c) {
-  for (int off = first; off > 0; off >>= 1)
-    a = combine(a, Stats{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.s, off),
-                         __shfl_xor_sync(0xffffffffu, a.w, off)}, c);
-  return a;
-}
 __device__ __forceinline__ Stats block_combine(Stats a, Stats* red, float c) {
   a = shuffle_combine(a, 16, c);
   __syncthreads();

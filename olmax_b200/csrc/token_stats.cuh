@@ -145,6 +145,12 @@ __device__ __forceinline__ void add_class(Stats& a, float y, const Scaling& sc) 
   add_classes<false, true, 1>(a, f, y, sc);
 }
 
+__device__ __forceinline__ Stats shuffle_combine(Stats a, int first, float c) {
+  for (int off = first; off > 0; off >>= 1)
+    a = combine(a, Stats{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.s, off),
+                         __shfl_xor_sync(0xffffffffu, a.w, off)}, c);
+  return a;
+}
 static inline Scaling scaling(float softcap, double inv_temp) {
   const double k = softcap > 0.f ? 2.0 * 1.4426950408889634 / (double)softcap : 0.0;
   return Scaling{softcap, (float)k, (float)(1.4426950408889634 * inv_temp), (float)inv_temp};

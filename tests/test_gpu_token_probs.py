@@ -538,3 +538,32 @@ def test_head_scores_of_weight_shards():
         K.gemm_scores(a, b, ids, out[0][0], out[0][1], None, M, N, Kd, rows=M + 1)
     with pytest.raises(K.KernelError):
         K.gemm_scores(a, b, ids, out[0][0], out[0][1], None, M, N, Kd - 4, rows=rows)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 8, 9, 16, 17])
+@pytest.mark.parametrize("V,d,cap", [(128, 64, None), (1000, 1024, 30.0), (20008, 520, None), (50304, 256, None)])
+def test_head_scores_of_few_tokens(rows, V, d, cap):
+    """Up to 16 tokens the product is formed with its operands exchanged."""
+    head = _bf16_head(V, d, cap)
+    w = head.weight.full()
+    x = torch.randn(rows, d, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(torch.bfloat16)
+    ids = torch.randint(0, V, (rows,), generator=torch.Generator(device=DEV).manual_seed(4), device=DEV)
+    ids[0] = V - 1
+    if rows > 4:
+        ids[1], ids[2], ids[3], ids[4] = -100, V, 0, ids[0]
+    z = x.double() @ w.double().t()
+    gemm = d * 2.0 ** -24 * float((x.double().abs() @ w.double().abs().t()).max())
+    lp, ent, _, _ = scores_64(z, ids, 1, 1.0, cap or 0.0)
+    e = _eps(V, min(float(z.abs().max()), cap or math.inf), cap or 0.0) + 2 * gemm
+    with torch.no_grad():
+        out = head.token_log_probs(x, ids)
+        again = head.token_log_probs(x, ids)
+    _close(out.log_probs, lp, 2 * e)
+    _close(out.entropy, ent, (2 + ent) * e)
+    assert torch.equal(out.log_probs, again.log_probs) and torch.equal(out.entropy, again.entropy)
+    leaf = x.clone().requires_grad_(True)                          # and the gradient, from the logits computed again
+    got = head.token_log_probs(leaf, ids)
+    gx, = torch.autograd.grad(got.log_probs.sum(), leaf)
+    dz, _ = score_gradients_64(z, ids, torch.ones(rows, device=DEV), torch.zeros(rows, device=DEV), 1.0, cap or 0.0)
+    want, size = dz @ w.double(), dz.abs() @ w.double().abs()
+    _close(gx, want, (2.0 ** -8 + 2.0 ** -12 + 4 * e) * size + 2.0 ** -8 * want.abs() + 1e-12)
