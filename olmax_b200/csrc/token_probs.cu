@@ -248,6 +248,17 @@ __device__ int collect_classes(TopWork& w, const Row<T>& r, int v0, int v1, int 
   return w.classes;
 }
 
+// log p of a class with capped logit y, and the entropy.  Neither passes 0 by the roundings of a soft-capped maximum; a NaN stays.
+__device__ __forceinline__ float log_prob(float y, float m, float log_s, const Scaling& sc) {
+  if (y == -INFINITY) return log_s == log_s ? y : log_s;
+  const float lp = LN2 * ((y - m) * sc.c - log_s);
+  return lp > 0.f ? 0.f : lp;
+}
+__device__ __forceinline__ float entropy_of(Stats a, float log_s) {
+  const float h = LN2 * (log_s - a.w / a.s);
+  return no_class(a) || h < 0.f ? 0.f : h;
+}
+
 struct ScoreArgs {
   const long long* ids;
   float *log_probs, *entropy, *norm;
@@ -398,13 +409,10 @@ __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 4 : sizeof(T) == 2 ? 
     __syncthreads();
   }
   const float log_s = log2f(a.s);
-  auto log_p = [&](float z) {
-    const float y = CAP ? p.sc.capped(z) : z;
-    return y == -INFINITY ? (log_s == log_s ? y : log_s) : LN2 * ((y - a.m) * p.sc.c - log_s);
-  };
+  auto log_p = [&](float z) { return log_prob(CAP ? p.sc.capped(z) : z, a.m, log_s, p.sc); };
   if (threadIdx.x == 0) {
     if (p.log_probs != nullptr) p.log_probs[row] = known ? log_p(taken) : 0.f;
-    if (p.entropy != nullptr) p.entropy[row] = no_class(a) ? 0.f : LN2 * (log_s - a.w / a.s);
+    if (p.entropy != nullptr) p.entropy[row] = entropy_of(a, log_s);
     if (p.norm != nullptr) *reinterpret_cast<float2*>(p.norm + row * 2) = make_float2(a.m, log_s);
   }
   if (TOP) {
@@ -461,12 +469,11 @@ __global__ void __launch_bounds__(1024)
     const long long id = p.ids[row];
     float lp = 0.f;
     if (id != (long long)p.ignore_index && id >= 0 && id < p.V) {
-      const float y = p.sc.capped(target[row]);
-      lp = y == -INFINITY ? (log_s == log_s ? y : log_s) : LN2 * ((y - a.m) * p.sc.c - log_s);
+      lp = log_prob(p.sc.capped(target[row]), a.m, log_s, p.sc);
     }
     p.log_probs[row] = lp;
   }
-  p.entropy[row] = no_class(a) ? 0.f : LN2 * (log_s - a.w / a.s);
+  p.entropy[row] = entropy_of(a, log_s);
   if (p.norm != nullptr) *reinterpret_cast<float2*>(p.norm + row * 2) = make_float2(a.m, log_s);
 }
 
@@ -974,13 +981,19 @@ template <class T, int U, bool CAP>
 static int launch_distill(const T* logits, long long ld, long long rows, const DistillArgs& args, cudaStream_t stream) {
   constexpr int N = Row<T>::N, LIMIT = 160 * 1024;
   auto kernel = distill_fwd_kernel<T, U, CAP>;
-  const int C = ctas_per_row(rows, args.V, TP_THREADS * U * N), vectors = args.V / N / C + 1;
-  // a bit for each vector of whole batches and a bit for each class, with the row's head and tail
-  const int bytes = (vectors + TP_THREADS * U - 1) / (TP_THREADS * U) * (TP_THREADS * U / 8) + (vectors * N + 4 * N + 31) / 32 * 4;
-  if (bytes > LIMIT) OB_FAIL(-6, "distillation: no room in shared memory for the bits of %d classes", args.V);
+  // a bit for each vector of whole batches and a bit for each class, with the row's head and tail; more CTAs where they do not fit
+  int C = ctas_per_row(rows, args.V, TP_THREADS * U * N), vectors;
+  long long bytes;
+  for (;; C *= 2) {
+    vectors = args.V / N / C + 1;
+    bytes = (vectors + TP_THREADS * U - 1) / (TP_THREADS * U) * (TP_THREADS * U / 8) + ((long long)vectors * N + 4 * N + 31) / 32 * 4;
+    if (bytes <= LIMIT) break;
+    if (C == 8) OB_FAIL(-6, "distillation: no room in shared memory for the bits of %d classes", args.V);
+  }
+  if (rows > INT_MAX / C) OB_FAIL(-3, "distillation: %lld rows of %d classes", rows, args.V);
   static bool done[64] = {};
   if (int rc = allow_shared(kernel, LIMIT, done)) return rc;
-  return launch_clusters(kernel, rows * C, C, bytes, stream, logits, ld, C, vectors, args);
+  return launch_clusters(kernel, rows * C, C, (int)bytes, stream, logits, ld, C, vectors, args);
 }
 
 // Calls launch(z, d, parts, per_block) with the types of the logits and of their gradient and the spans of a row.

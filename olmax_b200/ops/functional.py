@@ -1145,7 +1145,7 @@ class TokenLogProbs(NamedTuple):
     """Their classes (int64); equal logits in the order of their classes."""
 
 
-def _distribution_options(V: int, temperature: float, logit_softcap: Optional[float], top_k: int = 0) -> float:
+def _distribution_options(V: int, temperature: float, logit_softcap: Optional[float], top_k: int = 0, ignore_index: int = -100) -> float:
     if not (0.0 < temperature < math.inf):
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     cap = float(logit_softcap or 0.0)
@@ -1153,6 +1153,8 @@ def _distribution_options(V: int, temperature: float, logit_softcap: Optional[fl
         raise ValueError(f"logit_softcap must be positive and finite (or None), got {logit_softcap}")
     if V < 1:
         raise ValueError("logits need at least one class")
+    if not -(2 ** 31) <= ignore_index < 2 ** 31:
+        raise ValueError(f"ignore_index must fit 32 bits, got {ignore_index}")
     if not 0 <= top_k <= min(V, K.TOP_K_MAX):
         raise ValueError(f"top_k must lie between 0 and min(classes, {K.TOP_K_MAX}) = {min(V, K.TOP_K_MAX)}, got {top_k}")
     return cap
@@ -1255,7 +1257,7 @@ def token_log_probs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, *,
     ``log_probs`` and ``entropy`` are differentiable with respect to the logits, the top classes are not.  Masked classes
     (-inf) have no part; a row without any class has log p = -inf, entropy 0 and gradient 0; NaN in a row gives NaN.
     """
-    cap = _distribution_options(logits.shape[-1] if logits.dim() else 0, temperature, logit_softcap, top_k)
+    cap = _distribution_options(logits.shape[-1] if logits.dim() else 0, temperature, logit_softcap, top_k, ignore_index)
     z = _logit_rows(logits)
     shape = logits.shape[:-1]
     lab = _token_rows(ids, shape, logits.device) if ids is not None else None
@@ -1527,7 +1529,7 @@ def linear_token_log_probs(x: torch.Tensor, handle, ids: Optional[torch.Tensor] 
     """:func:`token_log_probs` of the LM head ``x @ W^T`` (``handle``: the ``(vocab, d)`` weight, x ``[..., d]``), whose logits are
     never formed: their statistics come out of the GEMM's epilogue.  With ``top_k``, and in the backward pass (it is differentiable
     with respect to x and the weight), they exist ``chunk_rows`` rows at a time."""
-    cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap, top_k)
+    cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap, top_k, ignore_index)
     shape = x.shape[:-1]
     lab = _token_rows(ids, shape, x.device) if ids is not None else None
     x2 = (x if x.dim() == 2 else x.reshape(math.prod(shape), x.shape[-1])).contiguous()

@@ -442,7 +442,7 @@ _LOGITS_DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 
 
 def _logits_dtype(t: torch.Tensor) -> int:
-    if t.dtype not in _LOGITS_DTYPE or not t.is_cuda or t.stride(-1) != 1:
+    if t.dtype not in _LOGITS_DTYPE or not t.is_cuda or (t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel()):
         raise KernelError(f"expected CUDA fp32 or bf16 logits with contiguous classes, got {t.dtype} on {t.device} "
                           f"with strides {tuple(t.stride())}")
     return _LOGITS_DTYPE[t.dtype]
@@ -482,8 +482,8 @@ def token_log_probs_bwd(logits, ids, norm, entropy, g_log_probs, g_entropy, dlog
 
 
 def _teacher_ids(t: torch.Tensor) -> int:
-    if t.dtype not in (torch.int32, torch.int64) or t.stride(1) != 1:
-        raise KernelError(f"teacher ids must be int32 or int64 [rows, k] with contiguous rows, got {t.dtype}")
+    if t.dtype not in (torch.int32, torch.int64) or not t.is_contiguous():
+        raise KernelError(f"teacher ids must be contiguous int32 or int64 [rows, k], got {t.dtype} with strides {t.stride()}")
     return int(t.dtype == torch.int64)
 
 
@@ -504,16 +504,16 @@ def _work_ptrs(work: torch.Tensor, rows: int, k: int, row0: int = 0):
 
 def distill_fwd(logits, teacher_ids, teacher_log_probs, work, *, renormalize, row0=0, total_rows=None, row_loss=None, softcap=0.0,
                 temperature=1.0) -> None:
-    """``teacher_ids`` (int32 / int64) and ``teacher_log_probs`` (fp32) [rows, k] with one row stride, for rows ``row0``, ... of the ``total_rows`` that
+    """``teacher_ids`` (int32 / int64) and ``teacher_log_probs`` (fp32), both contiguous [rows, k], for rows ``row0``, ... of the ``total_rows`` that
     ``work`` (:func:`distill_work`) is for; ``row_loss``: where the losses go instead of into ``work``."""
     rows, V = logits.shape
     k = teacher_ids.shape[1]
-    if teacher_log_probs.stride() != teacher_ids.stride() or teacher_log_probs.dtype != torch.float32:
-        raise KernelError("distillation: fp32 teacher values laid out like the teacher's ids are needed")
+    if not teacher_log_probs.is_contiguous() or teacher_log_probs.dtype != torch.float32 or teacher_log_probs.shape != teacher_ids.shape:
+        raise KernelError("distillation: contiguous fp32 teacher values of the ids' shape are needed")
     _, stats, q, loss = _work_ptrs(work, rows if total_rows is None else total_rows, k, row0)
     with _on(logits.device):
         check(lib().ob_distill_fwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), teacher_ids.data_ptr(),
-                                   _teacher_ids(teacher_ids), teacher_log_probs.data_ptr(), teacher_ids.stride(0), k, int(renormalize),
+                                   _teacher_ids(teacher_ids), teacher_log_probs.data_ptr(), k, k, int(renormalize),
                                    loss if row_loss is None else row_loss.data_ptr(), stats, q, rows, V, softcap, 1.0 / temperature,
                                    stream_ptr(logits.device)), "distill_fwd")
     _count()
@@ -526,7 +526,7 @@ def distill_bwd(logits, teacher_ids, work, g, dlogits, *, mean, row0=0, total_ro
     inv_count, stats, q, _ = _work_ptrs(work, rows if total_rows is None else total_rows, k, row0)
     with _on(logits.device):
         check(lib().ob_distill_bwd(logits.data_ptr(), _logits_dtype(logits), logits.stride(0), teacher_ids.data_ptr(),
-                                   _teacher_ids(teacher_ids), teacher_ids.stride(0), k, stats, q, _ptr(g),
+                                   _teacher_ids(teacher_ids), k, k, stats, q, _ptr(g),
                                    0 if g is None or g.dim() == 0 else g.stride(0), inv_count if mean else None, scale,
                                    dlogits.data_ptr(), _logits_dtype(dlogits), dlogits.stride(0), rows, V, softcap,
                                    1.0 / temperature, stream_ptr(logits.device)), "distill_bwd")
@@ -546,7 +546,7 @@ def distill_count(teacher_ids, teacher_log_probs, work, *, renormalize, V) -> No
     """1 / max(1, rows with a teacher) into ``work``, before the student's logits are there."""
     with _on(teacher_ids.device):
         check(lib().ob_distill_count(teacher_ids.data_ptr(), _teacher_ids(teacher_ids), teacher_log_probs.data_ptr(),
-                                     teacher_ids.stride(0), teacher_ids.shape[1], int(renormalize), teacher_ids.shape[0], V,
+                                     teacher_ids.shape[1], teacher_ids.shape[1], int(renormalize), teacher_ids.shape[0], V,
                                      work.data_ptr(), stream_ptr(teacher_ids.device)), "distill_count")
     _count()
 

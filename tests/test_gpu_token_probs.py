@@ -486,7 +486,7 @@ def test_top_classes_of_long_rows_in_bad_orders(dtype):
             assert torch.equal(out.top_ids, want)
 
 
-@pytest.mark.parametrize("rows,V,d,cap,temperature", [(1, 8, 64, None, 1.0), (7, 264, 128, None, 1.0), (300, 1000, 256, 30.0, 0.7), (2048, 5000, 512, None, 1.0),
+@pytest.mark.parametrize("rows,V,d,cap,temperature", [(1, 8, 64, None, 1.0), (16411, 264, 64, None, 1.0), (7, 264, 128, None, 1.0), (300, 1000, 256, 30.0, 0.7), (2048, 5000, 512, None, 1.0),
                                                       (1100, 20008, 72, None, 2.0), (328, 50304, 128, 30.0, 1.0)])
 def test_head_scores_out_of_the_epilogue(rows, V, d, cap, temperature):
     """Tiles of both geometries, ragged in rows, classes and contraction, against the same head's fp32 logits."""
@@ -567,3 +567,77 @@ def test_head_scores_of_few_tokens(rows, V, d, cap):
     dz, _ = score_gradients_64(z, ids, torch.ones(rows, device=DEV), torch.zeros(rows, device=DEV), 1.0, cap or 0.0)
     want, size = dz @ w.double(), dz.abs() @ w.double().abs()
     _close(gx, want, (2.0 ** -8 + 2.0 ** -12 + 4 * e) * size + 2.0 ** -8 * want.abs() + 1e-12)
+
+
+def test_certain_tokens_and_empty_batches():
+    for cap in (None, 30.0):
+        z = torch.full((64, 5000), -1000.0, device=DEV)
+        z[:, 17] = torch.linspace(-20, 20, 64, device=DEV)
+        out = F.token_log_probs(z, torch.full((64,), 17, device=DEV), logit_softcap=cap, temperature=0.25, top_k=2)
+        assert torch.all(out.log_probs <= 0) and torch.all(out.top_log_probs <= 0) and torch.all(out.entropy >= 0)
+    head = _bf16_head(64, 64)
+    x = torch.zeros(0, 64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    ids = torch.zeros(0, dtype=torch.int64, device=DEV)
+    out = head.token_log_probs(x, ids, top_k=3)
+    loss = head.distillation_loss(x, ids.view(0, 1).expand(0, 4), torch.zeros(0, 4, device=DEV))
+    z = torch.zeros(0, 10, device=DEV, requires_grad=True)
+    kd = F.distillation_loss(z, ids.view(0, 1), torch.zeros(0, 1, device=DEV))
+    gx, = torch.autograd.grad(out.log_probs.sum() + loss, x)
+    assert out.top_ids.shape == (0, 3) and float(loss.detach()) == 0 and float(kd.detach()) == 0 and gx.shape == (0, 64)
+    assert torch.autograd.grad(kd, z)[0].shape == (0, 10)
+
+
+def test_distillation_of_more_classes_than_one_block_has_bits_for():
+    rows, V = 400, 1_200_007
+    z = torch.randn(rows, V, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16)
+    ids = torch.randint(0, V, (rows, 5), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    ids[:, 4] = ids[:, 0]
+    t = torch.log(torch.tensor([0.4, 0.2, 0.1, 0.1, 0.7], device=DEV)).expand(rows, 5)
+    loss = F.distillation_loss(z, ids, t, reduction="none")
+    part = torch.arange(0, rows, 40, device=DEV)
+    want, _ = distillation_64(z[part], ids[part], t[part], "rest", "none")
+    _close(loss[part], want, 4 * _eps(V, 8.0) + 2.0 ** -23 * want.abs())
+
+
+def test_head_scores_with_the_weights_still_to_be_gathered():
+    """The epilogue's scores in a launch whose copy warps bring in the other shards (here from this GPU's memory)."""
+    from olmax_b200.ops import _lib
+    from olmax_b200.ops import kernels as K
+
+    M, N, Kd, R = 264, 4096, 256, 4
+    g = torch.Generator(device=DEV).manual_seed(6)
+    a = torch.randn(M, Kd, generator=g, device=DEV).to(torch.bfloat16)
+    b = torch.randn(N, Kd, generator=g, device=DEV).to(torch.bfloat16)
+    per = N // R
+    shards = [b[r * per : (r + 1) * per].clone() for r in range(R)]
+    table = K.pointer_table([s.data_ptr() for s in shards], a.device)
+    ids = _ids(M, N)
+    want = [torch.empty(M, device=DEV) for _ in range(2)]
+    K.gemm_scores(a, b, ids, *want, None, M, N, Kd, rows=M)
+    for rank in (0, 2):
+        buf = torch.zeros(R, per * Kd, dtype=torch.bfloat16, device=DEV)
+        buf[rank] = shards[rank].view(-1)
+        flags = torch.zeros(1024, dtype=torch.int32, device=DEV)
+        got = [torch.empty(M, device=DEV) for _ in range(2)]
+        K.gemm_scores(a, buf[0].view(per, Kd), ids, *got, None, M, N, Kd, rows=M, N_s=per, b_shard_stride=per * Kd, ag_src=table,
+                      ag_flags=flags, ag_rank=rank)
+        _lib.check_status()
+        assert torch.equal(buf.view(N, Kd), b)
+        for x, y in zip(got, want):
+            _close(x, y, 4 * _eps(N, float((a.float() @ b.float().t()).abs().max())))
+
+
+def test_extents_of_one_whatever_their_strides():
+    z = _logits(5, 300)
+    one = z[:, 7:8]                                                # one class: its stride says nothing
+    odd = one.as_strided((5, 1), (300, 77))
+    for t in (one, odd):
+        out = F.token_log_probs(t, torch.zeros(5, dtype=torch.int64, device=DEV), top_k=1)
+        assert torch.all(out.log_probs == 0) and torch.all(out.entropy == 0) and torch.all(out.top_ids == 0)
+    ids, t = _teacher(5, 300, 1)
+    for shape in ((5, 1), (1, 5)):                                 # one pair per row, one row
+        zz = z if shape[0] == 5 else z[:1]
+        i2, t2 = ids.view(shape), t.view(shape)
+        i3 = torch.zeros(400, dtype=torch.int64, device=DEV).as_strided(shape, (13 if shape[0] > 1 else 50, 1 if shape[0] == 1 else 29)).copy_(i2)
+        _check_distillation(zz, i3, t2, "rest")
+        _check_scores(zz, ids.view(-1)[: zz.shape[0]], 3)
