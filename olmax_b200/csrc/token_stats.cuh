@@ -32,7 +32,7 @@ __device__ __forceinline__ float min_nan(float x, float y) {
 
 // The capped logit cap(z) = softcap * tanh(z / softcap).  tanh(u) = 1 - 2 r and 1 - tanh^2(u) = 4 r (1 - r) with r = 1 / a, a = 1 + e^2u: the
 // approximate tanh instruction's error of 5e-4 would show in every log probability, this form's is below 8e-7 (the roundings of r <= 1 and the
-// exponential's).  It takes two special-function operations beside the exponential of the softmax, of which an SM does sixteen a clock: they
+// exponential's; 3e-7 is the largest seen), so that a cap of 256 costs a logit no more than 2e-4.  It takes two special-function operations beside the exponential of the softmax, of which an SM does sixteen a clock: they
 // bound the kernels.  So four classes share a reciprocal, that of the product of their a; a <= 2^30 changes no tanh and keeps the product
 // finite.  What follows is linear in r: t = (cap(z) - m) c is one multiply-add.
 struct Scaling {
@@ -112,10 +112,10 @@ __device__ __forceinline__ float largest(const float (&f)[E]) {
   for (int j = 1; j + 1 < E; j += 2) mx = max3(mx, f[j], f[j + 1]);
   return E % 2 ? mx : fmaxf(mx, f[E - 1]);
 }
-constexpr float ABSENT = 1e30f;   // the r of a class that is not there: its exponent is far below any, and finite
+constexpr float ABSENT = 1e20f;   // the r of a class that is not there: its exponent is far below any, and finite
 // Adds E classes of logits f with the largest (capped) logit mx, known first so that the exponentials do not wait for one another.  A masked class
-// (-inf) adds nothing: its exponent is kept finite where 0 * infinity would come up.  With CAP f are the classes' r (ABSENT for one that is not there).  Two-wide arithmetic
-// halves the instructions beside the exponentials, which the issue slots are short of at two bytes a class.
+// (-inf) adds nothing: its exponent is kept finite where 0 * infinity would come up.  With CAP f are the classes' r (ABSENT for one that is
+// not there).  Two-wide arithmetic halves the instructions beside the exponentials, which the issue slots are short of at two bytes a class.
 template <bool CAP, bool W, int E>
 __device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], float mx, const Scaling& sc) {
   if (mx > a.m) a = shifted(a, mx, sc.c);

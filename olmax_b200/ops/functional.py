@@ -1146,11 +1146,11 @@ class TokenLogProbs(NamedTuple):
 
 
 def _distribution_options(V: int, temperature: float, logit_softcap: Optional[float], top_k: int = 0, ignore_index: int = -100) -> float:
-    if not (0.0 < temperature < math.inf):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not (1e-6 <= temperature <= 1e6):
+        raise ValueError(f"temperature must lie between 1e-6 and 1e6, got {temperature}")
     cap = float(logit_softcap or 0.0)
-    if not (0.0 <= cap < math.inf):
-        raise ValueError(f"logit_softcap must be positive and finite (or None), got {logit_softcap}")
+    if not (cap == 0.0 or 1e-3 <= cap <= 256.0):   # (the kernels' tanh is accurate to some 1e-7 of the cap)
+        raise ValueError(f"logit_softcap must lie between 1e-3 and 256 (or be None), got {logit_softcap}")
     if V < 1:
         raise ValueError("logits need at least one class")
     if not -(2 ** 31) <= ignore_index < 2 ** 31:
@@ -1251,7 +1251,7 @@ def token_log_probs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, *,
     * ``log_probs``: log p of ``ids [...]``.  A token equal to ``ignore_index`` or outside ``[0, V)`` is not scored: 0 and
       no gradient.
     * ``entropy`` of every row.
-    * ``top_k`` > 0 (at most 128): log p and class of the largest logits, largest first, equal ones in the order of their
+    * ``top_k`` > 0 (at most 128, or the number of classes): log p and class of the largest logits, largest first, equal ones in the order of their
       classes.
 
     ``log_probs`` and ``entropy`` are differentiable with respect to the logits, the top classes are not.  Masked classes

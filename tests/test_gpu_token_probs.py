@@ -68,7 +68,7 @@ def test_scores(rows, V, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("temperature,cap", [(0.5, 0.0), (1.0, 30.0), (2.0, 5.0)])
+@pytest.mark.parametrize("temperature,cap", [(0.5, 0.0), (1.0, 30.0), (2.0, 5.0), (1.0, 256.0), (0.01, 1.0), (1e-6, 0.0), (1e6, 0.0), (1e-6, 30.0), (1.0, 1e-3)])
 def test_scores_scaled(temperature, cap, dtype):
     _check_scores(_logits(40, 5003, dtype, spread=8.0), _ids(40, 5003), 16, temperature, cap)
 

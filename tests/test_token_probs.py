@@ -268,7 +268,7 @@ def test_a_vocabulary_parallel_head_refuses():
 
 
 @pytest.mark.parametrize("bad", [
-    dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf),
+    dict(temperature=0.0), dict(temperature=1e-7), dict(temperature=1e7), dict(logit_softcap=300.0), dict(logit_softcap=1e-4), dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf),
     dict(logit_softcap=-1.0), dict(logit_softcap=math.inf), dict(top_k=-1), dict(top_k=11), dict(ids=torch.zeros(5, dtype=torch.int64)),
     dict(ids=torch.zeros(4)), dict(ignore_index=2 ** 32 + 5),
 ])
