@@ -4,6 +4,7 @@ Kernel micro-benchmarks with CUDA-event timing (and the small cases used for ncu
     python -m olmax_b200.ops.microbench gemm            # the GEMM shapes of a 7B layer, all three layouts
     python -m olmax_b200.ops.microbench attn            # flash attention forward / backward, B=2 S=4096 H=32
     python -m olmax_b200.ops.microbench elementwise     # rmsnorm / rope / glu / adamw / cross-entropy bandwidth
+    python -m olmax_b200.ops.microbench logits          # log probabilities, top classes, distillation over logits; LM head scores
     python -m olmax_b200.ops.microbench gemm --small    # one launch per variant on an 8192x4096x4096 case (for ncu)
     python -m olmax_b200.ops.microbench elementwise --small   # one rmsnorm fwd + bwd launch on [8192, 4096] (for ncu)
     python -m torch.distributed.run --nproc-per-node 2 --master-addr 127.0.0.1 -m olmax_b200.ops.microbench p2p
@@ -230,9 +231,52 @@ def bench_p2p(iters: int, small: bool):
     return out if rank == 0 else {}
 
 
+def bench_logits(iters: int, small: bool):
+    """The kernels over the LM head's distribution: 2048 rows (``--small``: 592) of the OLMo2 vocabulary, 0.4-0.8 GB of logits."""
+    dev = torch.device("cuda")
+    peaks = _peaks()
+    rows, V, k = (592 if small else 2048), 100352, 64
+    iters = 1 if small else iters
+    out = {}
+
+    def report(name, ms, nbytes):
+        gbs = nbytes / ms / 1e6
+        out[name] = {"ms": round(ms, 4), "GB/s": round(gbs, 1), "of_measured_copy": round(gbs / peaks["hbm_gbs"], 3)}
+        print(f"{name:34s} {ms:7.3f} ms  {gbs:8.1f} GB/s  {gbs / peaks['hbm_gbs']:5.2f} of measured copy bandwidth", flush=True)
+
+    ids = torch.randint(0, V, (rows,), device=dev)
+    lp, ent, g = (torch.ones(rows, device=dev) for _ in range(3))
+    norm = torch.empty((rows, 2), device=dev)
+    top, top_ids = torch.empty((rows, k), device=dev), torch.empty((rows, k), dtype=torch.int64, device=dev)
+    t_ids, t = torch.randint(0, V, (rows, k), device=dev), torch.full((rows, k), -5.0, device=dev)
+    work = K.distill_work(rows, k, dev)
+    for dtype, cap in ((torch.float32, 0.0), (torch.bfloat16, 0.0), (torch.bfloat16, 30.0)):
+        z = torch.randn(rows, V, device=dev).mul_(2.0).to(dtype)
+        d = torch.empty_like(z)
+        n = z.numel() * z.element_size()
+        name = f"{str(dtype)[6:]}{' soft-cap' if cap else ''} "
+        report(name + "scores", _time(lambda: K.token_log_probs_fwd(z, ids, lp, ent, norm, None, None, softcap=cap), iters), n)
+        report(name + "scores + top 64", _time(lambda: K.token_log_probs_fwd(z, ids, lp, ent, None, top, top_ids, softcap=cap), iters), n)
+        report(name + "scores bwd", _time(lambda: K.token_log_probs_bwd(z, ids, norm, ent, g, g, d, softcap=cap), iters), 2 * n)
+        report(name + "distill", _time(lambda: K.distill_fwd(z, t_ids, t, work, renormalize=False, softcap=cap), iters), n)
+        report(name + "distill bwd", _time(lambda: K.distill_bwd(z, t_ids, work, None, d, mean=False, softcap=cap), iters), 2 * n)
+        del z, d
+    d_model = 4096
+    w = torch.randn(V, d_model, device=dev).to(torch.bfloat16)
+    for tokens in (8, 1024, rows):
+        x = torch.randn(tokens, d_model, device=dev).to(torch.bfloat16)
+        xi, l2, e2 = ids[:1].expand(tokens).contiguous(), torch.empty(tokens, device=dev), torch.empty(tokens, device=dev)
+        ms = _time(lambda: K.gemm_scores(x, w, xi, l2, e2, None, tokens, V, d_model, rows=tokens), iters)
+        tf = 2 * tokens * V * d_model / ms / 1e9
+        out[f"head scores {tokens}"] = {"ms": round(ms, 4), "TFLOP/s": round(tf, 1), "of_measured": round(tf / peaks["bf16_tflops"], 3)}
+        print(f"{f'head scores, {tokens} tokens':34s} {ms:7.3f} ms  {tf:8.1f} TFLOP/s, weights at {w.numel() * 2 / ms / 1e6:.0f} GB/s", flush=True)
+    _lib.check_status()
+    return out
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["gemm", "attn", "elementwise", "p2p"])
+    ap.add_argument("what", choices=["gemm", "attn", "elementwise", "logits", "p2p"])
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--small", action="store_true", help="one launch per variant on a small case (for ncu)")
     ap.add_argument("--json", default=None, help="also write the results to this file")
@@ -240,7 +284,7 @@ def main():
     if not torch.cuda.is_available():
         print("needs a CUDA device")
         return 1
-    fn = {"gemm": bench_gemm, "attn": bench_attn, "elementwise": bench_elementwise, "p2p": bench_p2p}[args.what]
+    fn = {"gemm": bench_gemm, "attn": bench_attn, "elementwise": bench_elementwise, "logits": bench_logits, "p2p": bench_p2p}[args.what]
     out = fn(args.iters, args.small)
     if args.json and out:
         Path(args.json).write_text(json.dumps(out, indent=1))
