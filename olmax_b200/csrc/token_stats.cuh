@@ -47,12 +47,11 @@ struct Scaling {
   // f <- r of the logits f (one, or a multiple of four)
   template <int E>
   __device__ __forceinline__ void reciprocals(float (&f)[E]) const {
-    if (E == 1) {
+    if constexpr (E == 1) {
       f[0] = rcp_fast(1.f + exp2_fast(min_nan(f[0] * k, 30.f)));
-      return;
     }
 #pragma unroll
-    for (int j = 0; j + 3 < E; j += 4) {
+    for (int j = 0; j < E / 4 * 4; j += 4) {
       const float2 a = denominators(f[j], f[j + 1]), b = denominators(f[j + 2], f[j + 3]);
       const float2 p = mul2(make_float2(a.x, b.x), make_float2(a.y, b.y));
       const float all = rcp_fast(p.x * p.y);
