@@ -987,7 +987,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
   gemm_body<A_MN, B_MN, 2, BN_WIDE, SEG>(tmA, tmB, tmB2, tmC, tmS1, tmS2, p);
 }
 
-// The scores of tokens: K-major operands, no output.
+// The scores of tokens: K-major operands, no output.  Bound by the tensor cores (2048 x 100352 x 4096: 1.05-1.06 ms with the join, 1.6 PFLOP/s),
+// with few tokens by reading the weights.
 template <int BN, int SCORE>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
     gemm_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const KernelParams p) {
@@ -1416,7 +1417,7 @@ extern "C" int ob_gemm_scores(const ObGemmArgs* a, const ObScoreArgs* s, cudaStr
   if (s->rows < 0 || s->rows > a->M || s->parts == nullptr || s->entropy == nullptr || (reinterpret_cast<uintptr_t>(s->parts) & 15) != 0 ||
       (s->log_probs != nullptr && (s->ids == nullptr || s->target == nullptr)) || (s->ids != nullptr && s->target == nullptr))
     OB_FAIL(-5, "scores: missing tensor");
-  // Few tokens and unsharded weights, which are read at 5.4-5.6 TB/s with the operands exchanged: 8 x 100352 x 4096 150 us (195 with tokens as rows),
+  // Few tokens and unsharded weights, which are read at up to 5.5 TB/s with the operands exchanged: 8 x 100352 x 4096 150 us (195 with tokens as rows),
   // 8 x 256000 x 4608 441 (604), 8 x 50304 x 1024 35 (41).
   const bool few = s->rows <= FEW_TOKENS && a->M <= FEW_TOKENS && (a->N_s <= 0 || a->N_s == a->N) && a->ag_src == nullptr;
   ObGemmArgs turned = *a;
