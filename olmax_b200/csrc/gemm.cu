@@ -132,22 +132,14 @@ constexpr int FEW_TOKENS = 16;   // columns of SCORES_BY_COLUMN
 // Statistics of 32 logits of a row from a tile's columns [col, col + 32), of which the first n are there.
 template <bool CAP>
 __device__ __forceinline__ void score_columns(Stats& a, float (&f)[32], int n, const Scaling& sc) {
-  if (CAP) sc.reciprocals(f);
+  if (CAP) sc.cap_logits(f);
   if (n < 32) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
       if (j >= n) f[j] = CAP ? ABSENT : -INFINITY;
   }
-  float mx;
-  if (CAP) {
-    float least = f[0];
-#pragma unroll
-    for (int j = 1; j < 32; ++j) least = fminf(least, f[j]);
-    mx = sc.of_r(least);
-  } else {
-    mx = largest(f);
-  }
-  add_classes<CAP, true, 32>(a, f, mx, sc);
+  if (CAP) add_capped<true, 32>(a, f, sc);
+  else add_classes<false, true, 32>(a, f, largest(f), sc);
 }
 
 // One warp-interleaved copy of n16 16-byte words; cw = this copy warp's index among n_cw.

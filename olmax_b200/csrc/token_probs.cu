@@ -292,8 +292,8 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, unsigned long long 
 // first k.  The bound is the k-th largest of the threads' maxima so far, which no more than 1.2 k classes reach if they are spread over the
 // threads by chance; it is looked for at the first batch, whenever STEP more groups have come together, and at the end if there are many.  Then the
 // classes of the groups above it are read again and put in order.
-// Bound by HBM in fp32 (2048 x 100352: 132 us, 6.2 TB/s), by loads and the special-function unit in bf16 (80 us, 5.1 TB/s), by that unit with a
-// soft-cap (138 us, 77 % busy at 592 rows); the 64 top classes add 42 us to the first (instructions and barriers of the selection).
+// Bound by HBM in fp32 (2048 x 100352: 132 us, 6.2 TB/s), by loads and the special-function unit in bf16 (80 us, 5.1 TB/s), by instructions with a
+// soft-cap (118 us; 184 us where an eighth of the logits lie beyond 3/4 of the cap); the 64 top classes add 42 us to the first (instructions and barriers of the selection).
 template <class T, int U, bool CAP, bool TOP>
 __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 4 : sizeof(T) == 2 ? 5 : 6)
     token_log_probs_fwd_kernel(const T* __restrict__ logits, long long ld, int C, ScoreArgs p) {
@@ -336,13 +336,13 @@ __global__ void __launch_bounds__(TP_THREADS, TOP || CAP ? 4 : sizeof(T) == 2 ? 
       float y[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) y[j] = f[j];
-      p.sc.reciprocals(y);
+      p.sc.cap_logits(y);
       if (b + TP_THREADS * U > v1) {
 #pragma unroll
         for (int j = 0; j < E; ++j)
           if (b + j / N * TP_THREADS + (int)threadIdx.x >= v1) y[j] = ABSENT;
       }
-      add_classes<true, true, E>(a, y, b + (int)threadIdx.x < v1 ? p.sc.capped(mx) : -INFINITY, p.sc);
+      add_capped<true, E>(a, y, p.sc);
     } else {
       add_classes<false, true, E>(a, f, mx, p.sc);
     }
@@ -559,8 +559,8 @@ struct ScoreGradArgs {
 };
 
 // dz = dy/dz (g_lp (onehot - p) - g_H p (log p + H)) = dy/dz (g_lp onehot - p (k0 + k1 t)) with t = log2 p.
-// One read and one write of a class: 2048 x 100352 fp32 243 us, bf16 131 us (6.8 and 6.3 TB/s, HBM), with a soft-cap 146 us (special-function unit,
-// 72 % busy at 592 rows).
+// One read and one write of a class: 2048 x 100352 fp32 243 us, bf16 131 us (6.8 and 6.3 TB/s, HBM), with a soft-cap 153 us (instructions; 231 us
+// where an eighth of the logits lie beyond 3/4 of the cap).
 template <class T, class D, bool CAP>
 __global__ void __launch_bounds__(GRAD_THREADS, CAP && sizeof(T) == 2 ? 5 : 6)
     token_log_probs_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts,
@@ -584,14 +584,14 @@ __global__ void __launch_bounds__(GRAD_THREADS, CAP && sizeof(T) == 2 ? 5 : 6)
     norm = make_float2(0.f, 0.f);
     k0 = k1 = gl = 0.f;
   }
-  if (CAP) k0 *= 4.f, k1 *= 4.f, gl *= 4.f;   // of the slope 4 r (1 - r)
   k0 = -k0, k1 = -k1;
-  const float t0 = (p.sc.cap - norm.x) * p.sc.c - norm.y, t1 = -2.f * p.sc.cap * p.sc.c;
+  const float t0 = fmaf(-norm.x, p.sc.c, -norm.y);   // (capped logits are small: one rounding of this is no more than theirs)
   map_span<T, D>(logits + row * ld, dlogits + row * ld_d, p.V, part, parts, per_block, [&](auto& f, int i) {
     constexpr int M = sizeof(f) / sizeof(float);
-    if (CAP) p.sc.reciprocals(f);
+    float slope[M];
+    if (CAP) p.sc.template cap_logits<true>(f, slope);
     auto pair = [&](float2 x) {
-      const float2 t = CAP ? fma2(x, make_float2(t1, t1), make_float2(t0, t0))
+      const float2 t = CAP ? fma2(x, make_float2(p.sc.c, p.sc.c), make_float2(t0, t0))
                            : fma2(add2(x, make_float2(-norm.x, -norm.x)), make_float2(p.sc.c, p.sc.c), make_float2(-norm.y, -norm.y));
       // (2^t is 0 from -150 on; what it is multiplied by stays finite)
       const float2 u = CAP ? t : make_float2(fmaxf(t.x, -1024.f), fmaxf(t.y, -1024.f));
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, CAP && sizeof(T) == 2 ? 5 : 6)
         if (i + j == id) g[j] += gl;
     }
 #pragma unroll
-    for (int j = 0; j < M; ++j) f[j] = CAP ? g[j] * fmaf(-f[j], f[j], f[j]) : g[j];
+    for (int j = 0; j < M; ++j) f[j] = CAP ? g[j] * slope[j] : g[j];
   });
 }
 
@@ -650,20 +650,21 @@ __device__ __forceinline__ void rest_gradient(float (&f)[M], bool zero, float m,
     for (int j = 0; j < M; ++j) f[j] = 0.f;
     return;
   }
-  if (CAP) sc.reciprocals(f);
-  const float t0 = (sc.cap - m) * sc.c - log_s, t1 = -2.f * sc.cap * sc.c;
+  float slope[M];
+  if (CAP) sc.template cap_logits<true>(f, slope);
+  const float t0 = fmaf(-m, sc.c, -log_s);   // (as in the gradient of the scores)
   float g[M + 1];
 #pragma unroll
   for (int j = 0; j < M; j += 2) {
     const float2 x = make_float2(f[j], j + 1 < M ? f[j + 1] : f[j]);
-    const float2 t = CAP ? fma2(x, make_float2(t1, t1), make_float2(t0, t0))
+    const float2 t = CAP ? fma2(x, make_float2(sc.c, sc.c), make_float2(t0, t0))
                          : fma2(add2(x, make_float2(-m, -m)), make_float2(sc.c, sc.c), make_float2(-log_s, -log_s));
     const float2 o = mul2(make_float2(exp2_fast(t.x), exp2_fast(t.y)), make_float2(coef, coef));
     g[j] = o.x;
     g[j + 1] = o.y;
   }
 #pragma unroll
-  for (int j = 0; j < M; ++j) f[j] = CAP ? g[j] * fmaf(-f[j], f[j], f[j]) : g[j];
+  for (int j = 0; j < M; ++j) f[j] = CAP ? g[j] * slope[j] : g[j];
 }
 
 // Sums over the block, the same in every thread.
@@ -681,10 +682,9 @@ __device__ __forceinline__ double block_sum(double x, double* red) {
 // A row belongs to a cluster of C CTAs as in the log probabilities.  Thread t holds the teacher's pair t.  One bit of shared memory per vector, the
 // bits of a thread's batch side by side, says whether the teacher names one of its classes, one bit per class which: a batch without one, and
 // that is most of them, costs one look.
-// With 64 classes named, 2048 x 100352: fp32 140 us (5.9 TB/s, HBM), bf16 100 us (loads), with a soft-cap 146 us (special-function unit, 64 % busy at
-// 592 rows).
+// With 64 classes named, 2048 x 100352: fp32 140 us (5.9 TB/s, HBM), bf16 100 us (loads), with a soft-cap 144 us (instructions).
 template <class T, int U, bool CAP>
-__global__ void __launch_bounds__(TP_THREADS, 6)
+__global__ void __launch_bounds__(TP_THREADS, CAP ? 5 : 6)
     distill_fwd_kernel(const T* __restrict__ logits, long long ld, int C, int slice_vectors, DistillArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
   extern __shared__ __align__(16) char shared_bytes[];
@@ -743,7 +743,7 @@ __global__ void __launch_bounds__(TP_THREADS, 6)
     float f[E];
 #pragma unroll
     for (int k = 0; k < U; ++k) unpack<T>(v[k], f + k * N);
-    if (CAP) p.sc.reciprocals(f);
+    if (CAP) p.sc.cap_logits(f);
     const int bit = (batch * TP_THREADS + threadIdx.x) * U;
     const unsigned some = (flags[bit >> 5] >> (bit & 31)) & ((1u << U) - 1);
     if (some) {
@@ -762,10 +762,7 @@ __global__ void __launch_bounds__(TP_THREADS, 6)
         if (b + j / N * TP_THREADS + (int)threadIdx.x >= v1) f[j] = ABSENT;
     }
     if (CAP) {
-      float least = f[0];
-#pragma unroll
-      for (int j = 1; j < E; ++j) least = fminf(least, f[j]);
-      add_classes<true, false, E>(a, f, least == ABSENT ? -INFINITY : p.sc.of_r(least), p.sc);
+      add_capped<false, E>(a, f, p.sc);
     } else {
       add_classes<false, false, E>(a, f, largest(f), p.sc);
     }
@@ -844,9 +841,9 @@ struct DistillGradArgs {
 };
 
 // Every class as one outside the teacher's, then the teacher's anew.  2048 x 100352, 64 of the teacher's: fp32 244 us, bf16 131 us (6.7 and 6.3 TB/s,
-// HBM), with a soft-cap 143 us (special-function unit, 73 % busy at 592 rows).
+// HBM), with a soft-cap 157 us (instructions).
 template <class T, class D, bool CAP>
-__global__ void __launch_bounds__(GRAD_THREADS, 6)
+__global__ void __launch_bounds__(GRAD_THREADS, CAP && sizeof(T) == 2 ? 5 : 6)
     distill_bwd_kernel(const T* __restrict__ logits, long long ld, D* __restrict__ dlogits, long long ld_d, int parts, int per_block,
                        DistillGradArgs p) {
   const long long row = blockIdx.x / (unsigned)parts;
@@ -857,19 +854,22 @@ __global__ void __launch_bounds__(GRAD_THREADS, 6)
   const float4 norm = *reinterpret_cast<const float4*>(p.row_stats + row * 8 + 4);
   long long id = -1;
   float q = -1.f;
-  if ((int)threadIdx.x < p.k) {
+  auto teacher = [&] {
+    if ((int)threadIdx.x >= p.k) return;
     q = p.q[row * p.k + threadIdx.x];
     id = teacher_id(p.teacher_ids, p.ids_64, row * p.ld_t + threadIdx.x);
-  }
+  };
+  if (!CAP) teacher();   // (with a soft-cap the registers are short)
   const float gs = (p.g != nullptr ? p.g[row * p.stride_g] : 1.f) * p.scale * (p.inv_count != nullptr ? *p.inv_count : 1.f);
   const bool nothing = st.x < 0.f || (norm.x == -INFINITY && norm.y == -INFINITY);
   const bool zero = nothing || (norm.z == -INFINITY && norm.w == -INFINITY);   // no class outside the teacher's
-  const float coef = st.y * gs * p.sc.inv_temp * (CAP ? 4.f : 1.f);
+  const float coef = st.y * gs * p.sc.inv_temp;
   const int2 span = map_span<T, D>(z, d, p.V, part, parts, per_block, [&](auto& f, int) {
     rest_gradient<CAP>(f, zero, norm.z, norm.w, coef, p.sc);
   });
   // the teacher's classes, over what has just been written for them
   __syncthreads();
+  if (CAP) teacher();
   if (!nothing && !(q < 0.f) && id >= span.x && id < span.y) {
     float slope;
     const float x = p.sc.capped(to_f(z[id]), &slope);

@@ -23,59 +23,108 @@ __device__ __forceinline__ float rcp_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// (fminf would drop a NaN)
-__device__ __forceinline__ float min_nan(float x, float y) {
-  float z;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
-  return z;
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
-// The capped logit cap(z) = softcap * tanh(z / softcap).  tanh(u) = 1 - 2 r and 1 - tanh^2(u) = 4 r (1 - r) with r = 1 / a, a = 1 + e^2u: the
-// approximate tanh instruction's error of 5e-4 would show in every log probability, this form's is below 8e-7 (the roundings of r <= 1 and the
-// exponential's; 3e-7 is the largest seen), so that a cap of 256 costs a logit no more than 2e-4.  It takes two special-function operations beside the exponential of the softmax, of which an SM does sixteen a clock: they
-// bound the kernels.  So four classes share a reciprocal, that of the product of their a; a <= 2^30 changes no tanh and keeps the product
-// finite.  What follows is linear in r: t = (cap(z) - m) c is one multiply-add.
+// The capped logit y = cap tanh(u), u = z / cap.  Up to |u| = 3/4, where almost all logits lie, tanh(u) / u is a polynomial g in s = u^2, so that
+// y = z g(s) is relatively as exact as fp32 arithmetic is (off by at most 2.3 times 2^-24, 0.65 in the root of the mean square) and takes no special-function
+// operation, of which an SM does sixteen a clock; beyond, tanh|u| = 1 - 2 w with w = e / (1 + e) <= 0.19, e = e^-2|u|, whose error arrives at a third.
+// 1 - tanh^2(u) is formed of tanh(u) or as 4 w (1 - w).  The coefficients are the minimax fit of tanh(sqrt s) / sqrt s on [0, 9/16] by a polynomial that is 1
+// at 0 (relative error 3.3e-8, Remez exchange in 80-bit floats, then rounded).  w for every logit was off by 3e-7 cap, near zero
+// too: 1e-5 of a probability at a cap of 30.
 struct Scaling {
-  float cap, k;     // k = 2 log2(e) / cap
-  float c;          // log2(e) / T
-  float inv_temp;   // 1 / T
+  float cap, minus_s;   // -1 / cap^2
+  float k;              // 2 log2(e) / cap
+  float c;              // log2(e) / T
+  float inv_temp;       // 1 / T
 
-  __device__ __forceinline__ float2 denominators(float z0, float z1) const {
-    const float2 x = mul2(make_float2(z0, z1), make_float2(k, k));
-    return add2(make_float2(exp2_fast(min_nan(x.x, 30.f)), exp2_fast(min_nan(x.y, 30.f))), make_float2(1.f, 1.f));
-  }
-  // f <- r of the logits f (one, or a multiple of four)
-  template <int E>
-  __device__ __forceinline__ void reciprocals(float (&f)[E]) const {
-    if constexpr (E == 1) {
-      f[0] = rcp_fast(1.f + exp2_fast(min_nan(f[0] * k, 30.f)));
-    }
+  // w of four logits, which share a reciprocal: that of the product of their denominators
+  __device__ __forceinline__ void far_tails(const float (&z)[4], float (&w)[4]) const {
+    float a[4];
 #pragma unroll
-    for (int j = 0; j < E / 4 * 4; j += 4) {
-      const float2 a = denominators(f[j], f[j + 1]), b = denominators(f[j + 2], f[j + 3]);
-      const float2 p = mul2(make_float2(a.x, b.x), make_float2(a.y, b.y));
-      const float all = rcp_fast(p.x * p.y);
-      const float2 q = mul2(make_float2(all, all), make_float2(p.y, p.x));   // 1 / (a.x a.y), 1 / (b.x b.y)
-      const float2 ra = mul2(make_float2(q.x, q.x), make_float2(a.y, a.x)), rb = mul2(make_float2(q.y, q.y), make_float2(b.y, b.x));
-      f[j] = ra.x;
-      f[j + 1] = ra.y;
-      f[j + 2] = rb.x;
-      f[j + 3] = rb.y;
+    for (int j = 0; j < 4; ++j) {
+      w[j] = exp2_fast(-fabsf(z[j]) * k);
+      a[j] = 1.f + w[j];
+    }
+    const float p = a[0] * a[1], q = a[2] * a[3], all = rcp_fast(p * q), x = all * q, y = all * p;
+    w[0] *= x * a[1];
+    w[1] *= x * a[0];
+    w[2] *= y * a[3];
+    w[3] *= y * a[2];
+  }
+  // f <- capped logits, and with SLOPE slope <- dy / dz, of E logits (one, or a multiple of four)
+  template <bool SLOPE, int E>
+  __device__ __forceinline__ void cap_logits(float (&f)[E], float (&slope)[E]) const {
+    // (signs for a polynomial in -s)
+    constexpr float G[6] = {1.f, 0.33333068381f, 0.13326521175f, 0.05339025875f, 0.019664913816f, 0.0047694904028f};
+    constexpr float FAR = -0.5625f;
+    constexpr int Q = E < 4 ? E : 4;
+#pragma unroll
+    for (int j = 0; j < E; j += Q) {
+      float z[4], s[4], y[4], d[4];   // s: -u^2
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = f[i < Q ? j + i : j];
+#pragma unroll
+      for (int i = 0; i < Q; i += 2) {
+        const float2 v = make_float2(z[i], z[i + 1]), t = mul2(mul2(v, v), make_float2(minus_s, minus_s));
+        float2 g = make_float2(G[5], G[5]);
+#pragma unroll
+        for (int n = 4; n >= 0; --n) g = fma2(g, t, make_float2(G[n], G[n]));
+        const float2 o = mul2(v, g);
+        s[i] = t.x;
+        s[i + 1] = t.y;
+        y[i] = o.x;
+        y[i + 1] = o.y;
+        if (SLOPE) {
+          const float2 e = fma2(mul2(o, o), make_float2(minus_s, minus_s), make_float2(1.f, 1.f));
+          d[i] = e.x;
+          d[i + 1] = e.y;
+        }
+      }
+      if ((Q == 1 ? s[0] : fminf(min3(s[0], s[1], s[2]), s[3])) < FAR) {   // (a NaN goes through the polynomial)
+        float w[4];
+        far_tails(z, w);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          if (!(s[i] < FAR)) continue;
+          y[i] = copysignf(fmaf(-2.f * cap, w[i], cap), z[i]);
+          if (SLOPE) d[i] = 4.f * fmaf(-w[i], w[i], w[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        f[j + i] = y[i];
+        if (SLOPE) slope[j + i] = d[i];
+      }
     }
   }
-  __device__ __forceinline__ float of_r(float r) const { return fmaf(-2.f * cap, r, cap); }
-  // one class, whether there is a cap or not: its capped logit, and dy / dz
+  template <int E>
+  __device__ __forceinline__ void cap_logits(float (&f)[E]) const {
+    float none[E];
+    cap_logits<false>(f, none);
+  }
+  // one class, whether there is a cap or not: its capped logit, and dy / dz with the temperature
   __device__ __forceinline__ float capped(float z, float* slope) const {
     *slope = inv_temp;
     if (!(cap > 0.f)) return z;
-    float f[1] = {z};
-    reciprocals(f);
-    *slope *= 4.f * fmaf(-f[0], f[0], f[0]);
-    return of_r(f[0]);
+    float f[1] = {z}, d[1];
+    cap_logits<true>(f, d);
+    *slope *= d[0];
+    return f[0];
   }
   __device__ __forceinline__ float capped(float z) const {
-    float slope;
-    return capped(z, &slope);
+    if (!(cap > 0.f)) return z;
+    float f[1] = {z};
+    cap_logits(f);
+    return f[0];
   }
 };
 
@@ -99,11 +148,6 @@ __device__ __forceinline__ Stats combine(Stats a, Stats b, float c) {
 }
 __device__ __forceinline__ bool no_class(Stats a) { return a.m == -INFINITY && a.s == 0.f; }   // (a NaN makes the sum NaN)
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 template <int E>
 __device__ __forceinline__ float largest(const float (&f)[E]) {
   float mx = f[0];
@@ -111,32 +155,35 @@ __device__ __forceinline__ float largest(const float (&f)[E]) {
   for (int j = 1; j + 1 < E; j += 2) mx = max3(mx, f[j], f[j + 1]);
   return E % 2 ? mx : fmaxf(mx, f[E - 1]);
 }
-constexpr float ABSENT = 1e20f;   // the r of a class that is not there: its exponent is far below any, and finite
-// Adds E classes of logits f with the largest (capped) logit mx, known first so that the exponentials do not wait for one another.  A masked class
-// (-inf) adds nothing: its exponent is kept finite where 0 * infinity would come up.  With CAP f are the classes' r (ABSENT for one that is
-// not there).  Two-wide arithmetic halves the instructions beside the exponentials, which the issue slots are short of at two bytes a class.
+constexpr float ABSENT = -1e30f;   // the capped logit of a class that is not there: far below any, and finite
+// Adds E classes of (capped) logits f with the largest one mx, known first so that the exponentials do not wait for one another.  A masked class (-inf)
+// adds nothing: its exponent is kept finite where 0 * infinity would come up.  CAP: there are no infinities among f.  Two-wide arithmetic halves the
+// instructions beside the exponentials, which the issue slots are short of at two bytes a class.
 template <bool CAP, bool W, int E>
 __device__ __forceinline__ void add_classes(Stats& a, const float (&f)[E], float mx, const Scaling& sc) {
   if (mx > a.m) a = shifted(a, mx, sc.c);
   const float ref = a.m == -INFINITY ? 0.f : a.m;
-  const float t0 = (sc.cap - ref) * sc.c, t1 = -2.f * sc.cap * sc.c;
   float2 s = make_float2(0.f, 0.f), w = s;
 #pragma unroll
   for (int j = 0; j + 1 < E; j += 2) {
-    const float2 x = make_float2(f[j], f[j + 1]);
-    const float2 t = CAP ? fma2(x, make_float2(t1, t1), make_float2(t0, t0))
-                         : mul2(add2(x, make_float2(-ref, -ref)), make_float2(sc.c, sc.c));
+    const float2 t = mul2(add2(make_float2(f[j], f[j + 1]), make_float2(-ref, -ref)), make_float2(sc.c, sc.c));
     const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
     s = add2(s, e);
     if (W) w = fma2(e, CAP ? t : make_float2(fmaxf(t.x, -FLT_MAX), fmaxf(t.y, -FLT_MAX)), w);
   }
   if (E % 2) {
-    const float t = CAP ? fmaf(f[E - 1], t1, t0) : (f[E - 1] - ref) * sc.c, e = exp2_fast(t);
+    const float t = (f[E - 1] - ref) * sc.c, e = exp2_fast(t);
     s.x += e;
     if (W) w.x = fmaf(e, fmaxf(t, -FLT_MAX), w.x);
   }
   a.s += s.x + s.y;
   if (W) a.w += w.x + w.y;
+}
+// ... of capped logits, ABSENT ones among them
+template <bool W, int E>
+__device__ __forceinline__ void add_capped(Stats& a, const float (&f)[E], const Scaling& sc) {
+  const float mx = largest(f);
+  add_classes<true, W, E>(a, f, mx == ABSENT ? -INFINITY : mx, sc);
 }
 // one class of capped logit y
 __device__ __forceinline__ void add_class(Stats& a, float y, const Scaling& sc) {
@@ -152,7 +199,7 @@ __device__ __forceinline__ Stats shuffle_combine(Stats a, int first, float c) {
 }
 static inline Scaling scaling(float softcap, double inv_temp) {
   const double k = softcap > 0.f ? 2.0 * 1.4426950408889634 / (double)softcap : 0.0;
-  return Scaling{softcap, (float)k, (float)(1.4426950408889634 * inv_temp), (float)inv_temp};
+  return Scaling{softcap, softcap > 0.f ? (float)(-1.0 / ((double)softcap * softcap)) : 0.f, (float)k, (float)(1.4426950408889634 * inv_temp), (float)inv_temp};
 }
 
 }  // namespace ob

@@ -1149,7 +1149,7 @@ def _distribution_options(V: int, temperature: float, logit_softcap: Optional[fl
     if not (1e-6 <= temperature <= 1e6):
         raise ValueError(f"temperature must lie between 1e-6 and 1e6, got {temperature}")
     cap = float(logit_softcap or 0.0)
-    if not (cap == 0.0 or 1e-3 <= cap <= 256.0):   # (the kernels' tanh is accurate to some 1e-7 of the cap)
+    if not (cap == 0.0 or 1e-3 <= cap <= 256.0):   # (the range that the kernels are tested in)
         raise ValueError(f"logit_softcap must lie between 1e-3 and 256 (or be None), got {logit_softcap}")
     if V < 1:
         raise ValueError("logits need at least one class")
