@@ -29,6 +29,12 @@ __all__ = [
 ]
 
 
+def _tracked(x: torch.Tensor) -> torch.Tensor:
+    """x as an autograd function may ask ``needs_input_grad`` about it, which does not look at the grad mode: without it a loss that forms
+    its gradients in the forward pass must form none."""
+    return x if torch.is_grad_enabled() else x.detach()
+
+
 def _on_gpu(x: torch.Tensor) -> bool:
     if x.is_cuda:
         if x.dtype != torch.bfloat16:
@@ -1371,7 +1377,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     z = _logit_rows(logits)
     shape = logits.shape[:-1]
     ids, values = _teacher_rows(teacher_ids, teacher_log_probs, shape, logits.device)
-    loss = _DistillationFn.apply(z, ids, values, renormalize, cap, float(temperature), reduction)
+    loss = _DistillationFn.apply(_tracked(z), ids, values, renormalize, cap, float(temperature), reduction)
     return loss.view(shape) if reduction == "none" else loss
 
 
@@ -1604,4 +1610,4 @@ def linear_distillation_loss(x: torch.Tensor, handle, teacher_ids: torch.Tensor,
     shape = x.shape[:-1]
     ids, values = _teacher_rows(teacher_ids, teacher_log_probs, shape, x.device)
     x2 = x.reshape(math.prod(shape), x.shape[-1]).contiguous()
-    return _LinearDistillationFn.apply(x2, handle, ids, values, float(weight), renormalize, cap, float(temperature), int(chunk_rows))
+    return _LinearDistillationFn.apply(_tracked(x2), handle, ids, values, float(weight), renormalize, cap, float(temperature), int(chunk_rows))
