@@ -29,10 +29,10 @@ __all__ = [
 ]
 
 
-def _tracked(x: torch.Tensor) -> torch.Tensor:
-    """x as an autograd function may ask ``needs_input_grad`` about it, which does not look at the grad mode: without it a loss that forms
-    its gradients in the forward pass must form none."""
-    return x if torch.is_grad_enabled() else x.detach()
+def _wants_grad(x: torch.Tensor) -> bool:
+    """Whether a loss that forms its gradients in the forward pass has to: ``needs_input_grad`` inside an autograd function does not look at the grad
+    mode."""
+    return x.requires_grad and torch.is_grad_enabled()
 
 
 def _on_gpu(x: torch.Tensor) -> bool:
@@ -929,13 +929,12 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, x, handle, labels, ignore_index, softcap, z_loss, chunk_rows):
+    def forward(ctx, x, handle, labels, ignore_index, softcap, z_loss, chunk_rows, need_grad):
         shp = x.shape
         d = shp[-1]
         x2 = x.reshape(-1, d)
         lab = labels.reshape(-1)
         V = handle.tp_shape[0]
-        need_grad = bool(ctx.needs_input_grad[0])
         if _on_gpu(x):
             x2 = x2.contiguous()
             lab = lab.contiguous()
@@ -1002,7 +1001,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
     def backward(ctx, dloss, _dz):
         (dx,) = ctx.saved_tensors
         # dloss is 1 for loss.backward(); the weight gradient was already accumulated under that assumption
-        return dx.view(ctx.shape) * dloss.to(dx.dtype), None, None, None, None, None, None
+        return (dx.view(ctx.shape) * dloss.to(dx.dtype),) + (None,) * 7
 
 
 class _VocabParallelLinearCrossEntropyFn(torch.autograd.Function):
@@ -1022,7 +1021,7 @@ class _VocabParallelLinearCrossEntropyFn(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, x, handle, labels, ignore_index, softcap, z_loss, chunk_rows, group, tpc):
+    def forward(ctx, x, handle, labels, ignore_index, softcap, z_loss, chunk_rows, group, tpc, need_grad):
         shp = x.shape
         d = shp[-1]
         x2 = x.reshape(-1, d).contiguous()
@@ -1032,7 +1031,6 @@ class _VocabParallelLinearCrossEntropyFn(torch.autograd.Function):
         M = n * M_l
         V_l = handle.tp_shape[0]
         V, voff = V_l * n, me * V_l
-        need_grad = bool(ctx.needs_input_grad[0])
         dev = x.device
         counts = (lab != ignore_index).sum().to(torch.float32).clamp(min=1).view(1)
         inv_counts = 1.0 / coll.all_gather(counts, group, dim=0)              # [n]
@@ -1116,7 +1114,7 @@ class _VocabParallelLinearCrossEntropyFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dloss, _dz):
         (dx,) = ctx.saved_tensors
-        return dx.view(ctx.shape) * dloss.to(dx.dtype), None, None, None, None, None, None, None, None
+        return (dx.view(ctx.shape) * dloss.to(dx.dtype),) + (None,) * 9
 
 
 def vocab_parallel_linear_cross_entropy(x: torch.Tensor, handle, labels: torch.Tensor, group, tpc=None,
@@ -1125,14 +1123,14 @@ def vocab_parallel_linear_cross_entropy(x: torch.Tensor, handle, labels: torch.T
     """(loss, z_loss) with the head weight ``handle`` split over ``group`` along the vocabulary (``tp_dim = 0``); ``x`` and
     ``labels`` are this member's rows of the sequence-parallel batch.  ``tpc``: the group's ``TPSymmContext`` (GPU)."""
     return _VocabParallelLinearCrossEntropyFn.apply(x, handle, labels, ignore_index, float(logit_softcap or 0.0),
-                                                    float(z_loss_multiplier or 0.0), int(chunk_rows), group, tpc)
+                                                    float(z_loss_multiplier or 0.0), int(chunk_rows), group, tpc, _wants_grad(x))
 
 
 def linear_cross_entropy(x: torch.Tensor, handle, labels: torch.Tensor, ignore_index: int = -100,
                          logit_softcap: float = 0.0, z_loss_multiplier: float = 0.0, chunk_rows: int = 2048):
     """(loss, z_loss) of the LM head fused with the cross entropy; ``handle`` is the ``(vocab, d)`` head weight."""
     return _LinearCrossEntropyFn.apply(x, handle, labels, ignore_index, float(logit_softcap or 0.0),
-                                       float(z_loss_multiplier or 0.0), int(chunk_rows))
+                                       float(z_loss_multiplier or 0.0), int(chunk_rows), _wants_grad(x))
 
 
 # ----------------------------------------------------------------------------------------------------------------------
@@ -1313,10 +1311,9 @@ class _DistillationFn(torch.autograd.Function):
     """Row losses, or their sum / mean over the rows with a teacher."""
 
     @staticmethod
-    def forward(ctx, z, ids, values, renormalize, cap, temperature, reduction):
+    def forward(ctx, z, ids, values, renormalize, cap, temperature, reduction, keep):
         ctx.options = (renormalize, cap, temperature, reduction)
         rows, k = ids.shape
-        keep = ctx.needs_input_grad[0]
         if z.is_cuda:
             work = K.distill_work(rows, k, z.device)
             loss = torch.empty(rows if reduction == "none" else (), dtype=torch.float32, device=z.device)
@@ -1339,7 +1336,7 @@ class _DistillationFn(torch.autograd.Function):
         _refuse_double_backward()
         renormalize, cap, temperature, reduction = ctx.options
         if not ctx.needs_input_grad[0]:
-            return (None,) * 7
+            return (None,) * 8
         z, ids = ctx.saved_tensors[:2]
         rows = z.shape[0]
         if z.is_cuda:
@@ -1351,7 +1348,7 @@ class _DistillationFn(torch.autograd.Function):
             values, inv = ctx.saved_tensors[2:]
             d = ref.distillation_bwd(z, ids, values, g if reduction == "none" else (g * inv).expand(rows), renormalize, cap,
                                      temperature)
-        return d, None, None, None, None, None, None
+        return (d,) + (None,) * 7
 
 
 def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, *,
@@ -1377,7 +1374,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     z = _logit_rows(logits)
     shape = logits.shape[:-1]
     ids, values = _teacher_rows(teacher_ids, teacher_log_probs, shape, logits.device)
-    loss = _DistillationFn.apply(_tracked(z), ids, values, renormalize, cap, float(temperature), reduction)
+    loss = _DistillationFn.apply(z, ids, values, renormalize, cap, float(temperature), reduction, _wants_grad(z))
     return loss.view(shape) if reduction == "none" else loss
 
 
@@ -1551,8 +1548,7 @@ class _LinearDistillationFn(torch.autograd.Function):
     ``weight`` is the factor of this loss in the objective."""
 
     @staticmethod
-    def forward(ctx, x2, handle, ids, values, weight, renormalize, cap, temperature, chunk_rows):
-        need_grad = bool(ctx.needs_input_grad[0])
+    def forward(ctx, x2, handle, ids, values, weight, renormalize, cap, temperature, chunk_rows, need_grad):
         M, V = x2.shape[0], handle.tp_shape[0]
         if _on_gpu(x2):
             dev = x2.device
@@ -1594,7 +1590,7 @@ class _LinearDistillationFn(torch.autograd.Function):
         _refuse_double_backward()
         (dx,) = ctx.saved_tensors
         # g is 1 for loss.backward(); the weight gradient was already accumulated under that assumption
-        return (dx * g.to(dx.dtype),) + (None,) * 8
+        return (dx * g.to(dx.dtype),) + (None,) * 9
 
 
 def linear_distillation_loss(x: torch.Tensor, handle, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, *,
@@ -1610,4 +1606,4 @@ def linear_distillation_loss(x: torch.Tensor, handle, teacher_ids: torch.Tensor,
     shape = x.shape[:-1]
     ids, values = _teacher_rows(teacher_ids, teacher_log_probs, shape, x.device)
     x2 = x.reshape(math.prod(shape), x.shape[-1]).contiguous()
-    return _LinearDistillationFn.apply(_tracked(x2), handle, ids, values, float(weight), renormalize, cap, float(temperature), int(chunk_rows))
+    return _LinearDistillationFn.apply(x2, handle, ids, values, float(weight), renormalize, cap, float(temperature), int(chunk_rows), _wants_grad(x2))
