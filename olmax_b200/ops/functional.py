@@ -17,6 +17,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.distributed as dist
+from torch.autograd import forward_ad
 
 from . import kernels as K
 from ..parallel import collectives as coll
@@ -1195,6 +1196,13 @@ def _upstream(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return g.reshape(-1) if g.dim() > 1 else g
 
 
+def _refuse_forward_mode(x: torch.Tensor) -> None:
+    """The kernels see values alone: without an autograd function around them a tangent would be lost without a word, with one it is refused after the
+    kernels have run."""
+    if forward_ad.unpack_dual(x).tangent is not None:
+        raise NotImplementedError("log probabilities and distillation losses have no forward-mode derivative")
+
+
 def _refuse_double_backward() -> None:
     """The gradients below are kernels' results, not functions of the upstream gradient that autograd could go through again (grad mode is
     only on in a backward pass with ``create_graph``)."""
@@ -1258,13 +1266,14 @@ def token_log_probs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, *,
     * ``top_k`` > 0 (at most 128, or the number of classes): log p and class of the largest logits, largest first, equal ones in the order of their
       classes.
 
-    ``log_probs`` and ``entropy`` are differentiable with respect to the logits, the top classes are not.  Masked classes
+    ``log_probs`` and ``entropy`` are differentiable (once, in reverse mode) with respect to the logits, the top classes are not.  Masked classes
     (-inf) have no part; a row without any class has log p = -inf, entropy 0 and gradient 0; NaN in a row gives NaN.
     """
     cap = _distribution_options(logits.shape[-1] if logits.dim() else 0, temperature, logit_softcap, top_k, ignore_index)
     z = _logit_rows(logits)
     shape = logits.shape[:-1]
     lab = _token_rows(ids, shape, logits.device) if ids is not None else None
+    _refuse_forward_mode(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         out = _TokenLogProbsFn.apply(z, lab, int(top_k), int(ignore_index), cap, float(temperature))
     else:
@@ -1374,6 +1383,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     z = _logit_rows(logits)
     shape = logits.shape[:-1]
     ids, values = _teacher_rows(teacher_ids, teacher_log_probs, shape, logits.device)
+    _refuse_forward_mode(logits)
     loss = _DistillationFn.apply(z, ids, values, renormalize, cap, float(temperature), reduction, _wants_grad(z))
     return loss.view(shape) if reduction == "none" else loss
 
@@ -1535,6 +1545,7 @@ def linear_token_log_probs(x: torch.Tensor, handle, ids: Optional[torch.Tensor] 
     cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap, top_k, ignore_index)
     shape = x.shape[:-1]
     lab = _token_rows(ids, shape, x.device) if ids is not None else None
+    _refuse_forward_mode(x)
     x2 = (x if x.dim() == 2 else x.reshape(math.prod(shape), x.shape[-1])).contiguous()
     args = (x2, handle, lab, int(top_k), int(ignore_index), cap, float(temperature), int(chunk_rows))
     if x.requires_grad and torch.is_grad_enabled():
@@ -1605,5 +1616,6 @@ def linear_distillation_loss(x: torch.Tensor, handle, teacher_ids: torch.Tensor,
         raise ValueError(f"weight must be finite, got {weight}")
     shape = x.shape[:-1]
     ids, values = _teacher_rows(teacher_ids, teacher_log_probs, shape, x.device)
+    _refuse_forward_mode(x)
     x2 = x.reshape(math.prod(shape), x.shape[-1]).contiguous()
     return _LinearDistillationFn.apply(x2, handle, ids, values, float(weight), renormalize, cap, float(temperature), int(chunk_rows), _wants_grad(x2))

@@ -1,0 +1,55 @@
+"""How the kernels over the LM head's distribution are called: grad mode, forward-mode derivatives, upstream factors, repeated teachers, masks."""
+
+import math
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+pytestmark = pytest.mark.gpu
+
+from olmax_b200.nn import LMHead
+from olmax_b200.nn.module import build_module
+from olmax_b200.ops import functional as F
+from olmax_b200.ops import kernels as K
+from olmax_b200.parallel import MeshResource
+from olmax_b200.testing.token_probs import distillation_64, scores_64
+
+DEV = "cuda"
+
+
+def _head(V=512, d=64, cap=None):
+    return build_module(lambda: LMHead(d, V, logit_softcap=cap), mesh_resource=MeshResource.FSDP(1), device=torch.device(DEV))
+
+
+def _inputs(rows=24, V=512, d=64, k=3, seed=1):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(rows, d, generator=g, device=DEV).to(torch.bfloat16)
+    t = torch.randn(rows, V, generator=g, device=DEV).log_softmax(-1).topk(k, dim=-1)
+    return x, t.indices, t.values
+
+
+def test_losses_without_grad_mode_leave_no_gradient():
+    head = _head()
+    x, ids, t = _inputs()
+    x.requires_grad_(True)
+    labels = torch.arange(24, device=DEV)
+    for call in (lambda: head.distillation_loss(x, ids, t), lambda: head.loss(x, labels)[0]):
+        with torch.no_grad():
+            loss = call()
+        assert not loss.requires_grad and float(head.store.grad.abs().max()) == 0
+        assert torch.equal(call().detach(), loss) and float(head.store.grad.abs().max()) > 0
+        head.store.zero_grad()
+
+
+def test_forward_mode_derivatives_reach_no_kernel():
+    head = _head()
+    x, ids, t = _inputs()
+    z, lab = torch.randn(24, 512, device=DEV), torch.zeros(24, dtype=torch.int64, device=DEV)
+    before = K.launch_count()
+    for mode in (torch.no_grad, torch.enable_grad):
+        for call in (lambda z, x: F.token_log_probs(z, lab), lambda z, x: head.token_log_probs(x, lab), lambda z, x: F.distillation_loss(z, ids, t),
+                     lambda z, x: head.distillation_loss(x, ids, t)):
+            with mode(), forward_ad.dual_level(), pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(z, torch.ones_like(z)), forward_ad.make_dual(x, torch.ones_like(x)))
+    assert K.launch_count() == before

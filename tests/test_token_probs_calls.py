@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from olmax_b200.nn import LMHead
 from olmax_b200.nn.module import build_module
@@ -30,3 +31,21 @@ def test_a_distillation_loss_without_grad_mode_leaves_no_gradient():
     assert not loss.requires_grad and float(head.store.grad.abs().max()) == 0
     again = head.distillation_loss(x, ids, t)
     assert torch.equal(again.detach(), loss) and float(head.store.grad.abs().max()) > 0
+
+
+def test_forward_mode_derivatives_are_refused():
+    """By all of them alike, in either grad mode; a tangent that a kernel never saw would read as zero."""
+    head = _head()
+    x, ids, t = _inputs()
+    x = x.detach()
+    z = torch.randn(6, 40)
+    lab = torch.zeros(6, dtype=torch.int64)
+    for mode in (torch.no_grad, torch.enable_grad):
+        for call in (lambda z, x: F.token_log_probs(z, lab), lambda z, x: F.token_log_probs(z, top_k=2), lambda z, x: head.token_log_probs(x, lab),
+                     lambda z, x: F.distillation_loss(z, ids, t), lambda z, x: head.distillation_loss(x, ids, t)):
+            with mode(), forward_ad.dual_level():
+                with pytest.raises(NotImplementedError):
+                    call(forward_ad.make_dual(z, torch.ones_like(z)), forward_ad.make_dual(x, torch.ones_like(x)))
+                call(z, x)                       # no tangent, no refusal
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda z: F.token_log_probs(z, lab).log_probs, (z,), (torch.ones_like(z),))
