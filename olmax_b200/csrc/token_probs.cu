@@ -919,6 +919,7 @@ __global__ void __launch_bounds__(1024)
     for (int i = 0; i < k && !any; ++i) {
       const long long id = teacher_id(teacher_ids, ids_64, r * ld_t + i);
       any = id >= 0 && id < V && !(renormalize && teacher_log_probs[r * ld_t + i] == -INFINITY);
+      for (int j = 0; j < i && any && renormalize; ++j) any = teacher_id(teacher_ids, ids_64, r * ld_t + j) != id;   // (the first of a class counts)
     }
     n += any;
   }

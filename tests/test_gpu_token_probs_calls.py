@@ -53,3 +53,35 @@ def test_forward_mode_derivatives_reach_no_kernel():
             with mode(), forward_ad.dual_level(), pytest.raises(NotImplementedError):
                 call(forward_ad.make_dual(z, torch.ones_like(z)), forward_ad.make_dual(x, torch.ones_like(x)))
     assert K.launch_count() == before
+
+
+@pytest.mark.parametrize("int_type", [torch.int64, torch.int32])
+def test_a_repeated_class_whose_first_pair_is_nothing_is_no_teacher(int_type):
+    """Of several pairs with one id the first counts; renormalised, a row with none above -inf has no teacher and does not enter the mean, neither
+    the loss's nor the gradient's, which are divided by counts of their own."""
+    head = _head()
+    x, ids, t = _inputs(rows=24)
+    ids[::3, 1] = ids[::3, 0]
+    ids[::3, 2] = -1
+    t[::3, 0], t[::3, 1] = -math.inf, -1.0                 # the second pair of these rows does not count
+    ids[1, 2], t[1, 0] = ids[1, 1], -math.inf              # here the second does, the third does not
+    results = []
+    for blank in (False, True):
+        i2 = ids.clone()
+        if blank:
+            i2[::3] = -1
+        leaf = x.clone().requires_grad_(True)
+        head.store.zero_grad()
+        loss = head.distillation_loss(leaf, i2.to(int_type), t, tail="renormalize")
+        dx, = torch.autograd.grad(loss, leaf)
+        results.append((loss.detach(), dx, head.store.full_gradient("proj.weight").clone()))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    z = x.double() @ head.weight.full().double().t()
+    want, dz = distillation_64(z, ids, t, "renormalize")
+    # logits of 64 exact products each, off by less than 64 * 2^-24 of the sum of their absolute values; statistics and logarithms some steps of 2^-24
+    e = 2.0 ** -24 * (2 * 64 * float((x.double().abs() @ head.weight.full().double().abs().t()).max()) + 64)
+    assert abs(float(results[0][0]) - float(want)) <= e * 4
+    w = head.weight.full().double()
+    size = dz.abs() @ w.abs()
+    assert torch.all((results[0][1].double() - dz @ w).abs() <= (2.0 ** -8 + 2.0 ** -12 + 4 * e) * size + 2.0 ** -8 * (dz @ w).abs() + 1e-12)
