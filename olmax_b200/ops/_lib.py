@@ -172,7 +172,7 @@ _STATUS: dict = {}
 
 
 def status_buffer(device: torch.device) -> torch.Tensor:
-    """Per-device int32[4] that kernels write when a bounded wait runs out (all zero = healthy)."""
+    """Per-device int32[4] that kernels write when a bounded wait runs out, and :func:`report_where` (all zero = healthy)."""
     key = (device.type, device.index if (device.index is not None or device.type != "cuda") else torch.cuda.current_device())
     buf = _STATUS.get(key)
     if buf is None:
@@ -181,7 +181,14 @@ def status_buffer(device: torch.device) -> torch.Tensor:
     return buf
 
 
-_STATUS_NAMES = {1: "mbarrier wait timed out", 2: "peer flag wait timed out", 3: "bad argument"}
+STATUS_SCALED_LOSS = 4
+_STATUS_NAMES = {1: "mbarrier wait timed out", 2: "peer flag wait timed out", 3: "bad argument",
+                 STATUS_SCALED_LOSS: "a distillation loss through the head back-propagated with a factor other than 1 (pass it as weight)"}
+
+
+def report_where(bad: torch.Tensor, code: int) -> None:
+    """Put ``code`` into the status word of ``bad``'s device if that device scalar is true, without waiting for it."""
+    status_buffer(bad.device)[:1].masked_fill_(bad, code)
 
 
 def raise_for_status(vals) -> None:

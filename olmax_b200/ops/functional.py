@@ -19,6 +19,7 @@ import torch
 import torch.distributed as dist
 from torch.autograd import forward_ad
 
+from . import _lib
 from . import kernels as K
 from ..parallel import collectives as coll
 from . import reference as ref
@@ -1601,6 +1602,11 @@ class _LinearDistillationFn(torch.autograd.Function):
         _refuse_double_backward()
         (dx,) = ctx.saved_tensors
         # g is 1 for loss.backward(); the weight gradient was already accumulated under that assumption
+        if g.is_cuda:
+            _lib.report_where(g != 1, _lib.STATUS_SCALED_LOSS)
+        elif not bool(g == 1):
+            raise RuntimeError("a distillation loss through the head was back-propagated with a factor other than 1, which the weight's gradient "
+                               "cannot follow any more: pass it as weight")
         return (dx * g.to(dx.dtype),) + (None,) * 9
 
 
@@ -1609,7 +1615,8 @@ def linear_distillation_loss(x: torch.Tensor, handle, teacher_ids: torch.Tensor,
                              logit_softcap: Optional[float] = None, chunk_rows: int = 2048) -> torch.Tensor:
     """``weight`` times the mean :func:`distillation_loss` of the LM head ``x @ W^T``, whose logits exist ``chunk_rows`` rows at a
     time.  As with :func:`linear_cross_entropy` the weight's gradient is accumulated in the forward pass: add the loss to others as
-    it is and scale it with ``weight``."""
+    it is and scale it with ``weight``.  A backward pass with another factor is an error: at once on a CPU, on a GPU in the status word
+    that :func:`~olmax_b200.ops._lib.check_status` and the trainer look at."""
     cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap)
     renormalize = _check_tail(tail)
     if not math.isfinite(weight):

@@ -85,3 +85,19 @@ def test_a_repeated_class_whose_first_pair_is_nothing_is_no_teacher(int_type):
     w = head.weight.full().double()
     size = dz.abs() @ w.abs()
     assert torch.all((results[0][1].double() - dz @ w).abs() <= (2.0 ** -8 + 2.0 ** -12 + 4 * e) * size + 2.0 ** -8 * (dz @ w).abs() + 1e-12)
+
+
+def test_a_scaled_distillation_loss_of_the_head_is_reported():
+    """As on the CPU, but without waiting for the GPU: in the kernels' status word, which the trainer reads every step."""
+    from olmax_b200.ops import _lib
+
+    head = _head()
+    x, ids, t = _inputs()
+    x.requires_grad_(True)
+    _lib.check_status()
+    (head.distillation_loss(x, ids, t, weight=0.5) + 3 * x.float().square().mean()).backward()
+    _lib.check_status()
+    (0.5 * head.distillation_loss(x, ids, t)).backward()
+    with pytest.raises(_lib.KernelError, match="factor"):
+        _lib.check_status()
+    _lib.check_status()                                    # told once

@@ -49,3 +49,23 @@ def test_forward_mode_derivatives_are_refused():
                 call(z, x)                       # no tangent, no refusal
     with pytest.raises(NotImplementedError):
         torch.func.jvp(lambda z: F.token_log_probs(z, lab).log_probs, (z,), (torch.ones_like(z),))
+
+
+def test_a_scaled_distillation_loss_of_the_head_is_refused():
+    """The weight's gradient is formed in the forward pass: a factor behind it would scale one of the two gradients alone."""
+    head = _head()
+    x, ids, t = _inputs()
+    for factor in (0.5, 0.0, math.nan):
+        loss = head.distillation_loss(x, ids, t)
+        with pytest.raises(RuntimeError):
+            (factor * loss).backward()
+        assert x.grad is None
+    head.store.zero_grad()
+    other = x.square().mean()
+    (head.distillation_loss(x, ids, t, weight=0.5) + 3 * other).backward()      # a factor of the other loss is none of its own
+    half = [x.grad - 6 * x.detach() / x.numel(), head.store.full_gradient("proj.weight").clone()]
+    head.store.zero_grad()
+    whole, = torch.autograd.grad(head.distillation_loss(x, ids, t), x)
+    # (a few roundings of terms below 1: the mean's, the weight's, the sum's)
+    assert float((half[0] - 0.5 * whole).abs().max()) < 8 * 2.0 ** -24
+    assert float((half[1] - 0.5 * head.store.full_gradient("proj.weight")).abs().max()) < 8 * 2.0 ** -24
