@@ -34,7 +34,7 @@ import torch.distributed as dist
 from .. import fs, utils
 from ..checkpoint.utils import AsyncSaveHandle
 from ..data.data_loader import DataLoader
-from ..exceptions import CallbackExistsError
+from ..exceptions import CallbackExistsError, OLMaxConfigurationError
 from ..optim.config import OptimConfig
 from ..parallel import dist_utils
 from ..parallel.mesh import MeshResource
@@ -71,7 +71,8 @@ class Trainer:
     optim: OptimConfig
     loss_fun: Optional[Callable[[Any, Any, Any], torch.Tensor]] = None
     """``loss_fun(model, micro_batch, buffer_cache) -> scalar``; default: ``model(ids, labels, cache)[0]`` for a micro-batch of
-    two tensors, ``model.distillation_loss(ids, teacher_ids, teacher_log_probs, cache)`` for one of three."""
+    two tensors, ``model.distillation_loss(ids, teacher_ids, teacher_log_probs, cache)`` for one of three (without a z-loss, at temperature 1
+    with the rest of the vocabulary as one class: a function of your own passes ``temperature``, ``tail`` and ``weight``)."""
     mesh: Optional[MeshResource] = None
     grad_dtype: str = "float32"
     compute_dtype: str = "bfloat16"
@@ -285,6 +286,9 @@ class Trainer:
     # ------------------------------------------------------------------ the optimizer step
     def _default_loss(self, model, micro_batch, cache):
         if len(micro_batch) == 3:
+            if self.z_loss_multiplier:
+                raise OLMaxConfigurationError("the distillation loss of a micro-batch with a teacher has no z-loss: leave z_loss_multiplier at 0, or "
+                                              "give a loss_fun")
             ids, teacher_ids, teacher_log_probs = micro_batch
             return model.distillation_loss(ids, teacher_ids, teacher_log_probs, cache)
         ids, labels = micro_batch

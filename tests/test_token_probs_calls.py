@@ -6,6 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from olmax_b200.exceptions import OLMaxConfigurationError
 from olmax_b200.nn import LMHead
 from olmax_b200.nn.module import build_module
 from olmax_b200.ops import functional as F
@@ -69,3 +70,25 @@ def test_a_scaled_distillation_loss_of_the_head_is_refused():
     # (a few roundings of terms below 1: the mean's, the weight's, the sum's)
     assert float((half[0] - 0.5 * whole).abs().max()) < 8 * 2.0 ** -24
     assert float((half[1] - 0.5 * head.store.full_gradient("proj.weight")).abs().max()) < 8 * 2.0 ** -24
+
+
+def test_the_trainer_refuses_a_z_loss_beside_a_teacher(tmp_path):
+    """The distillation loss has no z-loss: a multiplier that would be dropped is refused."""
+    from olmax_b200.models import DefaultTransformerConfig, DefaultTransformerLayerConfig
+    from olmax_b200.nn import MultiheadSelfAttentionConfig
+    from olmax_b200.optim import AdamWConfig, ConstantSchedule
+    from olmax_b200.train import Trainer
+
+    cfg = DefaultTransformerConfig(vocab_size=64, d_model=64, hidden_size=96, num_layers=1,
+                                   layer=DefaultTransformerLayerConfig(attention=MultiheadSelfAttentionConfig(n_heads=4, head_dim=16)))
+    model = cfg.build(seed=0, mesh_resource=MeshResource.FSDP(1), device=torch.device("cpu"))
+    ids = torch.randint(0, 64, (2, 12), generator=torch.Generator().manual_seed(5))
+    with torch.no_grad():
+        best = model.token_log_probs(ids, top_k=4)
+    trainer = Trainer(work_dir=tmp_path, save_folder=tmp_path, optim=AdamWConfig(lr=ConstantSchedule(1e-2)), z_loss_multiplier=1e-4)
+    trainer.setup(model, 1)
+    with pytest.raises(OLMaxConfigurationError):
+        trainer.train_batch([(ids, best.top_ids, best.top_log_probs)])
+    trainer.train_batch([(ids, ids)])
+    trainer.z_loss_multiplier = 0.0
+    trainer.train_batch([(ids, best.top_ids, best.top_log_probs)])
