@@ -1268,7 +1268,8 @@ def token_log_probs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, *,
       classes.
 
     ``log_probs`` and ``entropy`` are differentiable (once, in reverse mode) with respect to the logits, the top classes are not.  Masked classes
-    (-inf) have no part; a row without any class has log p = -inf, entropy 0 and gradient 0; NaN in a row gives NaN.
+    (-inf) have no part; a row without any class has log p = -inf, entropy 0 and gradient 0; NaN in a row gives NaN.  A soft-cap knows no masks:
+    ``cap * tanh(-inf / cap)`` is ``-cap``, so logits are to be capped before they are masked, and given without ``logit_softcap``.
     """
     cap = _distribution_options(logits.shape[-1] if logits.dim() else 0, temperature, logit_softcap, top_k, ignore_index)
     z = _logit_rows(logits)

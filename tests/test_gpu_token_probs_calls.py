@@ -101,3 +101,21 @@ def test_a_scaled_distillation_loss_of_the_head_is_reported():
     with pytest.raises(_lib.KernelError, match="factor"):
         _lib.check_status()
     _lib.check_status()                                    # told once
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [7, 1003, 40000])
+def test_masked_classes_under_a_soft_cap(V, dtype):
+    """-cap, as the formula has it: in whole vectors and single classes, of rows of one CTA and of several."""
+    cap = 5.0
+    z = (torch.randn(4, V, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV) * 3).to(dtype)
+    z[0, 1::2], z[1, V // 2:], z[2], z[3, :1] = -math.inf, -math.inf, -math.inf, math.inf
+    ids = torch.tensor([1, V - 1, 0, 0], device=DEV)
+    k = min(V, 9)
+    out = F.token_log_probs(z, ids, top_k=k, logit_softcap=cap)
+    lp, ent, top, top_ids = scores_64(z, ids, k, 1.0, cap)
+    # steps of 2^-24: a log p is at most 2 cap + log V and off by 24 |y| + 16; the sum of V terms of a CTA of 256 threads by V / 256 + 32
+    tol = 2.0 ** -24 * (24 * cap + 16 + V / 256 + 32 + 4 * (2 * cap + math.log(V)))
+    assert torch.equal(out.top_ids, top_ids)
+    for a, b in ((out.log_probs, lp), (out.entropy, ent), (out.top_log_probs, top)):
+        assert float((a.double() - b).abs().max()) <= tol * (1 + math.log(V))

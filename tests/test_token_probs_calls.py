@@ -11,6 +11,7 @@ from olmax_b200.nn import LMHead
 from olmax_b200.nn.module import build_module
 from olmax_b200.ops import functional as F
 from olmax_b200.parallel import MeshResource
+from olmax_b200.testing.token_probs import scores_64
 
 
 def _head(V=40, d=16, cap=None):
@@ -92,3 +93,17 @@ def test_the_trainer_refuses_a_z_loss_beside_a_teacher(tmp_path):
     trainer.train_batch([(ids, ids)])
     trainer.z_loss_multiplier = 0.0
     trainer.train_batch([(ids, best.top_ids, best.top_log_probs)])
+
+
+def test_a_soft_cap_makes_a_masked_class_one_of_the_lowest():
+    """cap tanh(-inf / cap) = -cap: the formula has no masks, and the documentation says so."""
+    z = torch.tensor([[1.0, 2.0, -math.inf], [-math.inf] * 3])
+    out = F.token_log_probs(z, torch.tensor([2, 0]), top_k=3, logit_softcap=5.0)
+    lp, ent, top, top_ids = scores_64(z, torch.tensor([2, 0]), 3, 1.0, 5.0)
+    assert torch.allclose(out.log_probs.double(), lp, atol=2e-6) and torch.allclose(out.entropy.double(), ent, atol=2e-6)
+    assert torch.allclose(out.top_log_probs.double(), top, atol=2e-6) and torch.equal(out.top_ids, top_ids)
+    assert abs(float(out.log_probs[1]) + math.log(3)) < 2e-6
+    # a mask that holds: cap the logits first
+    y = torch.where(z == -math.inf, z, 5.0 * torch.tanh(z / 5.0))
+    masked = F.token_log_probs(y, torch.tensor([2, 0]))
+    assert masked.log_probs[0] == -math.inf and masked.log_probs[1] == -math.inf and masked.entropy[1] == 0
