@@ -76,7 +76,8 @@ class LMHead(Module):
     def token_log_probs(self, x: torch.Tensor, ids: Optional[torch.Tensor] = None, *, top_k: int = 0, temperature: float = 1.0,
                         ignore_index: int = -100, chunk_rows: int = 2048) -> F.TokenLogProbs:
         """Log probabilities of tokens, entropies and top classes of hidden states x ``[..., d]``
-        (:func:`~olmax_b200.ops.functional.linear_token_log_probs`), differentiable with respect to x and the head's weight."""
+        (:func:`~olmax_b200.ops.functional.linear_token_log_probs`), differentiable with respect to x and, where x has
+        ``requires_grad``, the head's weight."""
         self._refuse_vocab_parallel("token_log_probs")
         return F.linear_token_log_probs(x, self._weight, ids, top_k=top_k, temperature=temperature, logit_softcap=self.logit_softcap,
                                         ignore_index=ignore_index, chunk_rows=chunk_rows)

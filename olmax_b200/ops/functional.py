@@ -1542,8 +1542,9 @@ def linear_token_log_probs(x: torch.Tensor, handle, ids: Optional[torch.Tensor] 
                            temperature: float = 1.0, logit_softcap: Optional[float] = None, ignore_index: int = -100,
                            chunk_rows: int = 2048) -> TokenLogProbs:
     """:func:`token_log_probs` of the LM head ``x @ W^T`` (``handle``: the ``(vocab, d)`` weight, x ``[..., d]``), whose logits are
-    never formed: their statistics come out of the GEMM's epilogue.  With ``top_k``, and in the backward pass (it is differentiable
-    with respect to x and the weight), they exist ``chunk_rows`` rows at a time."""
+    never formed: their statistics come out of the GEMM's epilogue.  With ``top_k``, and in the backward pass, they exist
+    ``chunk_rows`` rows at a time.  It is differentiable with respect to x and the weight, which is no tensor of autograd's: its gradient is
+    accumulated in the backward pass of x, so that x has to have ``requires_grad`` for either."""
     cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap, top_k, ignore_index)
     shape = x.shape[:-1]
     lab = _token_rows(ids, shape, x.device) if ids is not None else None
@@ -1615,9 +1616,9 @@ def linear_distillation_loss(x: torch.Tensor, handle, teacher_ids: torch.Tensor,
                              weight: float = 1.0, temperature: float = 1.0, tail: str = "rest",
                              logit_softcap: Optional[float] = None, chunk_rows: int = 2048) -> torch.Tensor:
     """``weight`` times the mean :func:`distillation_loss` of the LM head ``x @ W^T``, whose logits exist ``chunk_rows`` rows at a
-    time.  As with :func:`linear_cross_entropy` the weight's gradient is accumulated in the forward pass: add the loss to others as
-    it is and scale it with ``weight``.  A backward pass with another factor is an error: at once on a CPU, on a GPU in the status word
-    that :func:`~olmax_b200.ops._lib.check_status` and the trainer look at."""
+    time.  As with :func:`linear_cross_entropy` the weight's gradient is accumulated in the forward pass (where x has
+    ``requires_grad``, else neither gets one): add the loss to others as it is and scale it with ``weight``.  A backward pass with another factor
+    is an error: at once on a CPU, on a GPU in the status word that :func:`~olmax_b200.ops._lib.check_status` and the trainer look at."""
     cap = _distribution_options(handle.tp_shape[0], temperature, logit_softcap)
     renormalize = _check_tail(tail)
     if not math.isfinite(weight):

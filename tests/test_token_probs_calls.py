@@ -107,3 +107,14 @@ def test_a_soft_cap_makes_a_masked_class_one_of_the_lowest():
     y = torch.where(z == -math.inf, z, 5.0 * torch.tanh(z / 5.0))
     masked = F.token_log_probs(y, torch.tensor([2, 0]))
     assert masked.log_probs[0] == -math.inf and masked.log_probs[1] == -math.inf and masked.entropy[1] == 0
+
+
+def test_the_heads_weight_gets_a_gradient_when_the_hidden_states_do():
+    """As with the cross entropy: hidden states without requires_grad are scored, and nothing is recorded of the weight."""
+    head = _head()
+    x, ids, t = _inputs()
+    for call in (lambda x: head.token_log_probs(x, ids[:, 0]).log_probs.sum(), lambda x: head.distillation_loss(x, ids, t), lambda x: head.loss(x, ids[:, 0])[0]):
+        assert not call(x.detach()).requires_grad and float(head.store.grad.abs().max()) == 0
+        call(x).backward()
+        assert float(head.store.grad.abs().max()) > 0
+        head.store.zero_grad()
