@@ -289,8 +289,9 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, unsigned long long 
 // loads in flight (AHEAD: those of the next batch) and takes the maximum of the batch before its exponentials.
 // Top classes in the same pass, at one comparison per thread and batch: a group (TopWork) is kept if its largest logit is above `cut`, a
 // lower bound of the row's k-th largest logit that k classes of earlier batches reach, so that no class of a later one at the bound is among the
-// first k.  The bound is the k-th largest of the threads' maxima so far, which no more than 1.2 k classes reach if they are spread over the
-// threads by chance; it is looked for at the first batch, whenever STEP more groups have come together, and at the end if there are many.  Then the
+// first k.  The bound is the k-th largest of the threads' maxima so far, which some 256 ln(256 / (256 - k)) classes reach if they are spread over
+// the threads by chance (1.15 k at 64, 1.4 k at 128; more by the bound's upper 16 bits only, and any number in a bad order: more than CLASSES are
+// sorted out exactly); it is looked for at the first batch, whenever STEP more groups have come together, and at the end if there are many.  Then the
 // classes of the groups above it are read again and put in order.
 // Bound by HBM in fp32 (2048 x 100352: 132 us, 6.2 TB/s), by loads and the special-function unit in bf16 (80 us, 5.1 TB/s), by instructions with a
 // soft-cap (118 us; 184 us where an eighth of the logits lie beyond 3/4 of the cap); the 64 top classes add 42 us to the first (instructions and barriers of the selection).
