@@ -113,3 +113,27 @@ def test_capped_logits_out_of_the_heads_epilogue(rows):
         out = head.token_log_probs(x, ids)
     _close(out.log_probs, lp, _tol(3.0))
     _close(out.entropy, ent, 2 * _tol(3.0))
+
+
+@pytest.mark.parametrize("V,k,temperature,cap,dtype", [(50257, 16, 2.0, 0.0, torch.float32), (100352, 64, 2.0, 0.0, torch.float32), (32000, 8, 3.0, 0.0, torch.float32),
+                                                       (256000, 128, 2.0, 0.0, torch.bfloat16), (100352, 64, 2.0, 30.0, torch.bfloat16)])
+@pytest.mark.parametrize("rows", [2, 64, 200])
+def test_a_small_distillation_loss(rows, V, k, temperature, cap, dtype):
+    """
+    A student near its teacher, most of whose mass P (the teacher's: Q) is the rest's.  The loss is a difference of logarithms of sums, of which the rest's
+    is a part of the whole: an error e of the rest's sum counts (1 - P) - (1 - Q) times, one of the named classes' sum P times.  e: the exponential is off by
+    2.4 steps, its exponent (|t| <= 12 where the mass lies) by 2.5 ln 2 |t| = 21; a thread adds 16 terms a batch, V / 4096 batches, 256 threads in a tree:
+    8 + V / 4096 + 8.  The logits of named classes enter in 64 bits, capped ones off by 4 steps of |y| / T.
+    """
+    g = torch.Generator(device=DEV).manual_seed(3)
+    z = (torch.randn(rows, V, generator=g, device=DEV) * 2).to(dtype)
+    y = z.double() + 0.1 * torch.randn(rows, V, generator=g, device=DEV)
+    y = cap * torch.tanh(y / cap) if cap else y
+    t = torch.log_softmax(y / temperature, -1).topk(k, -1)
+    ids, values = t.indices, t.values.float()
+    loss = F.distillation_loss(z, ids, values, temperature=temperature, logit_softcap=cap, reduction="none")
+    want, _ = distillation_64(z, ids, values, "rest", "none", temperature, cap)
+    ys = (cap * torch.tanh(z.double() / cap) if cap else z.double()) / temperature
+    named = torch.log_softmax(ys, -1).gather(1, ids).exp().sum(1) + values.double().exp().sum(1)
+    e = STEP * (2.4 + 21 + 16 + V / 4096 + (4 * float(ys.abs().max()) if cap else 0))
+    _close(loss, want, e * named + 2 * STEP * want)
