@@ -38,7 +38,8 @@ def test_losses_without_grad_mode_leave_no_gradient():
         with torch.no_grad():
             loss = call()
         assert not loss.requires_grad and float(head.store.grad.abs().max()) == 0
-        assert torch.equal(call().detach(), loss) and float(head.store.grad.abs().max()) > 0
+        # (the cross entropy adds its 24 rows in any order: 24 roundings of the sum)
+        assert abs(float(call().detach()) - float(loss)) <= 24 * 2.0 ** -24 * abs(float(loss)) and float(head.store.grad.abs().max()) > 0
         head.store.zero_grad()
 
 
