@@ -160,8 +160,11 @@ class SymmContext:
         # published that its stores of that unit are done.  The fold of unit u is deferred to the moment unit u-1 (the
         # next one in backward order) has been computed: [wgrads(u-1)] -> wait(u) -> fold(u) -> publish(u-1), so the
         # wait finds the others' epoch already there unless they lag by more than a whole unit.  Three buffers rotate
-        # (index % 3): a buffer is written again for unit u-3 only after this rank has passed wait(u-1), and a member
-        # publishes (u-1) only after its fold(u), the previous user of that buffer.
+        # in the order of the stagings: a buffer is written again for the third unit after u only when this rank has
+        # passed the wait for the first after u, which a member publishes only after its fold(u).  (By the units' indices the
+        # last unit of one backward pass and the head of the next can come to the same buffer with nothing in between.)
+        self._stage_next = -1
+        self._stage_of: Dict[int, int] = {}   # unit index -> buffer of its latest staging
         self.stage_slot = max((u.numel_local for u in store.units), default=0)
         self.stage_slot = (self.stage_slot + 7) // 8 * 8
         self.rs_stage = None
@@ -189,7 +192,7 @@ class SymmContext:
             all_stage = [int(p) + self.GUARD * self.wire_bytes for p in self._h_stage.buffer_ptrs]
             self.stage_ptrs = [all_stage[r] for r in mesh.shard.ranks]
         self.flags = torch.zeros(max(1, self.R) * 4096, dtype=torch.int32, device=dev)
-        self._rs_pending = None   # (unit, names, barrier token) of the unit whose fold is still to come
+        self._rs_pending = None   # (unit, names, buffer, barrier token) of the unit whose fold is still to come
         self._tables: Dict[tuple, torch.Tensor] = {}
         self._token = torch.zeros(1, dtype=torch.float32, device=dev)
         self._sync_group = world if mesh.replicate.size > 1 else mesh.shard.pg
@@ -216,8 +219,11 @@ class SymmContext:
 
     def stage_pointer_table(self, handle) -> torch.Tensor:
         """Device array: for every owner GPU r, the address inside r's staging buffer where THIS rank's contribution
-        to the row shard r of ``handle``'s gradient goes (buffer chosen by the parity of the unit index)."""
-        buf = handle.unit.index % self.N_STAGE
+        to the row shard r of ``handle``'s gradient goes (the next buffer in rotation with a unit's first weight)."""
+        if not handle.unit._staged:
+            self._stage_next = (self._stage_next + 1) % self.N_STAGE
+            self._stage_of[handle.unit.index] = self._stage_next
+        buf = self._stage_of[handle.unit.index]
         key = ("stage", handle.name, buf)
         t = self._tables.get(key)
         if t is None:
@@ -226,10 +232,9 @@ class SymmContext:
             self._tables[key] = t
         return t
 
-    def fold_stage(self, unit, names) -> None:
-        """accumulator += grad_scale * sum over the R slots of the unit's staging buffer, for the parameters in
+    def fold_stage(self, unit, names, buf: int) -> None:
+        """accumulator += grad_scale * sum over the R slots of staging buffer ``buf``, for the parameters of ``unit`` in
         ``names`` (those whose weight gradient was stored this pass; other regions of the slots hold stale data)."""
-        buf = unit.index % self.N_STAGE
         base = buf * self.R * self.stage_slot
         for h in unit.params:
             if h.name not in names:
@@ -255,14 +260,14 @@ class SymmContext:
         staging slots).  Folds the PREVIOUS unit's slots (waiting, normally without delay, for the members' epoch of
         that unit) and then publishes this unit's epoch; this unit is folded at the next call or by :meth:`rs_flush`."""
         self._fold_pending()
-        self._rs_pending = (unit, names, self._barrier.arrive())
+        self._rs_pending = (unit, names, self._stage_of[unit.index], self._barrier.arrive())
 
     def _fold_pending(self) -> None:
         if self._rs_pending is not None:
-            unit, names, token = self._rs_pending
+            unit, names, buf, token = self._rs_pending
             self._rs_pending = None
             self._barrier.wait(token)
-            self.fold_stage(unit, names)
+            self.fold_stage(unit, names, buf)
 
     def rs_flush(self) -> None:
         """Fold whatever is still staged (end of a backward pass)."""
