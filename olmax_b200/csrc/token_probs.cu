@@ -684,9 +684,10 @@ __device__ __forceinline__ double block_sum(double x, double* red) {
 // A row belongs to a cluster of C CTAs as in the log probabilities.  Thread t holds the teacher's pair t.  One bit of shared memory per vector, the
 // bits of a thread's batch side by side, says whether the teacher names one of its classes, one bit per class which: a batch without one, and
 // that is most of them, costs one look.
-// With 64 classes named, 2048 x 100352: fp32 140 us (5.9 TB/s, HBM), bf16 100 us (loads), with a soft-cap 144 us (instructions).
+// With 64 classes named, 2048 x 100352: fp32 140 us (5.9 TB/s, HBM), bf16 100 us (loads), with a soft-cap 133 us (instructions; 145 with five CTAs per SM
+// and no batch ahead).
 template <class T, int U, bool CAP>
-__global__ void __launch_bounds__(TP_THREADS, CAP ? 5 : 6)
+__global__ void __launch_bounds__(TP_THREADS, CAP ? 4 : 6)
     distill_fwd_kernel(const T* __restrict__ logits, long long ld, int C, int slice_vectors, DistillArgs p) {
   constexpr int N = Row<T>::N, E = U * N;
   extern __shared__ __align__(16) char shared_bytes[];
@@ -739,12 +740,15 @@ __global__ void __launch_bounds__(TP_THREADS, CAP ? 5 : 6)
   auto is_named = [&](int i) { return (named[(i + shift) >> 5] >> ((i + shift) & 31)) & 1; };
   const int single = r.single(threadIdx.x, part == 0, part == C - 1);
   if (single >= 0 && !is_named(single)) add_class(a, p.sc.capped(to_f(r.z[single])), p.sc);
+  uint4 v[U];
+  auto load = [&](int b) { load_batch<T, U>(r, b + threadIdx.x, b + TP_THREADS * U <= v1, v1, v); };
+  if (CAP) load(v0);   // (the next batch ahead: the instructions of this one hide it)
   for (int b = v0, batch = 0; b < v1; b += TP_THREADS * U, ++batch) {
-    uint4 v[U];
-    load_batch<T, U>(r, b + threadIdx.x, b + TP_THREADS * U <= v1, v1, v);
+    if (!CAP) load(b);
     float f[E];
 #pragma unroll
     for (int k = 0; k < U; ++k) unpack<T>(v[k], f + k * N);
+    if (CAP) load(b + TP_THREADS * U);
     if (CAP) p.sc.cap_logits(f);
     const int bit = (batch * TP_THREADS + threadIdx.x) * U;
     const unsigned some = (flags[bit >> 5] >> (bit & 31)) & ((1u << U) - 1);
